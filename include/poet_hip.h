@@ -58,8 +58,8 @@ extern "C" {
 
 #define POET_F32 0
 #define POET_BF16 1
-#define POET_F16 2   /* IEEE half STORAGE (11 significant bits in the same 2 bytes as bf16's 8): accepted only as the q_dtype of
-                        poet_msda_fused_fwd / _bwd -- the sampling offsets and attention logits, values of a few units that no GEMM
+#define POET_F16 2   /* IEEE half STORAGE (11 significant bits in the same 2 bytes as bf16's 8): accepted by poet_groupnorm_act_* and as
+                        the q_dtype of poet_msda_fused_fwd / _bwd -- the sampling offsets and attention logits, values of a few units that no GEMM
                         ever reads as an operand -- produced by poet_gemm with c_dtype = POET_BF16 and c_f16 = 1.  Gradients of
                         such a buffer are bf16. */
 
@@ -383,6 +383,27 @@ int poet_groupnorm_bwd(const void* dy, const void* x, const float* stats, const 
                        int N, int HW, int C, int G, int64_t x_off, int64_t x_stride,
                        int64_t y_off, int64_t y_stride, int dtype_x, int dtype_y,
                        float* scratch, int64_t scratch_floats, void* stream);
+
+/* GroupNorm with an activation on channels-last rows: x (N, HW, C) at image / row strides x_n / x_r (elements, channels contiguous),
+ * y likewise.  y = act(gamma h + beta), h = (x - mean) rstd over the HW x (C / G) values of (image, group); any C / G.
+ * act: POET_ACT_*.  Types of (x, y): (fp32, fp32), (bf16, bf16), (fp16, fp16), (bf16, fp32), (fp32, bf16); gamma / beta fp32 (C).
+ * stats (N, G, 2) fp32 = (mean, rstd): written by forward (optional there), read by backward, 8-byte aligned.
+ * y may be x itself.  Backward recomputes z = gamma h + beta: dx (optional; x's type) and dgamma / dbeta (optional, together; fp32 (C)),
+ * overwritten, or added to when `accumulate` != 0.  No atomics: results are bit-reproducible.
+ * workspace: caller-owned, poet_groupnorm_act_workspace(N, HW, C, G) bytes (negative: an error code), 8-byte aligned; contents
+ * undefined afterwards, not shared with a launch that may run at the same time. */
+#define POET_ACT_NONE 0
+#define POET_ACT_RELU 1
+#define POET_ACT_GELU 2 /* erf form */
+#define POET_ACT_SILU 3
+int64_t poet_groupnorm_act_workspace(int N, int HW, int C, int G);
+int poet_groupnorm_act_fwd(const void* x, int64_t x_n, int64_t x_r, const float* gamma, const float* beta, void* y, int64_t y_n, int64_t y_r,
+                           float* stats, int N, int HW, int C, int G, float eps, int act, int x_dtype, int y_dtype, void* workspace,
+                           int64_t workspace_bytes, void* stream);
+int poet_groupnorm_act_bwd(const void* dy, int64_t dy_n, int64_t dy_r, const void* x, int64_t x_n, int64_t x_r, const float* stats,
+                           const float* gamma, const float* beta, void* dx, int64_t dx_n, int64_t dx_r, float* dgamma, float* dbeta,
+                           int accumulate, int N, int HW, int C, int G, int act, int x_dtype, int y_dtype, void* workspace,
+                           int64_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------------------------------
  * Pose heads tail: rot_all (R, ncls*6), trans_all (R, ncls*3) fp32, cls (R,) int32 (<=0 -> slot 0)

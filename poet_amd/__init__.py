@@ -8,7 +8,7 @@ There is NO CPU / eager-PyTorch fallback: without the built library or without a
 from ._lib import PoetHipError, load as load_library  # noqa: F401
 from .modules import (BoundingBoxEmbeddingSine, DeformableTransformer, DeformableTransformerDecoder,  # noqa: F401
                       DeformableTransformerDecoderLayer, DeformableTransformerEncoder,
-                      DeformableTransformerEncoderLayer, MLP, MSDeformAttn, NestedTensor, PoET,
+                      DeformableTransformerEncoderLayer, GroupNormAct, MLP, MSDeformAttn, NestedTensor, PoET,
                       PositionEmbeddingLearned, PositionEmbeddingSine)
 from .engine import (BucketReducer, losses_for, GraphedTrainer, GraphedInference, ParamArena, PoseMatcher, SetCriterion, Trainer,  # noqa: F401
                      build_weight_dict, reduce_dict)

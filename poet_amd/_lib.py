@@ -76,6 +76,9 @@ _PROTOS = {
     "poet_col2im3x3s2_add": ([vp, vp, i32, i32, i32, i32, i32, i32, i64, i64, i32, i32, vp], i32),
     "poet_groupnorm_fwd": ([vp, vp, vp, vp, vp, i32, i32, i32, i32, i64, i64, i64, i64, f32, i32, i32, vp, i64, vp, vp], i32),
     "poet_groupnorm_bwd": ([vp, vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i64, i64, i64, i64, i32, i32, vp, i64, vp], i32),
+    "poet_groupnorm_act_workspace": ([i32, i32, i32, i32], i64),
+    "poet_groupnorm_act_fwd": ([vp, i64, i64, vp, vp, vp, i64, i64, vp, i32, i32, i32, i32, f32, i32, i32, i32, vp, i64, vp], i32),
+    "poet_groupnorm_act_bwd": ([vp, i64, i64, vp, i64, i64, vp, vp, vp, vp, i64, i64, vp, vp, i32, i32, i32, i32, i32, i32, i32, i32, vp, i64, vp], i32),
     "poet_pose_finish_fwd": ([vp, vp, vp, vp, vp, i32, i32, vp], i32),
     "poet_pose_finish_bwd": ([vp, vp, vp, vp, vp, vp, i32, i32, vp], i32),
     "poet_pose_loss": ([vp, vp, vp, vp, vp, i32, i32, i32, vp, vp, vp, vp, vp, vp, vp], i32),

@@ -1,0 +1,554 @@
+// GroupNorm with an activation on channels-last rows for gfx950, forward and backward.
+//
+//   forward :  m, v over the HW x (C / G) values of (image n, group g);  h = (x - m) / sqrt(v + eps);  y = act(gamma h + beta)
+//   backward:  z = gamma h + beta,  dz = dy act'(z);  dbeta = sum dz,  dgamma = sum dz h  (over n and the rows);
+//              dx = rstd (gamma dz - mean_g(gamma dz) - h mean_g(gamma dz h))
+//
+// Both are bound by HBM: a forward pass moves x in and y out, a backward pass x and dy in and dx out, plus one re-read for the
+// statistics.  Any C / G (a 16-byte vector of a row may span several groups: sums are kept per channel and folded into groups
+// at the end), any image / row strides, fp32 / bf16 / fp16.
+//
+// Two launches per direction, same grid in both (a chunk of rows x a slab of channels per workgroup, so the second launch finds
+// its chunk where the first one left it: in the L2 of its XCD or in the memory-side cache):
+//   1. partial sums of the chunk.  Forward: (mean, M2) per group -- a lane accumulates x - p and (x - p)^2 against its OWN first
+//      sample p of the channel (with n <= 64 samples per lane sum (x-p)^2 <= (n + 1) M2, so a lane loses at most n ulp whatever the
+//      mean / spread ratio or outliers are) and lanes / channels / chunks combine by the parallel-variance formula.
+//      Backward: sum dz and sum dz h per channel, and their gamma-weighted sums per group.
+//   2. every workgroup folds the partials of its image (a few KB out of L2) and streams its chunk once more.
+// Nothing is accumulated with atomics: results do not depend on the order of workgroups.
+#include "common.cuh"
+
+namespace poet {
+
+namespace {
+
+constexpr int NT = 256;
+
+struct GnaP {
+    const void* x; int64_t xn, xr;          // image / row strides in elements; channels are contiguous
+    const void* dy; int64_t dn, dr;
+    void* y; int64_t yn, yr;                // forward: y; backward: dx
+    const float* gamma;
+    const float* beta;
+    float* stats;                           // (N, G, 2) mean, rstd: written by forward, read by backward
+    float2* part;                           // (N, G, T * P) partials of a group
+    float2* cpart;                          // (N, T, C) backward: (sum dz, sum dz h) per channel
+    float* dgamma;
+    float* dbeta;
+    int N, HW, C, G, cpg;
+    int T, R;                               // row chunks of R rows
+    int nslab, gps, P, cpp;                 // slabs of gps whole groups (P == 1), or a group in P pieces of cpp channels
+    int tail;                               // backward, second launch: leading workgroups that reduce dgamma / dbeta
+    int accumulate;
+    float eps;
+};
+
+template <typename T, int V> __device__ __forceinline__ void ldv(const T* p, float* o) {
+    if constexpr (V == 1) o[0] = io<T>::ld(p);
+    else vec<T, V>::ld(p, o);
+}
+template <typename T, int V> __device__ __forceinline__ void stv(T* p, const float* o) {
+    if constexpr (V == 1) io<T>::st(p, o[0]);
+    else vec<T, V>::st(p, o);
+}
+
+// ---- activations (POET_ACT_*) -----------------------------------------------------------------------
+enum { A_NONE = 0, A_RELU = 1, A_GELU = 2, A_SILU = 3 };
+
+// Phi(-u) = e q(t), e = exp(-u^2 / 2), t = 1 / (1 + 0.3 u), u >= 0: a degree-8 relative minimax fit (1.5e-7) of
+// exp(u^2 / 2) erfc(u / sqrt 2) / 2 -- one exp and one reciprocal serve Phi AND the density of the backward pass, where erff alone
+// costs twice as many instructions and these kernels have ~30 per bf16 element before they stop being bound by HBM.
+__device__ __forceinline__ float gauss_cdf(float z, float& e) {
+    const float u = fabsf(z);
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.3f, u, 1.f));
+    e = __builtin_amdgcn_exp2f(-0.72134752f * u * u);
+    float q = 0.0356747722f;
+    q = fmaf(q, t, -0.157203075f);
+    q = fmaf(q, t, 0.206353494f);
+    q = fmaf(q, t, -0.0536836334f);
+    q = fmaf(q, t, 0.128561621f);
+    q = fmaf(q, t, 0.0999134936f);
+    q = fmaf(q, t, 0.120753956f);
+    q = fmaf(q, t, 0.119629299f);
+    q *= t * e;
+    return z < 0.f ? q : 1.f - q;
+}
+__device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504f * z)); }
+
+template <int ACT> __device__ __forceinline__ float act_f(float z) {
+    if constexpr (ACT == A_RELU) return z < 0.f ? 0.f : z;               // (a NaN stays one)
+    if constexpr (ACT == A_GELU) { float e; return z * gauss_cdf(z, e); }
+    if constexpr (ACT == A_SILU) return z * sigmoid(z);
+    return z;
+}
+template <int ACT> __device__ __forceinline__ float act_df(float z, float dy) {       // dy act'(z)
+    if constexpr (ACT == A_RELU) return z > 0.f ? dy : 0.f;
+    if constexpr (ACT == A_GELU) { float e; const float c = gauss_cdf(z, e); return dy * fmaf(z * 0.39894228f, e, c); }
+    if constexpr (ACT == A_SILU) { const float s = sigmoid(z); return dy * (s * fmaf(z, 1.f - s, 1.f)); }
+    return dy;
+}
+
+// ---- this workgroup's chunk and slab ------------------------------------------------------------------
+struct Blk {
+    int n, t, s, row0, row1;          // image, chunk, slab; rows [row0, row1)
+    int g0, ng, c0, Cs, cps, piece;   // first group, groups, first channel, channels, channels per group in this slab
+    int LPR, RP, r, l;                // lanes per row, rows per pass, this thread's row / lane
+    bool active;
+};
+template <int V> __device__ __forceinline__ Blk decode(const GnaP& p, int b) {
+    Blk k;
+    k.t = b % p.T;
+    const int q = b / p.T;
+    k.s = q % p.nslab;
+    k.n = q / p.nslab;
+    k.row0 = k.t * p.R;
+    k.row1 = min(p.HW, k.row0 + p.R);
+    if (p.P == 1) {
+        k.g0 = k.s * p.gps;
+        k.ng = min(p.G - k.g0, p.gps);
+        k.c0 = k.g0 * p.cpg;
+        k.cps = p.cpg;
+        k.Cs = k.ng * p.cpg;
+        k.piece = 0;
+    } else {
+        k.g0 = k.s / p.P;
+        k.piece = k.s - k.g0 * p.P;
+        k.ng = 1;
+        k.c0 = k.g0 * p.cpg + k.piece * p.cpp;
+        k.cps = k.Cs = min(p.cpp, p.cpg - k.piece * p.cpp);
+    }
+    k.LPR = k.Cs / V;
+    k.RP = NT / k.LPR;
+    k.r = threadIdx.x / k.LPR;
+    k.l = threadIdx.x - k.r * k.LPR;
+    k.active = k.r < k.RP;
+    return k;
+}
+
+// per-thread, per-channel values -> one sum per channel (chan) -> one per group of the slab (grp).  red: RP x Cs floats.
+template <int V> __device__ __forceinline__ void to_channels(const Blk& k, const float* v, float* red, float* chan) {
+    __syncthreads();
+    if (k.active)
+#pragma unroll
+        for (int i = 0; i < V; ++i) red[k.r * k.Cs + k.l * V + i] = v[i];
+    __syncthreads();
+    for (int c = threadIdx.x; c < k.Cs; c += NT) {
+        float s = 0.f;
+        for (int r = 0; r < k.RP; ++r) s += red[r * k.Cs + c];
+        chan[c] = s;
+    }
+    __syncthreads();
+}
+__device__ __forceinline__ float team_sum(float v, int team) {             // team: a power of two <= 64 of consecutive lanes
+    for (int o = team >> 1; o; o >>= 1) v += __shfl_xor(v, o, 64);
+    return v;
+}
+__device__ __forceinline__ int team_of(int ng) { return ng <= 4 ? 64 : 8; }
+__device__ __forceinline__ void to_groups(const Blk& k, const float* chan, float* grp) {
+    const int team = team_of(k.ng), per = NT / team, m = threadIdx.x & (team - 1);
+    for (int b = 0; b < k.ng; b += per) {
+        const int g = b + threadIdx.x / team;
+        float s = 0.f;
+        if (g < k.ng)
+            for (int c = m; c < k.cps; c += team) s += chan[g * k.cps + c];
+        s = team_sum(s, team);
+        if (g < k.ng && m == 0) grp[g] = s;
+    }
+    __syncthreads();
+}
+
+constexpr int ROWS_AHEAD = 4;      // vectors of a thread in flight
+
+// ---- forward, 1: (mean, M2) per group of the chunk ------------------------------------------------------
+template <typename TX, int V> __global__ __launch_bounds__(NT) void gna_stats_kernel(const GnaP p) {
+    __shared__ float red[NT * V], chan[NT * V], grp[NT * V], grp2[NT * V];
+    const Blk k = decode<V>(p, blockIdx.x);
+    const TX* x = (const TX*)p.x + k.n * p.xn + k.c0 + k.l * V;
+    float pv[V], S[V], Q[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) pv[i] = S[i] = Q[i] = 0.f;
+    int cnt = 0;
+    if (k.active) {
+        int row = k.row0 + k.r;
+        if (row < k.row1) ldv<TX, V>(x + (int64_t)row * p.xr, pv);
+        for (; row < k.row1; row += ROWS_AHEAD * k.RP) {
+            float v[ROWS_AHEAD][V];
+#pragma unroll
+            for (int u = 0; u < ROWS_AHEAD; ++u)
+                if (row + u * k.RP < k.row1) ldv<TX, V>(x + (int64_t)(row + u * k.RP) * p.xr, v[u]);
+#pragma unroll
+            for (int u = 0; u < ROWS_AHEAD; ++u)
+                if (row + u * k.RP < k.row1) {
+                    ++cnt;
+#pragma unroll
+                    for (int i = 0; i < V; ++i) {
+                        const float d = v[u][i] - pv[i];
+                        S[i] += d;
+                        Q[i] = fmaf(d, d, Q[i]);
+                    }
+                }
+        }
+    }
+    const float fc = (float)cnt, rc = cnt ? 1.f / fc : 0.f;
+    float w[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) w[i] = fmaf(fc, pv[i], S[i]);
+    to_channels<V>(k, w, red, chan);
+    to_groups(k, chan, grp);
+    const float inv = 1.f / ((float)(k.row1 - k.row0) * (float)k.cps);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const float d = k.active ? fmaf(S[i], rc, pv[i]) - grp[(k.l * V + i) / k.cps] * inv : 0.f;
+        w[i] = fmaf(-S[i] * rc, S[i], Q[i]) + fc * d * d;
+    }
+    to_channels<V>(k, w, red, chan);
+    to_groups(k, chan, grp2);
+    for (int g = threadIdx.x; g < k.ng; g += NT)
+        p.part[(((int64_t)k.n * p.G + k.g0 + g) * p.T + k.t) * p.P + k.piece] = make_float2(grp[g] * inv, fmaxf(grp2[g], 0.f));
+}
+
+// ---- forward, 2: fold the chunks, normalise, activate ----------------------------------------------------
+template <typename TX, typename TY, int V, int ACT>
+__device__ __forceinline__ void apply_rows(const GnaP& p, const Blk& k, const float* mean, const float* sc, const float* sh) {
+    const TX* x = (const TX*)p.x + k.n * p.xn + k.c0 + k.l * V;
+    TY* y = (TY*)p.y + k.n * p.yn + k.c0 + k.l * V;
+    for (int row = k.row0 + k.r; row < k.row1; row += ROWS_AHEAD * k.RP) {
+        float v[ROWS_AHEAD][V];
+#pragma unroll
+        for (int u = 0; u < ROWS_AHEAD; ++u)
+            if (row + u * k.RP < k.row1) ldv<TX, V>(x + (int64_t)(row + u * k.RP) * p.xr, v[u]);
+#pragma unroll
+        for (int u = 0; u < ROWS_AHEAD; ++u)
+            if (row + u * k.RP < k.row1) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) v[u][i] = act_f<ACT>(fmaf(v[u][i] - mean[i], sc[i], sh[i]));
+                stv<TY, V>(y + (int64_t)(row + u * k.RP) * p.yr, v[u]);
+            }
+    }
+}
+
+template <typename TX, typename TY, int V, int ACT> __global__ __launch_bounds__(NT) void gna_apply_kernel(const GnaP p) {
+    __shared__ float gm[NT * V], gr[NT * V];
+    const Blk k = decode<V>(p, blockIdx.x);
+    const int team = team_of(k.ng), per = NT / team, m = threadIdx.x & (team - 1), E = p.T * p.P;
+    const float total = (float)p.HW * (float)p.cpg;
+    for (int b = 0; b < k.ng; b += per) {
+        const int g = b + threadIdx.x / team;
+        const float2* e = p.part + ((int64_t)k.n * p.G + k.g0 + (g < k.ng ? g : 0)) * E;
+        auto weight = [&](int i) {
+            const int t = i / p.P, q = i - t * p.P;
+            return (float)(min(p.HW, (t + 1) * p.R) - t * p.R) * (float)(p.P == 1 ? p.cpg : min(p.cpp, p.cpg - q * p.cpp));
+        };
+        const float m0 = e[0].x;
+        float s = 0.f;
+        for (int i = m; i < E; i += team) s = fmaf(weight(i), e[i].x - m0, s);
+        const float mean = m0 + team_sum(s, team) / total;
+        float q = 0.f;
+        for (int i = m; i < E; i += team) {
+            const float d = e[i].x - mean;
+            q += fmaf(weight(i) * d, d, e[i].y);
+        }
+        const float rstd = 1.f / sqrtf(team_sum(q, team) / total + p.eps);
+        if (g < k.ng && m == 0) {
+            gm[g] = mean;
+            gr[g] = rstd;
+            if (k.t == 0 && k.piece == 0 && p.stats) *reinterpret_cast<float2*>(p.stats + 2 * ((int64_t)k.n * p.G + k.g0 + g)) = make_float2(mean, rstd);
+        }
+    }
+    __syncthreads();
+    if (!k.active) return;
+    float mean[V], sc[V], sh[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const int c = k.l * V + i, g = c / k.cps;
+        mean[i] = gm[g];
+        sc[i] = p.gamma[k.c0 + c] * gr[g];
+        sh[i] = p.beta[k.c0 + c];
+    }
+    apply_rows<TX, TY, V, ACT>(p, k, mean, sc, sh);
+}
+
+// ---- backward, 1: sum dz and sum dz h per channel, gamma-weighted per group ---------------------------------
+struct Chan { float mean, rstd, gamma, beta; };
+template <int V> __device__ __forceinline__ void load_chan(const GnaP& p, const Blk& k, Chan* ch) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const int c = k.l * V + i, g = k.g0 + c / k.cps;
+        const float2 st = *reinterpret_cast<const float2*>(p.stats + 2 * ((int64_t)k.n * p.G + g));
+        ch[i] = {st.x, st.y, p.gamma[k.c0 + c], p.beta[k.c0 + c]};
+    }
+}
+
+template <typename TX, typename TY, int V, int ACT> __global__ __launch_bounds__(NT) void gna_bwd_stats_kernel(const GnaP p) {
+    __shared__ float red[NT * V], chan[NT * V], chan2[NT * V], grp[NT * V], grp2[NT * V];
+    const Blk k = decode<V>(p, blockIdx.x);
+    float a[V], b[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) a[i] = b[i] = 0.f;
+    if (k.active) {
+        Chan ch[V];
+        load_chan<V>(p, k, ch);
+        const TX* x = (const TX*)p.x + k.n * p.xn + k.c0 + k.l * V;
+        const TY* dy = (const TY*)p.dy + k.n * p.dn + k.c0 + k.l * V;
+        for (int row = k.row0 + k.r; row < k.row1; row += ROWS_AHEAD * k.RP) {
+            float v[ROWS_AHEAD][V], w[ROWS_AHEAD][V];
+#pragma unroll
+            for (int u = 0; u < ROWS_AHEAD; ++u)
+                if (row + u * k.RP < k.row1) {
+                    ldv<TX, V>(x + (int64_t)(row + u * k.RP) * p.xr, v[u]);
+                    ldv<TY, V>(dy + (int64_t)(row + u * k.RP) * p.dr, w[u]);
+                }
+#pragma unroll
+            for (int u = 0; u < ROWS_AHEAD; ++u)
+                if (row + u * k.RP < k.row1)
+#pragma unroll
+                    for (int i = 0; i < V; ++i) {
+                        const float h = (v[u][i] - ch[i].mean) * ch[i].rstd;
+                        const float dz = act_df<ACT>(fmaf(h, ch[i].gamma, ch[i].beta), w[u][i]);
+                        a[i] += dz;
+                        b[i] = fmaf(dz, h, b[i]);
+                    }
+        }
+    }
+    to_channels<V>(k, a, red, chan);
+    to_channels<V>(k, b, red, chan2);
+    float2* cp = p.cpart + ((int64_t)k.n * p.T + k.t) * p.C + k.c0;
+    for (int c = threadIdx.x; c < k.Cs; c += NT) {
+        const float g = p.gamma[k.c0 + c];
+        cp[c] = make_float2(chan[c], chan2[c]);
+        chan[c] *= g;
+        chan2[c] *= g;
+    }
+    __syncthreads();
+    to_groups(k, chan, grp);
+    to_groups(k, chan2, grp2);
+    for (int g = threadIdx.x; g < k.ng; g += NT)
+        p.part[(((int64_t)k.n * p.G + k.g0 + g) * p.T + k.t) * p.P + k.piece] = make_float2(grp[g], grp2[g]);
+}
+
+// ---- backward, 2: dx of the chunk; the first p.tail workgroups reduce dgamma / dbeta of 16 channels each -------
+__device__ __forceinline__ void reduce_params(const GnaP& p, int b) {
+    __shared__ double ra[16][17], rb[16][17];
+    const int c = threadIdx.x & 15, r = threadIdx.x >> 4, cc = b * 16 + c;
+    double sa = 0.0, sb = 0.0;
+    const int E = p.N * p.T;
+    if (cc < p.C) {
+#pragma unroll 8
+        for (int e = r; e < E; e += 16) {
+            const float2 v = p.cpart[(int64_t)e * p.C + cc];
+            sa += v.x;
+            sb += v.y;
+        }
+    }
+    ra[r][c] = sa;
+    rb[r][c] = sb;
+    __syncthreads();
+    if (r == 0 && cc < p.C) {
+        for (int i = 1; i < 16; ++i) sa += ra[i][c], sb += rb[i][c];
+        p.dbeta[cc] = (p.accumulate ? p.dbeta[cc] : 0.f) + (float)sa;
+        p.dgamma[cc] = (p.accumulate ? p.dgamma[cc] : 0.f) + (float)sb;
+    }
+}
+
+template <typename TX, typename TY, int V, int ACT> __global__ __launch_bounds__(NT) void gna_bwd_apply_kernel(const GnaP p) {
+    if ((int)blockIdx.x < p.tail) return reduce_params(p, blockIdx.x);
+    __shared__ float g1[NT * V], g2[NT * V];
+    const Blk k = decode<V>(p, blockIdx.x - p.tail);
+    const int team = team_of(k.ng), per = NT / team, m = threadIdx.x & (team - 1), E = p.T * p.P;
+    const float inv = 1.f / ((float)p.HW * (float)p.cpg);
+    for (int b = 0; b < k.ng; b += per) {
+        const int g = b + threadIdx.x / team;
+        const float2* e = p.part + ((int64_t)k.n * p.G + k.g0 + (g < k.ng ? g : 0)) * E;
+        float s1 = 0.f, s2 = 0.f;
+        for (int i = m; i < E; i += team) s1 += e[i].x, s2 += e[i].y;
+        s1 = team_sum(s1, team);
+        s2 = team_sum(s2, team);
+        if (g < k.ng && m == 0) g1[g] = s1 * inv, g2[g] = s2 * inv;
+    }
+    __syncthreads();
+    if (!k.active) return;
+    Chan ch[V];
+    load_chan<V>(p, k, ch);
+    float k2[V], k3[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const int g = (k.l * V + i) / k.cps;
+        k2[i] = -ch[i].rstd * g1[g];
+        k3[i] = -ch[i].rstd * g2[g];
+    }
+    const TX* x = (const TX*)p.x + k.n * p.xn + k.c0 + k.l * V;
+    const TY* dy = (const TY*)p.dy + k.n * p.dn + k.c0 + k.l * V;
+    TX* dx = (TX*)p.y + k.n * p.yn + k.c0 + k.l * V;
+    for (int row = k.row0 + k.r; row < k.row1; row += ROWS_AHEAD * k.RP) {
+        float v[ROWS_AHEAD][V], w[ROWS_AHEAD][V];
+#pragma unroll
+        for (int u = 0; u < ROWS_AHEAD; ++u)
+            if (row + u * k.RP < k.row1) {
+                ldv<TX, V>(x + (int64_t)(row + u * k.RP) * p.xr, v[u]);
+                ldv<TY, V>(dy + (int64_t)(row + u * k.RP) * p.dr, w[u]);
+            }
+#pragma unroll
+        for (int u = 0; u < ROWS_AHEAD; ++u)
+            if (row + u * k.RP < k.row1) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    const float h = (v[u][i] - ch[i].mean) * ch[i].rstd;
+                    const float dz = act_df<ACT>(fmaf(h, ch[i].gamma, ch[i].beta), w[u][i]);
+                    v[u][i] = fmaf(ch[i].gamma * ch[i].rstd, dz, fmaf(k3[i], h, k2[i]));
+                }
+                stv<TX, V>(dx + (int64_t)(row + u * k.RP) * p.yr, v[u]);
+            }
+    }
+}
+
+// ---- host ----------------------------------------------------------------------------------------------
+bool aligned16(const void* p, int64_t a, int64_t b, int esz) { return ((uintptr_t)p % 16) == 0 && (a * esz) % 16 == 0 && (b * esz) % 16 == 0; }
+int esize(int dt) { return dt == POET_F32 ? 4 : 2; }
+
+// slabs and chunks for vectors of V elements; false: the channel layout does not split into such vectors
+bool plan(GnaP& p, int V) {
+    const int maxc = NT * V;
+    if (p.C % V) return false;
+    int gv = V;                                             // groups per slab: a multiple of gv keeps slab starts on vectors
+    while (gv > 1 && (gv / 2 * (int64_t)p.cpg) % V == 0) gv /= 2;
+    if ((int64_t)gv * p.cpg <= maxc || p.C <= maxc) {
+        p.P = 1;
+        p.cpp = p.cpg;
+        if (p.C <= maxc) p.gps = p.G;
+        else {
+            const int most = maxc / p.cpg / gv * gv, n = cdiv(p.G, most);
+            p.gps = cdiv(cdiv(p.G, n), gv) * gv;
+        }
+        p.nslab = cdiv(p.G, p.gps);
+    } else {
+        if (p.cpg % V) return false;
+        p.cpp = cdiv(cdiv(p.cpg, cdiv(p.cpg, maxc)), V) * V;
+        p.P = cdiv(p.cpg, p.cpp);
+        p.gps = 1;
+        p.nslab = p.G * p.P;
+    }
+    // chunks: ~1024 workgroups (4 per CU), 8 .. 64 rows per lane
+    const int cs = p.P == 1 ? p.gps * p.cpg : p.cpp, rp = NT / (cs / V);
+    const int64_t want = 1024 / ((int64_t)p.N * p.nslab) + 1;
+    int64_t rows = (p.HW + want - 1) / want;
+    rows = (rows + rp - 1) / rp * rp;
+    if (rows < 8 * rp) rows = 8 * rp;
+    if (rows > 64 * rp) rows = 64 * rp;
+    p.R = (int)rows;
+    p.T = cdiv(p.HW, p.R);
+    return true;
+}
+
+int64_t ws_need(const GnaP& p, bool bwd) { return 8 * ((int64_t)p.N * p.G * p.T * p.P + (bwd ? (int64_t)p.N * p.T * p.C : 0)); }
+
+template <template <typename, typename, int, int> class L, typename TX, typename TY, int V> void by_act(const GnaP& p, int act, hipStream_t s) {
+    if (act == A_NONE) L<TX, TY, V, A_NONE>::go(p, s);
+    else if (act == A_RELU) L<TX, TY, V, A_RELU>::go(p, s);
+    else if (act == A_GELU) L<TX, TY, V, A_GELU>::go(p, s);
+    else L<TX, TY, V, A_SILU>::go(p, s);
+}
+template <template <typename, typename, int, int> class L, typename TX, typename TY> void by_vec(const GnaP& p, int act, bool wide, hipStream_t s) {
+    if (wide) by_act<L, TX, TY, 16 / (int)sizeof(TX)>(p, act, s);
+    else by_act<L, TX, TY, 1>(p, act, s);
+}
+// x and y of one type, or one of them fp32
+template <template <typename, typename, int, int> class L> bool by_type(const GnaP& p, int xt, int yt, int act, bool wide, hipStream_t s) {
+    if (xt == POET_F32 && yt == POET_F32) by_vec<L, float, float>(p, act, wide, s);
+    else if (xt == POET_BF16 && yt == POET_BF16) by_vec<L, bf16_t, bf16_t>(p, act, wide, s);
+    else if (xt == POET_F16 && yt == POET_F16) by_vec<L, f16_t, f16_t>(p, act, wide, s);
+    else if (xt == POET_BF16 && yt == POET_F32) by_vec<L, bf16_t, float>(p, act, wide, s);
+    else if (xt == POET_F32 && yt == POET_BF16) by_vec<L, float, bf16_t>(p, act, wide, s);
+    else return false;
+    return true;
+}
+int blocks(const GnaP& p) { return p.N * p.nslab * p.T; }
+
+template <typename TX, typename TY, int V, int ACT> struct Fwd {
+    static void go(const GnaP& p, hipStream_t s) {
+        hipLaunchKernelGGL((gna_stats_kernel<TX, V>), dim3(blocks(p)), dim3(NT), 0, s, p);
+        hipLaunchKernelGGL((gna_apply_kernel<TX, TY, V, ACT>), dim3(blocks(p)), dim3(NT), 0, s, p);
+    }
+};
+template <typename TX, typename TY, int V, int ACT> struct Bwd {
+    static void go(const GnaP& p, hipStream_t s) {
+        hipLaunchKernelGGL((gna_bwd_stats_kernel<TX, TY, V, ACT>), dim3(blocks(p)), dim3(NT), 0, s, p);
+        const int main = p.y ? blocks(p) : 0;
+        if (main + p.tail) hipLaunchKernelGGL((gna_bwd_apply_kernel<TX, TY, V, ACT>), dim3(main + p.tail), dim3(NT), 0, s, p);
+    }
+};
+
+// the part of the checks and of the plan that both directions share; returns POET_OK or an error
+int setup(GnaP& p, const char* what, int N, int HW, int C, int G, int act, int x_dtype, int y_dtype, bool wide_ok, void* ws, int64_t ws_bytes, bool bwd, bool& wide) {
+    POET_CHECK(N > 0 && HW > 0 && C > 0 && G > 0 && C % G == 0, POET_ERR_ARG, "%s: bad dims (N %d, HW %d, C %d, G %d)", what, N, HW, C, G);
+    POET_CHECK(act >= A_NONE && act <= A_SILU, POET_ERR_ARG, "%s: unknown activation %d", what, act);
+    POET_CHECK(C <= (1 << 20) && HW <= (1 << 30), POET_ERR_UNSUPPORTED, "%s: C > 2^20 or HW > 2^30", what);
+    p.N = N; p.HW = HW; p.C = C; p.G = G; p.cpg = C / G;
+    wide = wide_ok && plan(p, x_dtype == POET_F32 ? 4 : 8);
+    if (!wide) plan(p, 1);
+    POET_CHECK((int64_t)N * p.nslab * p.T < (1ll << 30), POET_ERR_UNSUPPORTED, "%s: too many row chunks", what);
+    const int64_t need = ws_need(p, bwd);
+    POET_CHECK(ws && ((uintptr_t)ws % 8) == 0 && ws_bytes >= need, POET_ERR_ARG, "%s: workspace of %lld bytes needed (8-byte aligned), %lld given", what,
+               (long long)need, (long long)ws_bytes);
+    p.part = (float2*)ws;
+    p.cpart = p.part + (int64_t)N * G * p.T * p.P;
+    return POET_OK;
+}
+
+}  // namespace
+
+}  // namespace poet
+
+using namespace poet;
+
+extern "C" int64_t poet_groupnorm_act_workspace(int N, int HW, int C, int G) {
+    POET_CHECK(N > 0 && HW > 0 && C > 0 && G > 0 && C % G == 0 && C <= (1 << 20) && HW <= (1 << 30), POET_ERR_ARG, "groupnorm_act: bad dims (N %d, HW %d, C %d, G %d)", N, HW, C, G);
+    int64_t need = 0;
+    for (int V : {1, 4, 8}) {                                // the largest of the layouts the launch may choose
+        GnaP p = {};
+        p.N = N; p.HW = HW; p.C = C; p.G = G; p.cpg = C / G;
+        if (plan(p, V)) need = ws_need(p, true) > need ? ws_need(p, true) : need;
+    }
+    return need;
+}
+
+extern "C" int poet_groupnorm_act_fwd(const void* x, int64_t x_n, int64_t x_r, const float* gamma, const float* beta, void* y, int64_t y_n, int64_t y_r,
+                                      float* stats, int N, int HW, int C, int G, float eps, int act, int x_dtype, int y_dtype, void* workspace,
+                                      int64_t workspace_bytes, void* stream) {
+    POET_CHECK(x && gamma && beta && y, POET_ERR_ARG, "groupnorm_act_fwd: null pointer");
+    GnaP p = {};
+    bool wide = false;
+    const int rc = setup(p, "groupnorm_act_fwd", N, HW, C, G, act, x_dtype, y_dtype,
+                         aligned16(x, x_n, x_r, esize(x_dtype)) && aligned16(y, y_n, y_r, esize(y_dtype)), workspace, workspace_bytes, false, wide);
+    if (rc != POET_OK) return rc;
+    POET_CHECK(!stats || ((uintptr_t)stats % 8) == 0, POET_ERR_ARG, "groupnorm_act_fwd: stats must be 8-byte aligned");
+    p.x = x; p.xn = x_n; p.xr = x_r;
+    p.y = y; p.yn = y_n; p.yr = y_r;
+    p.gamma = gamma; p.beta = beta; p.stats = stats; p.eps = eps;
+    POET_CHECK(by_type<Fwd>(p, x_dtype, y_dtype, act, wide, (hipStream_t)stream), POET_ERR_UNSUPPORTED, "groupnorm_act_fwd: dtypes %d -> %d", x_dtype, y_dtype);
+    POET_LAUNCH_CHECK();
+    return POET_OK;
+}
+
+extern "C" int poet_groupnorm_act_bwd(const void* dy, int64_t dy_n, int64_t dy_r, const void* x, int64_t x_n, int64_t x_r, const float* stats,
+                                      const float* gamma, const float* beta, void* dx, int64_t dx_n, int64_t dx_r, float* dgamma, float* dbeta,
+                                      int accumulate, int N, int HW, int C, int G, int act, int x_dtype, int y_dtype, void* workspace,
+                                      int64_t workspace_bytes, void* stream) {
+    POET_CHECK(dy && x && stats && gamma && beta, POET_ERR_ARG, "groupnorm_act_bwd: null pointer");
+    POET_CHECK((dgamma == nullptr) == (dbeta == nullptr) && (dx || dgamma), POET_ERR_ARG, "groupnorm_act_bwd: dgamma and dbeta go together, and something must be asked for");
+    POET_CHECK(((uintptr_t)stats % 8) == 0, POET_ERR_ARG, "groupnorm_act_bwd: stats must be 8-byte aligned");
+    GnaP p = {};
+    bool wide = false;
+    const int rc = setup(p, "groupnorm_act_bwd", N, HW, C, G, act, x_dtype, y_dtype,
+                         aligned16(x, x_n, x_r, esize(x_dtype)) && aligned16(dy, dy_n, dy_r, esize(y_dtype)) && (!dx || aligned16(dx, dx_n, dx_r, esize(x_dtype))),
+                         workspace, workspace_bytes, true, wide);
+    if (rc != POET_OK) return rc;
+    p.x = x; p.xn = x_n; p.xr = x_r;
+    p.dy = dy; p.dn = dy_n; p.dr = dy_r;
+    p.y = dx; p.yn = dx_n; p.yr = dx_r;
+    p.gamma = gamma; p.beta = beta; p.stats = const_cast<float*>(stats);
+    p.dgamma = dgamma; p.dbeta = dbeta; p.accumulate = accumulate;
+    p.tail = dgamma ? cdiv(C, 16) : 0;
+    POET_CHECK(by_type<Bwd>(p, x_dtype, y_dtype, act, wide, (hipStream_t)stream), POET_ERR_UNSUPPORTED, "groupnorm_act_bwd: dtypes %d, %d", x_dtype, y_dtype);
+    POET_LAUNCH_CHECK();
+    return POET_OK;
+}

@@ -166,6 +166,23 @@ class BoundingBoxEmbeddingSine(nn.Module):
         return out
 
 
+class GroupNormAct(nn.GroupNorm):
+    """nn.GroupNorm + activation over channels-LAST input (N, ..., C), one operator (same state_dict keys as nn.GroupNorm).
+    act: "none", "relu", "gelu", "silu"."""
+
+    def __init__(self, num_groups, num_channels, act="none", eps=1e-5):
+        if act not in ops.ACT:
+            raise ValueError(f"activation must be one of {sorted(ops.ACT)}, got {act!r}")
+        super().__init__(num_groups, num_channels, eps=eps)
+        self.act = act
+
+    def forward(self, x):
+        return Fn.group_norm_act(x, self.weight, self.bias, self.num_groups, act=self.act, eps=self.eps)
+
+    def extra_repr(self):
+        return f"{super().extra_repr()}, act={self.act}"
+
+
 def _check_activation(name):
     """deformable_transformer.py:347-355 (`_get_activation_fn`): "relu" / "gelu" / "glu", anything else raises RuntimeError at
     construction.  "glu" halves the hidden width, so the reference's own forward fails in linear2 (d_ffn / 2 columns against a

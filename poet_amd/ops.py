@@ -527,6 +527,120 @@ def groupnorm_bwd(dy, x, stats, gamma, dx, dgamma, dbeta, N, HW, Cc, G, x_off, x
                "poet_groupnorm_bwd")
 
 
+ACT = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}          # POET_ACT_*
+
+
+class _on_device:
+    """Launch context of the operators that allocate their own workspace: `with _on_device(t) as stream:` makes t's device current
+    (when it is not) and gives the raw handle of THAT device's current stream."""
+
+    def __init__(self, t):
+        self.dev = t.device.index
+        self.guard = None if self.dev == torch.cuda.current_device() else torch.cuda.device(self.dev)
+
+    def __enter__(self):
+        if self.guard is None:
+            return _stream()
+        self.guard.__enter__()
+        return torch.cuda.current_stream().cuda_stream
+
+    def __exit__(self, *exc):
+        return self.guard.__exit__(*exc) if self.guard is not None else False
+
+
+def _rows3(t: torch.Tensor, name: str, N: int, HW: int, C: int, out: bool = False):
+    """(image stride, row stride) of a channels-last (N, HW, C) tensor; an output must not write an element twice."""
+    if t.dim() != 3 or tuple(t.shape) != (N, HW, C):
+        raise ValueError(f"poet_amd: {name} must be ({N}, {HW}, {C}), got {tuple(t.shape)}")
+    if t.numel() == 0:
+        return 0, 0
+    if C > 1 and t.stride(2) != 1:
+        raise ValueError(f"poet_amd: {name} must hold its channels contiguously (stride {t.stride(2)})")
+    n, r = t.stride(0) if N > 1 else 0, t.stride(1) if HW > 1 else 0
+    if out and not ((HW == 1 or r >= C) and (N == 1 or n >= (HW - 1) * r + C) or (N == 1 or n >= C) and (HW == 1 or r >= (N - 1) * n + C)):
+        raise ValueError(f"poet_amd: rows of the output {name} overlap (strides {n}, {r})")
+    return n, r
+
+
+def _chan_params(x, C, G, **params):
+    if G <= 0 or C % G:
+        raise ValueError(f"poet_amd: {C} channels do not split into {G} groups")
+    for k, t in params.items():
+        if t is None:
+            continue
+        if t.dtype != torch.float32 or t.numel() != C or not t.is_contiguous():
+            raise ValueError(f"poet_amd: {k} must be a contiguous fp32 tensor of {C} elements")
+        if t.device != x.device:
+            raise ValueError(f"poet_amd: {k} lives on {t.device}, x on {x.device}")
+
+
+def _act_code(act):
+    try:
+        return ACT[act]
+    except KeyError:
+        raise ValueError(f"poet_amd: activation must be one of {sorted(ACT)}, got {act!r}") from None
+
+
+def groupnorm_act_fwd(x, gamma, beta, y, G, act="none", stats=None, eps=1e-5):
+    """y = act(gamma (x - mean) rstd + beta), statistics over the rows and the C / G channels of each (image, group).  x, y (N, HW, C) with
+    contiguous channels, any image / row strides (a level's rows of a token buffer); types: equal (fp32, bf16, fp16), or fp32 with bf16.
+    stats: optional (N, G, 2) fp32 output (mean, rstd), what groupnorm_act_bwd reads.  y may be x."""
+    lib = _lib.load()
+    _req(x, "x")
+    if x.dim() != 3:
+        raise ValueError(f"poet_amd: x must be (N, HW, C), got {tuple(x.shape)}")
+    N, HW, C = x.shape
+    _chan_params(x, C, G, gamma=gamma, beta=beta)
+    (xn, xr), (yn, yr) = _rows3(x, "x", N, HW, C), _rows3(y, "y", N, HW, C, out=True)
+    xd, yd, a = dcode(x), dcode(y), _act_code(act)
+    if y.device != x.device or stats is not None and (stats.device != x.device or stats.dtype != torch.float32 or not stats.is_contiguous() or stats.numel() != 2 * N * G):
+        raise ValueError("poet_amd: y and stats must live on x's device, stats as a contiguous fp32 (N, G, 2) tensor")
+    if x.numel() == 0:
+        return y
+    with _on_device(x) as stream:
+        ws = torch.empty(_gna_ws(lib, N, HW, C, G), dtype=torch.uint8, device=x.device)
+        _lib.check(lib.poet_groupnorm_act_fwd(x.data_ptr(), xn, xr, gamma.data_ptr(), beta.data_ptr(), y.data_ptr(), yn, yr, _ptr(stats), N, HW, C, G,
+                                              eps, a, xd, yd, ws.data_ptr(), ws.numel(), stream), "poet_groupnorm_act_fwd")
+    return y
+
+
+def _gna_ws(lib, N, HW, C, G):
+    n = lib.poet_groupnorm_act_workspace(N, HW, C, G)
+    if n < 0:
+        _lib.check(int(n), "poet_groupnorm_act_workspace")
+    return n
+
+
+def groupnorm_act_bwd(dy, x, stats, gamma, beta, G, act="none", dx=None, dgamma=None, dbeta=None, accumulate=False):
+    """Gradients of groupnorm_act_fwd from its input and stats (z is recomputed): dx in x's type, dgamma / dbeta fp32, overwritten or
+    (accumulate) added to.  Any of them may be left out (dgamma and dbeta together)."""
+    lib = _lib.load()
+    _req(x, "x")
+    if x.dim() != 3:
+        raise ValueError(f"poet_amd: x must be (N, HW, C), got {tuple(x.shape)}")
+    N, HW, C = x.shape
+    _chan_params(x, C, G, gamma=gamma, beta=beta, dgamma=dgamma, dbeta=dbeta)
+    (xn, xr), (dn, dr) = _rows3(x, "x", N, HW, C), _rows3(dy, "dy", N, HW, C)
+    on, orow = (0, 0) if dx is None else _rows3(dx, "dx", N, HW, C, out=True)
+    if dx is not None and (dx.dtype != x.dtype or dx.device != x.device) or dy.device != x.device:
+        raise ValueError("poet_amd: dx has x's type, and dy, dx live on x's device")
+    if stats.dtype != torch.float32 or stats.device != x.device or not stats.is_contiguous() or stats.numel() != 2 * N * G:
+        raise ValueError("poet_amd: stats must be the contiguous fp32 (N, G, 2) tensor of the forward pass")
+    if (dgamma is None) != (dbeta is None):
+        raise ValueError("poet_amd: dgamma and dbeta go together")
+    xd, yd, a = dcode(x), dcode(dy), _act_code(act)
+    if x.numel() == 0 or dx is None and dgamma is None:
+        if dgamma is not None and not accumulate:
+            dgamma.zero_(), dbeta.zero_()
+        return dx, dgamma, dbeta
+    with _on_device(x) as stream:
+        ws = torch.empty(_gna_ws(lib, N, HW, C, G), dtype=torch.uint8, device=x.device)
+        _lib.check(lib.poet_groupnorm_act_bwd(dy.data_ptr(), dn, dr, x.data_ptr(), xn, xr, stats.data_ptr(), gamma.data_ptr(), beta.data_ptr(),
+                                              _ptr(dx), on, orow, _ptr(dgamma), _ptr(dbeta), int(accumulate), N, HW, C, G, a, xd, yd, ws.data_ptr(),
+                                              ws.numel(), stream), "poet_groupnorm_act_bwd")
+    return dx, dgamma, dbeta
+
+
 # ---- attention -------------------------------------------------------------------------------------
 def mha_fwd(q, k, v, ld, out, ld_out, N, Q, M, hd, drop_p=0.0, seed=0):
     lib = _lib.load()
@@ -833,6 +947,7 @@ def _instrument(name, tag):
 
 for _n, _t in [("msda_fused_fwd", "msda_fused_fwd"), ("ln_fwd", "ln_fwd"), ("ln_bwd", "ln_bwd"),
                ("colsum", "colsum"), ("vgrad_to_rows", "vgrad_to_rows"), ("add", "add"), ("cast", "cast"),
-               ("groupnorm_fwd", "groupnorm"), ("groupnorm_bwd", "groupnorm"), ("mha_fwd", "mha"), ("mha_bwd", "mha"),
+               ("groupnorm_fwd", "groupnorm"), ("groupnorm_bwd", "groupnorm"),
+               ("groupnorm_act_fwd", "groupnorm_act"), ("groupnorm_act_bwd", "groupnorm_act"), ("mha_fwd", "mha"), ("mha_bwd", "mha"),
                ("pos_sine", "pos_sine"), ("adamw", "adamw"), ("sqnorm", "sqnorm")]:
     _instrument(_n, _t)
