@@ -456,6 +456,32 @@ int poet_adamw(float* p, const float* g, float* m, float* v, uint16_t* p_bf16, u
                const float* lr_scale /* optional: lr multiplier per block of 64 elements, ceil(n/64) floats (the 0.1x group of
                                         main.py:41,253-271 inside one contiguous range) */,
                void* stream);
+/* ------------------------------------------------------------------------------------------------
+ * Orthogonalised updates of weight matrices (the Muon optimiser), a LIST of n matrices of any shapes in one chain of launches.
+ * Matrix i is rows[i] x cols[i] (1 .. 2^20 each).  With u the input (orthogonalize) or the update direction (muon_step):
+ *     X = u / (||u||_F + eps), turned so that rows <= cols;  steps times: A = X X^T, X <- (a I + b A + c A^2) X;  result X, turned back.
+ * coeffs_host: steps x (a, b, c), 1 <= steps <= 16; coefficients under which the scalar iteration leaves |x| < 1e3 on [0, 1] are refused.
+ * Products run on fp16 hi + lo operands (22 bits) with fp32 sums: the error of fp32 products.  A matrix with a NaN or an infinity comes
+ * out all NaN, the others of the list are untouched by it.  No atomics: bit-reproducible, and independent of the rest of the list.
+ * Lists and coefficients are host arrays, read before the call returns; matrices must not overlap, except that an output may be its
+ * own input.  workspace: poet_muon_workspace(rows, cols, n) bytes (negative: an error code), 256-byte aligned, not shared with a launch
+ * that may run at the same time.
+ *
+ * poet_orthogonalize: o[i] = orthogonalised g[i]; row strides ldg / ldo in elements; types POET_F32 / BF16 / F16.
+ * poet_muon_step (fp32, contiguous): g' = g grad_scale [x min(1, max_norm / (sqrt(*sqnorm) grad_scale + 1e-6)) with sqnorm];
+ *     m <- momentum m + (1 - momentum) g';   u = nesterov ? momentum m + (1 - momentum) g' : m;
+ *     p <- p - lr_i wd p - lr_i shape_scale[i] X,   lr_i = lr |*lr_scale[i]|  (optional device words; the sign is the caller's mark);
+ *     p_bf16 / p_bf16_lo (optional lists, as of poet_adamw): bf16 image of p and the bf16 residual.
+ * ---------------------------------------------------------------------------------------------- */
+int64_t poet_muon_workspace(const int* rows_host, const int* cols_host, int n);
+int poet_orthogonalize(const void* const* g_host, const int64_t* ldg_host, void* const* o_host, const int64_t* ldo_host, const int* rows_host,
+                       const int* cols_host, int n, int g_dtype, int o_dtype, int steps, const double* coeffs_host, float eps, void* workspace,
+                       int64_t workspace_bytes, void* stream);
+int poet_muon_step(float* const* p_host, const float* const* g_host, float* const* m_host, uint16_t* const* p_bf16_host,
+                   uint16_t* const* p_bf16_lo_host, const float* const* lr_scale_host, const float* shape_scale_host, const int* rows_host,
+                   const int* cols_host, int n, float lr, double momentum, int nesterov, float weight_decay, int steps,
+                   const double* coeffs_host, float eps, const float* sqnorm, float max_norm, float grad_scale, void* workspace,
+                   int64_t workspace_bytes, void* stream);
 /* *word += delta (single-thread kernel): advances the device-side dropout seed / Adam step between graph replays. */
 int poet_counter_add(uint32_t* word, uint32_t delta, void* stream);
 

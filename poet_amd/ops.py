@@ -920,6 +920,157 @@ def adamw(p, g, m, v, n, lr, beta1, beta2, eps, wd, step, sqnorm_buf=None, max_n
                               eps, wd, step, _ptr(sqnorm_buf), max_norm, grad_scale, _ptr(step_dev), _ptr(lr_scale), _stream()), "poet_adamw")
 
 
+NS_COEFFS = (3.4445, -4.7750, 2.0315)           # the quintic step of the Muon optimiser: steep at 0, |x| stays within 0.7 .. 1.2 afterwards
+
+
+def _ns_coeffs(coeffs, steps):
+    flat = [float(v) for c in coeffs for v in c] if len(coeffs) and hasattr(coeffs[0], "__len__") else [float(v) for v in coeffs] * int(steps)
+    if len(flat) != 3 * steps:
+        raise ValueError(f"poet_amd: coeffs is one (a, b, c) or one per step ({steps})")
+    return (C.c_double * len(flat))(*flat)
+
+
+def _muon_dims(shapes):
+    """rows / cols arrays; a tensor of more than two dimensions (a convolution's weight) is rows x everything else."""
+    n = len(shapes)
+    rows, cols = (C.c_int * n)(), (C.c_int * n)()
+    for i, s in enumerate(shapes):
+        if len(s) < 2:
+            raise ValueError(f"poet_amd: a matrix has at least two dimensions, got {tuple(s)}")
+        c = 1
+        for v in s[1:]:
+            c *= v
+        if not (0 < s[0] <= 1 << 20 and 0 < c <= 1 << 20):
+            raise ValueError(f"poet_amd: matrix dimensions must be in 1 .. 2^20, got {tuple(s)}")
+        rows[i], cols[i] = s[0], c
+    return rows, cols
+
+
+def _muon_ws(lib, rows, cols, n, device):
+    need = lib.poet_muon_workspace(rows, cols, n)
+    if need < 0:
+        _lib.check(int(need), "poet_muon_workspace")
+    return torch.empty(need, dtype=torch.uint8, device=device)
+
+
+def orthogonalize(g, out=None, steps=5, coeffs=NS_COEFFS, eps=1e-7):
+    """Newton-Schulz orthogonalisation: X = g / (|g|_F + eps), then `steps` times X <- (a I + b X X^T + c (X X^T)^2) X (from the shorter
+    side).  g: a tensor (..., m, n), or a list of 2-D tensors of any shapes, one type (fp32, bf16, fp16) and device; the result has g's
+    form and type (or goes to `out`, which may be g).  coeffs: (a, b, c), or one such triple per step.  Products carry 22-bit operands
+    and fp32 sums.  All matrices of a call run in one chain of 2 + 3 steps launches, so a list costs little more than its longest chain."""
+    single = torch.is_tensor(g)
+    if single and g.dim() < 2:
+        raise ValueError(f"poet_amd: g must be (..., m, n), got {tuple(g.shape)}")
+    if not single:
+        g = list(g)
+        if any(t.dim() != 2 for t in g):
+            raise ValueError("poet_amd: the tensors of a list are 2-D")
+    if out is None:
+        out = torch.empty(g.shape, dtype=g.dtype, device=g.device) if single else [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in g]
+    gs = [g] if single else g
+    os_ = [out] if single else list(out)
+    if len(gs) != len(os_) or any(a.shape != b.shape for a, b in zip(gs, os_)):
+        raise ValueError("poet_amd: out must have g's shapes")
+    for t in (*gs, *os_):
+        _req(t, "g")
+        if t.device != gs[0].device or t.dtype != (gs[0] if any(t is v for v in gs) else os_[0]).dtype:
+            raise ValueError("poet_amd: the matrices of a call share one device and one type")
+    if not 1 <= steps <= 16:
+        raise ValueError(f"poet_amd: 1 .. 16 steps, got {steps}")
+    cf = _ns_coeffs(coeffs, steps)
+    gp, gl, op, ol, shapes, keep, spans = [], [], [], [], [], [], []
+    for a, b in zip(gs, os_):
+        if a.numel() == 0:
+            continue
+        m, n = a.shape[-2:]
+        if (n > 1 and b.stride(-1) != 1) or (m > 1 and b.stride(-2) < n):
+            raise ValueError("poet_amd: an output's rows must be contiguous and apart")
+        if (n > 1 and a.stride(-1) != 1) or (m > 1 and a.stride(-2) < n):
+            a = a.contiguous()
+            keep.append(a)
+        if a.dim() > 3:
+            a = a.reshape(-1, m, n)
+        if b.dim() > 3:
+            b = b.view(-1, m, n)
+        k = a.shape[0] if a.dim() == 3 else 1
+        if k > 1 and b.stride(0) < (m - 1) * max(b.stride(-2), n) + n:
+            raise ValueError("poet_amd: the matrices of the output overlap")
+        a0, b0, sa, sb = a.data_ptr(), b.data_ptr(), (a.stride(0) * a.element_size() if k > 1 else 0), (b.stride(0) * b.element_size() if k > 1 else 0)
+        keep.append(a)
+        gp += [a0 + i * sa for i in range(k)]
+        op += [b0 + i * sb for i in range(k)]
+        gl += [a.stride(-2) if m > 1 else n] * k
+        ol += [b.stride(-2) if m > 1 else n] * k
+        shapes += [(m, n)] * k
+    n = len(gp)
+    if n == 0:
+        return out
+    if len(set(op)) != n:
+        raise ValueError("poet_amd: the same output twice in one call")
+    lib = _lib.load()
+    dev = gs[0].device
+    rows, cols = _muon_dims(shapes)
+    ptrs, i64s = C.c_void_p * n, C.c_int64 * n
+    with _on_device(gs[0]) as stream:
+        ws = _muon_ws(lib, rows, cols, n, dev)
+        _lib.check(lib.poet_orthogonalize(ptrs(*gp), i64s(*gl), ptrs(*op), i64s(*ol), rows, cols, n, dcode(gs[0]), dcode(os_[0]), steps, cf, eps,
+                                          ws.data_ptr(), ws.numel(), stream), "poet_orthogonalize")
+    return out
+
+
+MUON_SCALES = {"spectral": lambda r, c: max(1.0, r / c) ** 0.5, "rms": lambda r, c: 0.2 * max(r, c) ** 0.5}
+
+
+def muon_step(params, grads, moments, lr, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5, coeffs=NS_COEFFS, eps=1e-7, scale="spectral",
+              p_bf16=None, p_bf16_lo=None, lr_scale=None, sqnorm_buf=None, max_norm=0.0, grad_scale=1.0):
+    """One Muon update, in place, of a list of fp32 weight matrices (more than two dimensions: rows x the rest):
+        m <- momentum m + (1 - momentum) g;  u = momentum m + (1 - momentum) g (nesterov) or m;
+        p <- p (1 - lr weight_decay) - lr s orthogonalize(u)
+    s: "spectral" = sqrt(max(1, rows / cols)), "rms" = 0.2 sqrt(max(rows, cols)) (the step size of AdamW).  Optional, as of adamw: the
+    gradient scale and clip (sqnorm_buf, max_norm), the bf16 images of p (lists), lr_scale = one device word per matrix (its magnitude)."""
+    params, grads, moments = list(params), list(grads), list(moments)
+    n = len(params)
+    if not (len(grads) == len(moments) == n) or any(l is not None and len(l) != n for l in (p_bf16, p_bf16_lo, lr_scale)):
+        raise ValueError("poet_amd: muon_step takes lists of one length")
+    if scale not in MUON_SCALES:
+        raise ValueError(f"poet_amd: scale must be one of {sorted(MUON_SCALES)}, got {scale!r}")
+    if not 0.0 <= momentum < 1.0:
+        raise ValueError(f"poet_amd: momentum must be in [0, 1), got {momentum}")
+    if not 1 <= steps <= 16:
+        raise ValueError(f"poet_amd: 1 .. 16 steps, got {steps}")
+    if p_bf16_lo is not None and p_bf16 is None:
+        raise ValueError("poet_amd: p_bf16_lo goes with p_bf16")
+    if n == 0:
+        return
+    dev = _req(params[0], "params").device
+    f32, bf16 = torch.float32, torch.bfloat16
+    for p, g, m in zip(params, grads, moments):
+        if not (p.dtype == g.dtype == m.dtype == f32 and p.is_contiguous() and g.is_contiguous() and m.is_contiguous()
+                and p.device == g.device == m.device == dev and p.shape == g.shape == m.shape):
+            raise ValueError("poet_amd: parameter, gradient and moment of a matrix are contiguous fp32 tensors of one shape on one device")
+    for l, dt in ((p_bf16, bf16), (p_bf16_lo, bf16), (lr_scale, f32)):
+        if l is not None:
+            for p, t in zip(params, l):
+                if t.dtype != dt or t.device != dev or not t.is_contiguous() or (dt is bf16 and t.numel() != p.numel()):
+                    raise ValueError("poet_amd: bf16 images are contiguous bf16 tensors of the parameter's size, lr_scale fp32 words, on its device")
+    if sqnorm_buf is not None and (sqnorm_buf.dtype != f32 or sqnorm_buf.device != dev):
+        raise ValueError("poet_amd: sqnorm_buf is an fp32 tensor on the parameters' device")
+    rows, cols = _muon_dims([p.shape for p in params])
+    pp, mp = [p.data_ptr() for p in params], [m.data_ptr() for m in moments]
+    if len(set(pp + mp)) != 2 * n:
+        raise ValueError("poet_amd: the same parameter or moment twice in one call")
+    lib = _lib.load()
+    fn = MUON_SCALES[scale]
+    cf = _ns_coeffs(coeffs, steps)
+    ptrs = C.c_void_p * n
+    lst = lambda l: None if l is None else ptrs(*[t.data_ptr() for t in l])        # noqa: E731
+    with _on_device(params[0]) as stream:
+        ws = _muon_ws(lib, rows, cols, n, dev)
+        _lib.check(lib.poet_muon_step(ptrs(*pp), lst(grads), ptrs(*mp), lst(p_bf16), lst(p_bf16_lo), lst(lr_scale),
+                                      (C.c_float * n)(*[fn(r, c) for r, c in zip(rows, cols)]), rows, cols, n, lr, momentum, int(nesterov), weight_decay,
+                                      steps, cf, eps, _ptr(sqnorm_buf), max_norm, grad_scale, ws.data_ptr(), ws.numel(), stream), "poet_muon_step")
+
+
 def counter_add(word, delta=1):
     lib = _lib.load()
     _lib.check(lib.poet_counter_add(_req(word, "word").data_ptr(), delta, _stream()), "poet_counter_add")

@@ -60,3 +60,45 @@ def test_cpu_tensors_are_refused():
     x, w = torch.zeros(1, 4, 8), torch.ones(8)
     with pytest.raises(PoetHipError):
         functional.group_norm_act(x, w, w, 2)
+
+
+def orth(lib, rows=(8,), cols=(16,), n=None, gd=0, od=0, steps=5, coeffs=None, eps=1e-7, ws=FAKE, nws=None, ptr=0x1000, ld=None):
+    n = len(rows) if n is None else n
+    r, c = (ctypes.c_int * len(rows))(*rows), (ctypes.c_int * len(cols))(*cols)
+    need = lib.poet_muon_workspace(r, c, n)
+    ptrs = (ctypes.c_void_p * len(rows))(*[ptr] * len(rows))
+    lds = (ctypes.c_int64 * len(rows))(*(ld or cols))
+    cf = (ctypes.c_double * (3 * max(steps, 1)))(*(coeffs or (3.4445, -4.7750, 2.0315)) * max(steps, 1))
+    return lib.poet_orthogonalize(ptrs, lds, ptrs, lds, r, c, n, gd, od, steps, cf, eps, ws, need if nws is None else nws, None)
+
+
+def test_orthogonalize_refuses_bad_arguments(lib):
+    for kw in (dict(n=0), dict(rows=(0,)), dict(rows=(1 << 21,)), dict(cols=(-3,)), dict(gd=3), dict(od=-1), dict(steps=0), dict(steps=17),
+               dict(coeffs=(50.0, 0.0, 0.0)), dict(coeffs=(float("nan"), 0.0, 0.0)), dict(coeffs=(float("inf"), 0.0, 0.0)), dict(eps=-1.0), dict(eps=float("nan")),
+               dict(ws=None), dict(ws=ctypes.c_void_p(0x1008)), dict(nws=256), dict(ptr=None), dict(ld=(15,))):
+        assert orth(lib, **kw) < 0, kw
+        assert b"orthogonalize" in lib.poet_hip_last_error() or b"muon" in lib.poet_hip_last_error(), kw
+
+
+def test_muon_step_refuses_bad_arguments(lib):
+    r, c = (ctypes.c_int * 1)(8), (ctypes.c_int * 1)(16)
+    need = lib.poet_muon_workspace(r, c, 1)
+    ptrs, cf = (ctypes.c_void_p * 1)(0x1000), (ctypes.c_double * 15)(*(3.4445, -4.7750, 2.0315) * 5)
+
+    def step(p=ptrs, g=ptrs, m=ptrs, hi=None, lo=None, mu=0.95, n=1, nws=need):
+        return lib.poet_muon_step(p, g, m, hi, lo, None, None, r, c, n, 0.02, mu, 1, 0.0, 5, cf, 1e-7, None, 0.0, 1.0, FAKE, nws, None)
+
+    for kw in (dict(p=None), dict(g=None), dict(m=None), dict(lo=ptrs), dict(mu=1.0), dict(mu=-0.1), dict(mu=float("nan")), dict(n=0), dict(nws=0)):
+        assert step(**kw) < 0, kw
+        assert b"muon_step" in lib.poet_hip_last_error(), kw
+
+
+def test_muon_workspace_counts_every_plane(lib):
+    """Two X buffers and the two square matrices, as fp16 pairs on whole tiles, and nothing that grows with the list beyond them."""
+    one = lib.poet_muon_workspace((ctypes.c_int * 1)(256), (ctypes.c_int * 1)(256), 1)
+    assert one >= 4 * 4 * 256 * 256
+    five = lib.poet_muon_workspace((ctypes.c_int * 5)(*[256] * 5), (ctypes.c_int * 5)(*[256] * 5), 5)
+    assert five <= 5 * one
+    big = (ctypes.c_int * 9)(*[1 << 20] * 9)
+    assert lib.poet_muon_workspace(big, big, 1) >= 16 << 40               # (64-bit sizes)
+    assert lib.poet_muon_workspace(big, big, 9) < 0                       # more tiles than a launch can have
