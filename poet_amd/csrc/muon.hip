@@ -14,7 +14,7 @@
 //    come from bounds of the scalar iteration on [0, 1] (host), so that nothing overflows and lo parts stay normal numbers.
 //  * Iterating on A alone (d x d, cheaper for n >> d) was rejected: it squares the condition number, 2e-4 off at fp32.
 //  * A LIST of matrices of any shapes runs in ONE chain of launches (2 + 3 steps): a device table of records, each workgroup finds
-//    its (matrix, tile) by binary search.  A stage's tiles of all matrices overlap; PoET's encoder alone has 30 matrices of which none
+//    its (matrix, tile) from the first tiles.  A stage's tiles of all matrices overlap; PoET's encoder alone has 30 matrices of which none
 //    fills the chip.
 //  * No atomics anywhere: results do not depend on workgroup order, nor on the other matrices of the list.
 #include "common.cuh"
@@ -34,6 +34,7 @@ constexpr int NT = 256;
 constexpr int MAX_STEPS = 16;
 constexpr int CHUNK = 24;                  // matrices per launch of the first kernel (records by value)
 constexpr int NORM_ELEMS = 4096;           // elements per workgroup of the norm pass (and at most 256 workgroups per matrix)
+enum { SYM = 0, UPD = 1, PACK = 2, GRIDS = 3 };      // (narrow matrices: SYM = slabs)
 
 // One matrix.  Offsets in 16-bit elements from the start of the workspace's plane area; a plane pair is hi followed by lo.
 struct Rec {
@@ -44,24 +45,29 @@ struct Rec {
     uint16_t* p16lo;
     const float* lr_scale;                 // optional device word
     int64_t ldg, ldo;
-    int64_t x0, x1, am, bm;                // planes: X (two buffers, dp x np), A and q (dp x dp)
+    int64_t x0, x1, am, bm;                // planes: X (two buffers, dp x np), A and q (dp x dp).  Narrow matrices in slabs: X, and two buffers
+                                           // of fp32 partial Gram matrices in am, bm
     int rows, cols, d, n, dp, np, turned;  // X = u^T when turned (rows > cols)
     int nb, part0;                         // workgroups of the norm pass, first partial sum
-    int sym0, upd0, pack0;                 // first tile of the matrix in the symmetric / update / pack grids
+    int first[GRIDS];                      // first tile of the matrix in each grid
+    int W;                                 // narrow matrices: columns of a slab
+    int gvec, ovec;                        // 16-byte accesses of g (and the moment) as one flat range / of the output rows
     float out_scale;                       // muon: the shape's learning-rate factor
 };
 struct Recs { Rec r[CHUNK]; };
 
 struct NormP {
     Rec* table;
+    int* firsts;                           // [GRIDS][n]: the records' first tiles
     double* part;
-    int first, count;                      // records of this launch
+    int first, count, n;                   // records of this launch, of the list
     int g_dtype, muon, nesterov;
     float mu, omu, gscale, max_norm;       // momentum, 1 - momentum (each rounded once)
     const float* sqnorm;
 };
 struct StageP {
     const Rec* table;
+    const int* firsts;
     const double* part;
     _Float16* planes;
     int count, total;                      // matrices, workgroups
@@ -91,6 +97,10 @@ __device__ __forceinline__ float grad_scale_of(float gscale, const float* sqnorm
 }
 
 // ---- 1: momentum, partial sums of squares (in 64 bits: neither tiny nor huge gradients lose the norm), the table --------------
+__device__ __forceinline__ float direction(float g, float& m, float mu, float omu, int nesterov) {
+    m = fmaf(mu, m, omu * g);
+    return nesterov ? fmaf(mu, m, omu * g) : m;
+}
 __global__ __launch_bounds__(NT) void muon_norm_kernel(const NormP p, const Recs recs) {
     int k = 0, b = blockIdx.x;
     while (b >= recs.r[k].nb) b -= recs.r[k].nb, ++k;
@@ -99,22 +109,55 @@ __global__ __launch_bounds__(NT) void muon_norm_kernel(const NormP p, const Recs
         const uint32_t* src = (const uint32_t*)&r;
         uint32_t* dst = (uint32_t*)(p.table + p.first + k);
         for (int i = threadIdx.x; i < (int)(sizeof(Rec) / 4); i += NT) dst[i] = src[i];
+        if (threadIdx.x < GRIDS) p.firsts[threadIdx.x * p.n + p.first + k] = r.first[threadIdx.x];
     }
     const float gs = grad_scale_of(p.gscale, p.sqnorm, p.max_norm);
-    const int64_t E = (int64_t)r.rows * r.cols;
+    const int64_t E = (int64_t)r.rows * r.cols, step = (int64_t)r.nb * NT;
     double s = 0.0;
-    for (int64_t i = (int64_t)b * NT + threadIdx.x; i < E; i += (int64_t)r.nb * NT) {
-        float v;
-        if (p.muon) {
-            const float g = ((const float*)r.g)[i] * gs;
-            const float m = fmaf(p.mu, r.mom[i], p.omu * g);
-            r.mom[i] = m;
-            v = p.nesterov ? fmaf(p.mu, m, p.omu * g) : m;
-        } else {
-            const int64_t row = i / r.cols;
-            v = ld_any(r.g, row * r.ldg + (i - row * r.cols), p.g_dtype);
+    if (p.muon && r.gvec) {
+        for (int64_t i = (int64_t)b * NT + threadIdx.x; i < E / 4; i += step) {
+            const f32x4_t g = ((const f32x4_t*)r.g)[i];
+            f32x4_t m = ((f32x4_t*)r.mom)[i];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                float me = m[e];
+                const double v = (double)direction(g[e] * gs, me, p.mu, p.omu, p.nesterov);
+                m[e] = me;
+                s = fma(v, v, s);
+            }
+            ((f32x4_t*)r.mom)[i] = m;
         }
-        s += (double)v * (double)v;
+    } else if (p.muon) {
+        for (int64_t i = (int64_t)b * NT + threadIdx.x; i < E; i += step) {
+            float m = r.mom[i];
+            const double v = (double)direction(((const float*)r.g)[i] * gs, m, p.mu, p.omu, p.nesterov);
+            r.mom[i] = m;
+            s = fma(v, v, s);
+        }
+    } else if (r.gvec && p.g_dtype == POET_F32) {
+        for (int64_t i = (int64_t)b * NT + threadIdx.x; i < E / 4; i += step) {
+            const f32x4_t g = ((const f32x4_t*)r.g)[i];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s = fma((double)g[e], (double)g[e], s);
+        }
+    } else if (r.gvec) {
+        for (int64_t i = (int64_t)b * NT + threadIdx.x; i < E / 8; i += step) {
+            float g[8];
+            if (p.g_dtype == POET_BF16) vec<bf16_t, 8>::ld((const bf16_t*)r.g + i * 8, g);
+            else vec<f16_t, 8>::ld((const f16_t*)r.g + i * 8, g);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s = fma((double)g[e], (double)g[e], s);
+        }
+    } else {
+        int row = (b * NT + (int)threadIdx.x) / r.cols, col = (b * NT + (int)threadIdx.x) % r.cols;
+        const int drow = (int)(step / r.cols), dcol = (int)(step % r.cols);
+        while (row < r.rows) {
+            const double v = (double)ld_any(r.g, row * r.ldg + col, p.g_dtype);
+            s = fma(v, v, s);
+            row += drow;
+            col += dcol;
+            if (col >= r.cols) col -= r.cols, ++row;
+        }
     }
     __shared__ double red[NT / 64];
     for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o, 64);
@@ -123,15 +166,15 @@ __global__ __launch_bounds__(NT) void muon_norm_kernel(const NormP p, const Recs
     if (threadIdx.x == 0) p.part[r.part0 + b] = (red[0] + red[1]) + (red[2] + red[3]);
 }
 
-// workgroup -> record whose [first tile, next first tile) holds b (FIRST: member of Rec); tiles of one matrix go to one XCD range
-template <int Rec::*FIRST> __device__ __forceinline__ int find(const Rec* table, int count, int b) {
-    int lo = 0, hi = count - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (table[mid].*FIRST <= b) lo = mid;
-        else hi = mid - 1;
+// workgroup -> the record whose [first tile, next first tile) holds b: the wave compares 64 first tiles at once (one load's latency, where
+// a binary search pays one per halving)
+__device__ __forceinline__ const Rec& find(const Rec* table, const int* firsts, int count, int b) {
+    int k = -1;
+    for (int c = 0; c < count; c += 64) {
+        const int i = c + (threadIdx.x & 63);
+        k += __popcll(__ballot(i < count && firsts[min(i, count - 1)] <= b));
     }
-    return lo;
+    return table[__builtin_amdgcn_readfirstlane(k)];
 }
 __device__ __forceinline__ int xcd_order(int b, int total) {          // workgroup b runs on XCD b % 8: give each a contiguous range of tiles
     const int q = total >> 3, rem = total & 7, x = b & 7;
@@ -145,8 +188,8 @@ __device__ __forceinline__ void split16(float v, _Float16& hi, _Float16& lo) {
 
 // ---- 2: X_0 as scaled hi / lo planes, zero-padded to whole tiles ------------------------------------------------------------
 __global__ __launch_bounds__(NT) void muon_pack_kernel(const StageP p) {
-    const int b = blockIdx.x, k = find<&Rec::pack0>(p.table, p.count, b);
-    const Rec r = p.table[k];
+    const int b = blockIdx.x;
+    const Rec r = find(p.table, p.firsts + PACK * p.count, p.count, b);
     __shared__ float tile[64][65];
     __shared__ double s_inv;
     if (threadIdx.x < 64) {
@@ -158,7 +201,7 @@ __global__ __launch_bounds__(NT) void muon_pack_kernel(const StageP p) {
         }
     }
     const float gs = grad_scale_of(p.gscale, p.sqnorm, p.max_norm);
-    const int t = b - r.pack0, tn = r.np >> 6, i0 = (t / tn) << 6, j0 = (t % tn) << 6;
+    const int t = b - r.first[PACK], tn = r.np >> 6, i0 = (t / tn) << 6, j0 = (t % tn) << 6;
     const int sr = r.turned ? j0 : i0, sc = r.turned ? i0 : j0;       // the tile's place in u
     const int c = threadIdx.x & 63;
     for (int q = threadIdx.x >> 6; q < 64; q += 4) {
@@ -167,7 +210,7 @@ __global__ __launch_bounds__(NT) void muon_pack_kernel(const StageP p) {
         if (row < r.rows && col < r.cols) {
             if (p.muon) {
                 const int64_t i = (int64_t)row * r.cols + col;
-                const float m = r.mom[i];
+                const float m = r.mom[i];                              // (already this step's)
                 v = p.nesterov ? fmaf(p.mu, m, p.omu * (((const float*)r.g)[i] * gs)) : m;
             } else v = ld_any(r.g, row * r.ldg + col, p.g_dtype);
         }
@@ -304,13 +347,38 @@ template <int T, int BK, bool KM> struct Core {
 
 union H4 { _Float16 h[4]; uint2 u; };
 
+// A wave's T/2 x T/2 part of the tile, restaged through LDS so that results leave in whole rows of either orientation (straight from the
+// accumulators a lane owns 4 consecutive columns of one row, the mirror image would leave in 2-byte stores).  16-byte pieces of row i are
+// XORed with i / 4: both the rows and the columns of 4 read back without bank conflicts.
+template <int T> struct Sub {
+    static constexpr int S = T / 2;
+    static __device__ __forceinline__ int at(int i, int piece) { return i * S + ((piece ^ (i >> 2)) & (S / 4 - 1)) * 4; }
+    static __device__ __forceinline__ float* put(char* smem, const f32x4_t (&acc)[T / 32][T / 32], int wave, int lane) {
+        float* sub = reinterpret_cast<float*>(smem) + wave * S * S;
+        __syncthreads();                                                      // (the last stage's operands have been read)
+#pragma unroll
+        for (int f = 0; f < T / 32; ++f)
+#pragma unroll
+            for (int s = 0; s < T / 32; ++s) *reinterpret_cast<f32x4_t*>(sub + at(s * 16 + (lane & 15), f * 4 + (lane >> 4))) = acc[f][s];
+        __syncthreads();
+        return sub;
+    }
+    static __device__ __forceinline__ f32x4_t row(const float* sub, int i, int j) { return *reinterpret_cast<const f32x4_t*>(sub + at(i, j >> 2)); }
+    static __device__ __forceinline__ f32x4_t col(const float* sub, int i, int j) {       // elements (i .. i + 3, j)
+        f32x4_t v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = sub[at(i + e, j >> 2) + (j & 3)];
+        return v;
+    }
+};
+
 // A = X X^T (Q = 0), or q = a I + b A + c A A (Q = 1): tiles on and below the diagonal, written twice
 template <int T, int BK, int Q> __global__ __launch_bounds__(NT, 2) void muon_sym_kernel(const StageP p) {
     __shared__ __attribute__((aligned(16))) char smem[2 * Core<T, BK, false>::STAGE];
     constexpr int F = T / 32;
-    const int b = xcd_order(blockIdx.x, p.total), kk = find<&Rec::sym0>(p.table, p.count, b);
-    const Rec& r = p.table[kk];
-    const int t = b - r.sym0, dp = r.dp;
+    const int b = xcd_order(blockIdx.x, p.total);
+    const Rec r = find(p.table, p.firsts + SYM * p.count, p.count, b);
+    const int t = b - r.first[SYM], dp = r.dp;
     int bi = (int)((sqrtf(8.f * (float)t + 1.f) - 1.f) * 0.5f);
     while ((bi + 1) * (bi + 2) / 2 <= t) ++bi;
     while (bi * (bi + 1) / 2 > t) --bi;
@@ -325,55 +393,75 @@ template <int T, int BK, int Q> __global__ __launch_bounds__(NT, 2) void muon_sy
         for (int s = 0; s < F; ++s) acc[f][s] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     Core<T, BK, false>::run(in + j0 * ld, in + plane + j0 * ld, ld, in + i0 * ld, in + plane + i0 * ld, ld, K, smem, acc);
 
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wf = (wave >> 1) * (T / 2), ws = (wave & 1) * (T / 2), m16 = lane & 15, kc = lane >> 4;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wf = (wave >> 1) * (T / 2), ws = (wave & 1) * (T / 2);
     const int64_t sq = (int64_t)dp * dp;
     const _Float16* am = p.planes + r.am;
     _Float16* out = p.planes + (Q ? r.bm : r.am);
+    float* sub = Sub<T>::put(smem, acc, wave, lane);
+    constexpr int LPR = Sub<T>::S / 4;                                        // lanes per row of 4-element pieces
 #pragma unroll
-    for (int f = 0; f < F; ++f)
-#pragma unroll
-        for (int s = 0; s < F; ++s) {
-            const int i = i0 + ws + s * 16 + m16, j = j0 + wf + f * 16 + 4 * kc;          // row i, columns j .. j + 3
-            H4 h, l;
-            if constexpr (Q) {
-                H4 ah, al;
-                ah.u = *reinterpret_cast<const uint2*>(am + (int64_t)i * dp + j);
-                al.u = *reinterpret_cast<const uint2*>(am + sq + (int64_t)i * dp + j);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float v = fmaf(p.c * p.in_scale, acc[f][s][e], p.b * ((float)ah.h[e] + (float)al.h[e]));
-                    if (i == j + e && i < r.d) v += p.a;
-                    split16(v * p.out_exp, h.h[e], l.h[e]);
-                }
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) split16(acc[f][s][e] * (p.in_scale * p.out_exp), h.h[e], l.h[e]);
-            }
-            if (i >= j + 3) {
-                *reinterpret_cast<uint2*>(out + (int64_t)i * dp + j) = h.u;
-                *reinterpret_cast<uint2*>(out + sq + (int64_t)i * dp + j) = l.u;
-            }
+    for (int it = 0; it < Sub<T>::S * LPR / 64; ++it) {
+        const int li = it * (64 / LPR) + lane / LPR, lj = (lane % LPR) * 4, i = i0 + ws + li, j = j0 + wf + lj;
+        if (i < j) continue;                                                  // (pieces on and below the diagonal; pieces start at multiples of 4)
+        const f32x4_t v = Sub<T>::row(sub, li, lj);
+        H4 h, l;
+        if constexpr (Q) {
+            H4 ah, al;
+            ah.u = *reinterpret_cast<const uint2*>(am + (int64_t)i * dp + j);
+            al.u = *reinterpret_cast<const uint2*>(am + sq + (int64_t)i * dp + j);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                if (i < j + 3 && i >= j + e) {
-                    out[(int64_t)i * dp + j + e] = h.h[e];
-                    out[sq + (int64_t)i * dp + j + e] = l.h[e];
-                }
-                if (i > j + e) {
-                    out[(int64_t)(j + e) * dp + i] = h.h[e];
-                    out[sq + (int64_t)(j + e) * dp + i] = l.h[e];
-                }
+                float w = fmaf(p.c * p.in_scale, v[e], p.b * ((float)ah.h[e] + (float)al.h[e]));
+                if (i == j + e && i < r.d) w += p.a;
+                split16(w * p.out_exp, h.h[e], l.h[e]);
             }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) split16(v[e] * (p.in_scale * p.out_exp), h.h[e], l.h[e]);
         }
+        _Float16* o = out + (int64_t)i * dp + j;
+        if (i >= j + 3) {
+            *reinterpret_cast<uint2*>(o) = h.u;
+            *reinterpret_cast<uint2*>(o + sq) = l.u;
+        } else
+#pragma unroll
+            for (int e = 0; e < 3; ++e)
+                if (i >= j + e) o[e] = h.h[e], o[sq + e] = l.h[e];
+    }
+    // the mirror image: row j of the result, columns i .. i + 3
+#pragma unroll
+    for (int it = 0; it < Sub<T>::S * LPR / 64; ++it) {
+        const int lj = it * (64 / LPR) + lane / LPR, li = (lane % LPR) * 4, i = i0 + ws + li, j = j0 + wf + lj;
+        if (i + 3 <= j) continue;
+        const f32x4_t v = Sub<T>::col(sub, li, lj);
+        H4 h, l, ah, al;
+        if constexpr (Q) {                                                    // (A is symmetric to the bit)
+            ah.u = *reinterpret_cast<const uint2*>(am + (int64_t)j * dp + i);
+            al.u = *reinterpret_cast<const uint2*>(am + sq + (int64_t)j * dp + i);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if constexpr (Q) split16(fmaf(p.c * p.in_scale, v[e], p.b * ((float)ah.h[e] + (float)al.h[e])) * p.out_exp, h.h[e], l.h[e]);
+            else split16(v[e] * (p.in_scale * p.out_exp), h.h[e], l.h[e]);
+        }
+        _Float16* o = out + (int64_t)j * dp + i;
+        if (i > j) {
+            *reinterpret_cast<uint2*>(o) = h.u;
+            *reinterpret_cast<uint2*>(o + sq) = l.u;
+        } else
+#pragma unroll
+            for (int e = 1; e < 4; ++e)
+                if (i + e > j) o[e] = h.h[e], o[sq + e] = l.h[e];
+    }
 }
 
 // X' = q X; the last step leaves the planes: the output matrix, or the weight update
 template <int T, int BK, bool LAST> __global__ __launch_bounds__(NT, 2) void muon_update_kernel(const StageP p) {
     __shared__ __attribute__((aligned(16))) char smem[2 * Core<T, BK, true>::STAGE];
     constexpr int F = T / 32;
-    const int b = xcd_order(blockIdx.x, p.total), kk = find<&Rec::upd0>(p.table, p.count, b);
-    const Rec& r = p.table[kk];
-    const int t = b - r.upd0, tn = r.np / T, i0 = (t / tn) * T, j0 = (t % tn) * T, dp = r.dp;
+    const int b = xcd_order(blockIdx.x, p.total);
+    const Rec r = find(p.table, p.firsts + UPD * p.count, p.count, b);
+    const int t = b - r.first[UPD], tn = r.np / T, i0 = (t / tn) * T, j0 = (t % tn) * T, dp = r.dp;
     const int64_t np = r.np, plane = (int64_t)dp * np, sq = (int64_t)dp * dp;
     const _Float16* x = p.planes + (p.flip ? r.x1 : r.x0);
     const _Float16* qm = p.planes + r.bm;
@@ -384,96 +472,620 @@ template <int T, int BK, bool LAST> __global__ __launch_bounds__(NT, 2) void muo
         for (int s = 0; s < F; ++s) acc[f][s] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     Core<T, BK, true>::run(x + j0, x + plane + j0, np, qm + (int64_t)i0 * dp, qm + sq + (int64_t)i0 * dp, dp, (r.d + BK - 1) / BK * BK, smem, acc);
 
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wf = (wave >> 1) * (T / 2), ws = (wave & 1) * (T / 2), m16 = lane & 15, kc = lane >> 4;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wf = (wave >> 1) * (T / 2), ws = (wave & 1) * (T / 2);
+    float* sub = Sub<T>::put(smem, acc, wave, lane);
+    constexpr int LPR = Sub<T>::S / 4;
     const float lr = p.lr * (r.lr_scale ? fabsf(*r.lr_scale) : 1.f);
 #pragma unroll
-    for (int f = 0; f < F; ++f)
+    for (int it = 0; it < Sub<T>::S * LPR / 64; ++it) {
+        const int la = it * (64 / LPR) + lane / LPR, lb = (lane % LPR) * 4;
+        if constexpr (!LAST) {
+            const f32x4_t v = Sub<T>::row(sub, la, lb);
+            _Float16* out = p.planes + (p.flip ? r.x0 : r.x1) + (int64_t)(i0 + ws + la) * np + j0 + wf + lb;
+            H4 h, l;
 #pragma unroll
-        for (int s = 0; s < F; ++s) {
-            const int i = i0 + ws + s * 16 + m16, j = j0 + wf + f * 16 + 4 * kc;
-            if constexpr (!LAST) {
-                _Float16* out = p.planes + (p.flip ? r.x0 : r.x1) + (int64_t)i * np + j;
-                H4 h, l;
+            for (int e = 0; e < 4; ++e) split16(v[e] * (p.in_scale * p.out_exp), h.h[e], l.h[e]);
+            *reinterpret_cast<uint2*>(out) = h.u;
+            *reinterpret_cast<uint2*>(out + plane) = l.u;
+        } else {
+            // output rows: X's rows, or X's columns when turned
+            f32x4_t v = r.turned ? Sub<T>::col(sub, lb, la) : Sub<T>::row(sub, la, lb);
+            const int row = r.turned ? j0 + wf + la : i0 + ws + la, col = r.turned ? i0 + ws + lb : j0 + wf + lb;
+            if (row >= r.rows || col >= r.cols) continue;
+            const int64_t at = row * r.ldo + col;
+            v *= p.in_scale;
+            if (p.muon) {
+                float* w = (float*)r.o + at;
+                if (r.ovec) {                                                 // (cols % 4 == 0)
+                    f32x4_t o = *reinterpret_cast<f32x4_t*>(w);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) split16(acc[f][s][e] * (p.in_scale * p.out_exp), h.h[e], l.h[e]);
-                *reinterpret_cast<uint2*>(out) = h.u;
-                *reinterpret_cast<uint2*>(out + plane) = l.u;
-            } else {
+                    for (int e = 0; e < 4; ++e) o[e] = fmaf(-lr * r.out_scale, v[e], o[e] - lr * p.wd * o[e]);
+                    *reinterpret_cast<f32x4_t*>(w) = o;
+                    if (r.p16) {
+                        const uint2 hi = make_uint2(pack_bf2(o[0], o[1]), pack_bf2(o[2], o[3]));
+                        *reinterpret_cast<uint2*>(r.p16 + at) = hi;
+                        if (r.p16lo)
+                            *reinterpret_cast<uint2*>(r.p16lo + at) =
+                                make_uint2(pack_bf2(o[0] - __uint_as_float(hi.x << 16), o[1] - __uint_as_float(hi.x & 0xffff0000u)),
+                                           pack_bf2(o[2] - __uint_as_float(hi.y << 16), o[3] - __uint_as_float(hi.y & 0xffff0000u)));
+                    }
+                    continue;
+                }
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    if (i >= r.d || j + e >= r.n) continue;
-                    const float v = acc[f][s][e] * p.in_scale;
-                    const int64_t row = r.turned ? j + e : i, col = r.turned ? i : j + e, at = row * r.ldo + col;
-                    if (p.muon) {
-                        float* w = (float*)r.o;
-                        const float nw = fmaf(-lr * r.out_scale, v, w[at] - lr * p.wd * w[at]);
-                        w[at] = nw;
-                        if (r.p16) {
-                            const bf16_t hi = f2bf(nw);
-                            r.p16[at] = hi;
-                            if (r.p16lo) r.p16lo[at] = f2bf(nw - bf2f(hi));
-                        }
-                    } else st_any(r.o, at, v, p.o_dtype);
+                    if (col + e >= r.cols) break;
+                    const float nw = fmaf(-lr * r.out_scale, v[e], w[e] - lr * p.wd * w[e]);
+                    w[e] = nw;
+                    if (r.p16) {
+                        const bf16_t hi = f2bf(nw);
+                        r.p16[at + e] = hi;
+                        if (r.p16lo) r.p16lo[at + e] = f2bf(nw - bf2f(hi));
+                    }
+                }
+            } else if (r.ovec && p.o_dtype == POET_F32) *reinterpret_cast<f32x4_t*>((float*)r.o + at) = v;
+            else if (r.ovec) {
+                float o[4] = {v[0], v[1], v[2], v[3]};
+                if (p.o_dtype == POET_BF16) vec<bf16_t, 4>::st((bf16_t*)r.o + at, o);
+                else vec<f16_t, 4>::st((f16_t*)r.o + at, o);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (col + e < r.cols) st_any(r.o, at + e, v[e], p.o_dtype);
+            }
+        }
+    }
+}
+
+// ---- narrow matrices: d <= 160 ------------------------------------------------------------------------------------------------
+// The chain above costs 3 dependent launches a step whatever the size, ~6 us each with next to no work in them.  With few rows a
+// workgroup can hold everything that the step needs in LDS: q (dp x dp planes) and a SLAB of X's columns.  X' = q X stays inside a slab; only
+// A = X X^T couples the slabs, through dp x dp partial sums.
+//   * one slab (n <= W_max): ONE launch does momentum, norm, all steps and the update of a matrix per workgroup;
+//   * up to 8 slabs: the norm pass, a launch for X_0 and its partial A, then one launch a step, in which every workgroup folds the partial
+//     A's of its matrix, forms q for itself (redundant, but dp^3 is small), updates its slab and leaves the partial A of the next step.
+// 8 waves.  All of it is bound by LDS bandwidth and latency (one workgroup a CU), so: A and A^2 in 32 x 32 macro tiles on and below the
+// diagonal (each fragment read serves two tiles; a diagonal one reads its fragments once), the update in PAIRS of 16-column strips (each
+// fragment of q serves both), rewritten in place by the wave that owns them.  Rows of the LDS images are padded by 16 bytes: an odd number
+// of 16-byte pieces, so that the 16 rows of a fragment read start in different banks.
+constexpr int NW_T = 512, NWAVES = NW_T / 64, MAX_SLABS = 8, MAX_D = 5;
+template <int D> struct Narrow {
+    static constexpr int DP = 32 * D, NM = D * (D + 1) / 2;
+    static constexpr int PARTS = D == 1 ? 8 : D == 2 ? 2 : 1;             // few macro tiles: the columns in PARTS ranges, so that all waves have some
+    static constexpr int ITEMS = NM * PARTS, ROUNDS = (ITEMS + NWAVES - 1) / NWAVES;
+    static constexpr int AROW = DP * 2 + 16, APLANE = DP * AROW;
+    static constexpr int SCRATCH = PARTS > 1 ? ITEMS * 4096 : 0;
+    static constexpr int REGION = 2 * APLANE > SCRATCH ? 2 * APLANE : SCRATCH;      // A / q planes, or partial tiles
+};
+constexpr int W_MAX[MAX_D + 1] = {0, 896, 512, 288, 160, 64};       // columns that leave room for REGION in 160 KB
+struct NarrowP {
+    StageP s;
+    int mode, k, steps;                              // N_*; this launch's step
+    float a[MAX_STEPS], b[MAX_STEPS], c[MAX_STEPS];  // b carries A's exponent, c the square of it
+    float ascale[MAX_STEPS], qscale[MAX_STEPS], xscale[MAX_STEPS];
+};
+enum { N_INIT, N_STEP, N_LAST };
+
+template <int D> struct Slab {
+    typedef Narrow<D> N;
+    char* reg;                             // REGION bytes
+    char* x;                               // hi plane, then lo plane: DP rows of W columns
+    int W, xs, xplane;
+    int lane, wave, m16, kc;
+
+    __device__ __forceinline__ Slab(char* smem, int W_) : reg(smem), x(smem + N::REGION), W(W_), xs(W_ * 2 + 16), xplane(N::DP * (W_ * 2 + 16)) {
+        lane = threadIdx.x & 63;
+        wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        m16 = lane & 15;
+        kc = lane >> 4;
+    }
+    static __device__ __forceinline__ void macro(int t, int& bi, int& bj) {
+        bi = 0;
+        while ((bi + 1) * (bi + 2) / 2 <= t) ++bi;
+        bj = t - bi * (bi + 1) / 2;
+    }
+    // u's columns [j0, j0 + W) of X into the planes as the two halves of their fp32 bits, zero outside the matrix; `at(row, col)` order
+    // follows the matrix's rows.  FIRST: the momentum is this step's only afterwards.  Returns this thread's sum of squares.
+    template <bool FIRST> __device__ __forceinline__ double load(const Rec& r, const StageP& p, float gs, int j0) const {
+        for (int o = threadIdx.x * 16; o < 2 * xplane; o += NW_T * 16) *reinterpret_cast<u32x4_t*>(x + o) = u32x4_t{0, 0, 0, 0};
+        __syncthreads();
+        const int jn = min(W, r.n - j0), cols = r.turned ? r.d : jn, total = r.d * jn;
+        const int row0 = r.turned ? j0 : 0, col0 = r.turned ? 0 : j0;
+        int a = threadIdx.x / cols, c = threadIdx.x % cols;
+        const int da = NW_T / cols, dc = NW_T % cols;
+        double sum = 0.0;
+        constexpr int U = 8;                                                  // loads in flight
+        auto batches = [&](auto&& fetch, auto&& value) {                      // fetch(u, offset of the element), then value(u, offset)
+            for (int e = threadIdx.x; e < total; e += U * NW_T) {
+                int64_t at[U];
+                int o[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const bool in = e + u * NW_T < total;                     // (behind the end: the first element again)
+                    const int ra = in ? a : 0, rc = in ? c : 0;
+                    at[u] = (row0 + ra) * r.ldg + col0 + rc;
+                    o[u] = (r.turned ? rc : ra) * xs + (r.turned ? ra : rc) * 2;
+                    fetch(u, at[u]);
+                    a += da;
+                    c += dc;
+                    if (c >= cols) c -= cols, ++a;
+                }
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    if (e + u * NW_T >= total) break;
+                    const float v = value(u, at[u]);
+                    sum = fma((double)v, (double)v, sum);
+                    *reinterpret_cast<uint16_t*>(x + o[u]) = (uint16_t)(__float_as_uint(v) >> 16);
+                    *reinterpret_cast<uint16_t*>(x + xplane + o[u]) = (uint16_t)__float_as_uint(v);
+                }
+            }
+        };
+        float g[U], m[U];
+        uint16_t h[U];
+        if (p.muon) {
+            batches([&](int u, int64_t at) { g[u] = ((const float*)r.g)[at], m[u] = r.mom[at]; },
+                    [&](int u, int64_t at) {
+                        if constexpr (!FIRST) return p.nesterov ? fmaf(p.mu, m[u], p.omu * (g[u] * gs)) : m[u];
+                        const float v = direction(g[u] * gs, m[u], p.mu, p.omu, p.nesterov);
+                        r.mom[at] = m[u];
+                        return v;
+                    });
+        } else if (p.g_dtype == POET_F32)
+            batches([&](int u, int64_t at) { g[u] = ((const float*)r.g)[at]; }, [&](int u, int64_t) { return g[u]; });
+        else {
+            const bool bf = p.g_dtype == POET_BF16;
+            batches([&](int u, int64_t at) { h[u] = ((const uint16_t*)r.g)[at]; },
+                    [&](int u, int64_t) { return bf ? bf2f(h[u]) : h_lo(h[u]); });
+        }
+        return sum;
+    }
+    // the fp32 halves -> normalised, scaled hi / lo planes: times `by` (a mantissa and an exponent: 64-bit arithmetic per element costs
+    // several times the pass, and the factor alone may leave fp32's range)
+    __device__ __forceinline__ void normalise(double by) const {
+        int ex = 0;
+        const float inv = (float)frexp(by, &ex);
+        __syncthreads();
+#pragma unroll 4
+        for (int o = threadIdx.x * 4; o < xplane; o += NW_T * 4) {
+            const uint32_t h = *reinterpret_cast<const uint32_t*>(x + o), l = *reinterpret_cast<const uint32_t*>(x + xplane + o);
+            union { _Float16 f[2]; uint32_t u; } nh, nl;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const uint32_t bits = e ? (h & 0xffff0000u) | (l >> 16) : (h << 16) | (l & 0xffffu);
+                split16(ldexpf(__uint_as_float(bits) * inv, ex), nh.f[e], nl.f[e]);
+            }
+            *reinterpret_cast<uint32_t*>(x + o) = nh.u;
+            *reinterpret_cast<uint32_t*>(x + xplane + o) = nl.u;
+        }
+        __syncthreads();
+    }
+    static __device__ __forceinline__ void product(f32x4_t (&acc)[2][2], const char* fb, const char* sb, int row, int plane, bool diagonal) {
+        f16x8_t fh[2], fl[2], sh[2], sl[2];
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            fh[q] = *reinterpret_cast<const f16x8_t*>(fb + q * 16 * row);
+            fl[q] = *reinterpret_cast<const f16x8_t*>(fb + q * 16 * row + plane);
+        }
+        if (diagonal) {
+#pragma unroll
+            for (int q = 0; q < 2; ++q) sh[q] = fh[q], sl[q] = fl[q];
+        } else {
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                sh[q] = *reinterpret_cast<const f16x8_t*>(sb + q * 16 * row);
+                sl[q] = *reinterpret_cast<const f16x8_t*>(sb + q * 16 * row + plane);
+            }
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) acc[q >> 1][q & 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fl[q >> 1], sh[q & 1], acc[q >> 1][q & 1], 0, 0, 0);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) acc[q >> 1][q & 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fh[q >> 1], sl[q & 1], acc[q >> 1][q & 1], 0, 0, 0);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) acc[q >> 1][q & 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fh[q >> 1], sh[q & 1], acc[q >> 1][q & 1], 0, 0, 0);
+    }
+    // tiles of X X^T: acc[round] of item wave + 8 round = part * NM + macro tile
+    typedef f32x4_t Tile[2][2];
+    __device__ __forceinline__ void gram(Tile (&acc)[N::ROUNDS]) const {
+        const int KS = W / 32;
+#pragma unroll
+        for (int u = 0; u < N::ROUNDS; ++u) {
+            const int item = wave + u * NWAVES;
+            if (item >= N::ITEMS) break;
+            const int mt = item % N::NM, part = item / N::NM;
+            int bi, bj;
+            macro(mt, bi, bj);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) acc[u][q >> 1][q & 1] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+            const char* fb = x + (bj * 32 + m16) * xs + kc * 16;
+            const char* sb = x + (bi * 32 + m16) * xs + kc * 16;
+            for (int ks = part * KS / N::PARTS; ks < (part + 1) * KS / N::PARTS; ++ks) product(acc[u], fb + ks * 64, sb + ks * 64, xs, xplane, bi == bj);
+        }
+    }
+    // a tile in memory: 32 rows of 8 pieces of 4 columns, XORed with the row (the 16 rows of a store in different banks)
+    static __device__ __forceinline__ int tile_at(int i, int piece) { return i * 32 + ((piece ^ (i & 7)) * 4); }
+    __device__ __forceinline__ void put_tile(float* out, const Tile& acc) const {
+#pragma unroll
+        for (int f = 0; f < 2; ++f)
+#pragma unroll
+            for (int q = 0; q < 2; ++q) *reinterpret_cast<f32x4_t*>(out + tile_at(q * 16 + m16, f * 4 + kc)) = acc[f][q];
+    }
+    __device__ __forceinline__ void put_a(int i, int j, float v) const {
+        _Float16 h, l;
+        split16(v, h, l);
+        *reinterpret_cast<_Float16*>(reg + i * N::AROW + j * 2) = h;
+        *reinterpret_cast<_Float16*>(reg + N::APLANE + i * N::AROW + j * 2) = l;
+        *reinterpret_cast<_Float16*>(reg + j * N::AROW + i * 2) = h;
+        *reinterpret_cast<_Float16*>(reg + N::APLANE + j * N::AROW + i * 2) = l;
+    }
+    // this thread's 2 NM elements of the macro tiles, summed over the partial tiles at t[(q NM + m) 1024 ...], q < count
+    __device__ __forceinline__ void sum_tiles(const float* t, int count, float* v) const {
+#pragma unroll
+        for (int m = 0; m < 2 * N::NM; ++m) v[m] = 0.f;
+#pragma unroll D == 1 ? 4 : 1
+        for (int q = 0; q < count; ++q) {                                     // (2 NM loads and more in flight)
+            float w[2 * N::NM];
+#pragma unroll
+            for (int m = 0; m < 2 * N::NM; ++m) w[m] = t[(int64_t)q * N::NM * 1024 + m * 512 + threadIdx.x];
+#pragma unroll
+            for (int m = 0; m < 2 * N::NM; ++m) v[m] += w[m];
+        }
+    }
+    // A's planes from partial tiles; in_region: these lie where the planes go
+    __device__ __forceinline__ void fold(const float* t, int count, float scale, bool in_region) const {
+        float v[2 * N::NM];
+        sum_tiles(t, count, v);
+        if (in_region) __syncthreads();
+#pragma unroll
+        for (int m = 0; m < 2 * N::NM; ++m) {
+            int bi, bj;
+            macro(m >> 1, bi, bj);
+            const int li = (m & 1) * 16 + (threadIdx.x >> 5), lp = ((threadIdx.x >> 2) & 7) ^ (li & 7);
+            const int i = bi * 32 + li, j = bj * 32 + lp * 4 + (threadIdx.x & 3);
+            if (i >= j) put_a(i, j, v[m] * scale);
+        }
+        __syncthreads();
+    }
+    __device__ __forceinline__ void planes(const Tile& acc, int mt, float scale) const {
+        int bi, bj;
+        macro(mt, bi, bj);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int i = bi * 32 + (q & 1) * 16 + m16, j = bj * 32 + (q >> 1) * 16 + 4 * kc;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (i >= j + e) put_a(i, j + e, acc[q >> 1][q & 1][e] * scale);
+        }
+    }
+    // A of the whole slab, for a matrix of one slab
+    __device__ __forceinline__ void gram_planes(float scale) const {
+        Tile acc[N::ROUNDS];
+        gram(acc);
+        if constexpr (N::PARTS > 1) {
+#pragma unroll
+            for (int u = 0; u < N::ROUNDS; ++u)
+                if (wave + u * NWAVES < N::ITEMS) put_tile(reinterpret_cast<float*>(reg) + (wave + u * NWAVES) * 1024, acc[u]);
+            __syncthreads();
+            fold(reinterpret_cast<const float*>(reg), N::PARTS, scale, true);
+        } else {
+#pragma unroll
+            for (int u = 0; u < N::ROUNDS; ++u)
+                if (wave + u * NWAVES < N::ITEMS) planes(acc[u], wave + u * NWAVES, scale);
+            __syncthreads();
+        }
+    }
+    // q = a I + b A + c A A in A's place
+    __device__ __forceinline__ void square(float a, float b, float c, float scale, int d) const {
+        constexpr int R = (N::NM + NWAVES - 1) / NWAVES;
+        Tile acc[R];
+#pragma unroll
+        for (int u = 0; u < R; ++u) {
+            const int mt = wave + u * NWAVES;
+            if (mt >= N::NM) break;
+            int bi, bj;
+            macro(mt, bi, bj);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) acc[u][q >> 1][q & 1] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int ks = 0; ks < D; ++ks)
+                product(acc[u], reg + (bj * 32 + m16) * N::AROW + ks * 64 + kc * 16, reg + (bi * 32 + m16) * N::AROW + ks * 64 + kc * 16, N::AROW, N::APLANE, bi == bj);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int i = bi * 32 + (q & 1) * 16 + m16, j = bj * 32 + (q >> 1) * 16 + 4 * kc;
+                H4 ah, al;
+                ah.u = *reinterpret_cast<const uint2*>(reg + i * N::AROW + j * 2);
+                al.u = *reinterpret_cast<const uint2*>(reg + N::APLANE + i * N::AROW + j * 2);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float v = fmaf(c, acc[u][q >> 1][q & 1][e], b * ((float)ah.h[e] + (float)al.h[e]));
+                    if (i == j + e && i < d) v += a;
+                    acc[u][q >> 1][q & 1][e] = v;
                 }
             }
         }
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < R; ++u)
+            if (wave + u * NWAVES < N::NM) planes(acc[u], wave + u * NWAVES, scale);
+        __syncthreads();
+    }
+    // q X of S neighbouring strips from ct on: out(i, j, four columns of row i)
+    template <int S, typename F> __device__ __forceinline__ void strip(int ct, F&& out) const {
+        f32x4_t acc[S][2 * D];
+#pragma unroll
+        for (int q = 0; q < S; ++q)
+#pragma unroll
+            for (int t = 0; t < 2 * D; ++t) acc[q][t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int ks = 0; ks < D; ++ks) {
+            f16x8_t fh[S], fl[S];
+#pragma unroll
+            for (int q = 0; q < S; ++q) {
+                const char* xa = x + (ks * 32 + 8 * kc + (m16 >> 2)) * xs + (ct + q) * 32 + (m16 & 3) * 8;
+                struct { v4s_t lo, hi; } u;
+                u.lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s_t*)(xa));
+                u.hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s_t*)(xa + 4 * xs));
+                fh[q] = __builtin_bit_cast(f16x8_t, u);
+                u.lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s_t*)(xa + xplane));
+                u.hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s_t*)(xa + xplane + 4 * xs));
+                fl[q] = __builtin_bit_cast(f16x8_t, u);
+            }
+#pragma unroll
+            for (int t = 0; t < 2 * D; ++t) {
+                const char* qa = reg + (t * 16 + m16) * N::AROW + ks * 64 + kc * 16;
+                const f16x8_t sh = *reinterpret_cast<const f16x8_t*>(qa), sl = *reinterpret_cast<const f16x8_t*>(qa + N::APLANE);
+#pragma unroll
+                for (int q = 0; q < S; ++q) acc[q][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fl[q], sh, acc[q][t], 0, 0, 0);
+#pragma unroll
+                for (int q = 0; q < S; ++q) acc[q][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fh[q], sl, acc[q][t], 0, 0, 0);
+#pragma unroll
+                for (int q = 0; q < S; ++q) acc[q][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fh[q], sh, acc[q][t], 0, 0, 0);
+            }
+        }
+#pragma unroll
+        for (int q = 0; q < S; ++q)
+#pragma unroll
+            for (int t = 0; t < 2 * D; ++t) out(t * 16 + m16, (ct + q) * 16 + 4 * kc, acc[q][t]);
+    }
+    template <typename F> __device__ __forceinline__ void strips(F&& out) const {
+        const int n = W / 16;                                                 // (even)
+        if constexpr (W_MAX[D] / 16 >= 2 * NWAVES) {
+            if (n >= 2 * NWAVES) {
+                for (int ct = 2 * wave; ct < n; ct += 2 * NWAVES) strip<2>(ct, out);
+                return;
+            }
+        }
+        for (int ct = wave; ct < n; ct += NWAVES) strip<1>(ct, out);
+    }
+    __device__ __forceinline__ void update(float scale) const {
+        strips([&](int i, int j, const f32x4_t& v) {
+            H4 h, l;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) split16(v[e] * scale, h.h[e], l.h[e]);
+            *reinterpret_cast<uint2*>(x + i * xs + j * 2) = h.u;
+            *reinterpret_cast<uint2*>(x + xplane + i * xs + j * 2) = l.u;
+        });
+        __syncthreads();
+    }
+    // the last step: results go back in place as the two halves of their fp32 bits, then out in whole rows of the matrix
+    __device__ __forceinline__ void finish(const Rec& r, const StageP& p, float scale, int j0) const {
+        strips([&](int i, int j, const f32x4_t& v) {
+            uint32_t u[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) u[e] = __float_as_uint(v[e] * scale);
+            *reinterpret_cast<uint2*>(x + i * xs + j * 2) = make_uint2((u[0] >> 16) | (u[1] & 0xffff0000u), (u[2] >> 16) | (u[3] & 0xffff0000u));
+            *reinterpret_cast<uint2*>(x + xplane + i * xs + j * 2) = make_uint2((u[0] & 0xffffu) | (u[1] << 16), (u[2] & 0xffffu) | (u[3] << 16));
+        });
+        __syncthreads();
+        const float lr = p.lr * (r.lr_scale ? fabsf(*r.lr_scale) : 1.f);
+        const int jn = min(W, r.n - j0), cols = r.turned ? r.d : jn, total = r.d * jn;
+        int a = threadIdx.x / cols, c = threadIdx.x % cols;                    // output row (of this slab) and column
+        const int da = NW_T / cols, dc = NW_T % cols, row0 = r.turned ? j0 : 0, col0 = r.turned ? 0 : j0;
+        constexpr int U = 8;
+        for (int e = threadIdx.x; e < total; e += U * NW_T) {
+            float v[U], w[U];
+            int64_t at[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const bool in = e + u * NW_T < total;
+                const int ra = in ? a : 0, rc = in ? c : 0, o = (r.turned ? rc : ra) * xs + (r.turned ? ra : rc) * 2;
+                at[u] = (row0 + ra) * r.ldo + col0 + rc;
+                v[u] = __uint_as_float(((uint32_t)*reinterpret_cast<const uint16_t*>(x + o) << 16) | *reinterpret_cast<const uint16_t*>(x + xplane + o));
+                if (p.muon) w[u] = ((const float*)r.o)[at[u]];
+                a += da;
+                c += dc;
+                if (c >= cols) c -= cols, ++a;
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (e + u * NW_T >= total) break;
+                if (!p.muon) st_any(r.o, at[u], v[u], p.o_dtype);
+                else {
+                    const float nw = fmaf(-lr * r.out_scale, v[u], w[u] - lr * p.wd * w[u]);
+                    ((float*)r.o)[at[u]] = nw;
+                    if (r.p16) {
+                        const bf16_t hi = f2bf(nw);
+                        r.p16[at[u]] = hi;
+                        if (r.p16lo) r.p16lo[at[u]] = f2bf(nw - bf2f(hi));
+                    }
+                }
+            }
+        }
+    }
+};
+
+// one matrix per workgroup, start to end
+template <int D> __global__ __launch_bounds__(NW_T, 2) void muon_narrow_kernel(const NarrowP p, const Recs recs) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    __shared__ double red[NWAVES];
+    const Rec& r = recs.r[blockIdx.x];
+    const StageP& sp = p.s;
+    const Slab<D> L(smem, r.W);
+    double s = L.template load<true>(r, sp, grad_scale_of(sp.gscale, sp.sqnorm, sp.max_norm), 0);
+    for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o, 64);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+    __syncthreads();
+    s = 0.0;
+#pragma unroll
+    for (int i = 0; i < NWAVES; ++i) s += red[i];
+    L.normalise(s < INFINITY ? (double)sp.out_exp / (sqrt(s) + (double)sp.eps) : (double)NAN);
+    for (int k = 0; k < p.steps; ++k) {
+        L.gram_planes(p.ascale[k]);
+        L.square(p.a[k], p.b[k], p.c[k], p.qscale[k], r.d);
+        if (k + 1 < p.steps) L.update(p.xscale[k]);
+        else L.finish(r, sp, p.xscale[k], 0);
+    }
+}
+
+// one slab per workgroup, one step per launch
+template <int D> __global__ __launch_bounds__(NW_T, 2) void muon_slab_kernel(const NarrowP p) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    typedef Narrow<D> N;
+    const StageP& sp = p.s;
+    const Rec r = find(sp.table, sp.firsts + SYM * sp.count, sp.count, blockIdx.x);
+    const int slab = blockIdx.x - r.first[SYM], slabs = (r.n + r.W - 1) / r.W;
+    const Slab<D> L(smem, r.W);
+    char* xg = reinterpret_cast<char*>(sp.planes + r.x0) + (int64_t)slab * 2 * N::DP * r.W * 2;       // this slab's planes, rows of W columns
+    const int cpr = r.W / 8;
+    const float* part_in = reinterpret_cast<const float*>(sp.planes + (p.k & 1 ? r.bm : r.am));
+    float* part_out = reinterpret_cast<float*>(sp.planes + (p.mode == N_INIT || (p.k & 1) ? r.am : r.bm));
+    if (p.mode == N_INIT) {
+        __shared__ double s_sum;
+        if (threadIdx.x < 64) {
+            double s = 0.0;
+            for (int i = threadIdx.x; i < r.nb; i += 64) s += sp.part[r.part0 + i];
+            for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o, 64);
+            if (threadIdx.x == 0) s_sum = s;
+        }
+        L.template load<false>(r, sp, grad_scale_of(sp.gscale, sp.sqnorm, sp.max_norm), slab * r.W);
+        const double s = s_sum;                                               // (load has a barrier)
+        L.normalise(s < INFINITY ? (double)sp.out_exp / (sqrt(s) + (double)sp.eps) : (double)NAN);
+    } else {
+        for (int c = threadIdx.x; c < 2 * N::DP * cpr; c += NW_T) {
+            const int row = c / cpr, q = c - row * cpr;
+            *reinterpret_cast<u32x4_t*>(L.x + row * L.xs + q * 16) = *reinterpret_cast<const u32x4_t*>(xg + (int64_t)c * 16);
+        }
+        L.fold(part_in, slabs, p.ascale[p.k], false);
+        L.square(p.a[p.k], p.b[p.k], p.c[p.k], p.qscale[p.k], r.d);
+        if (p.mode == N_LAST) return L.finish(r, sp, p.xscale[p.k], slab * r.W);
+        L.update(p.xscale[p.k]);
+    }
+    typename Slab<D>::Tile acc[N::ROUNDS];
+    L.gram(acc);
+    part_out += (int64_t)slab * N::NM * 1024;
+    float* to = N::PARTS > 1 ? reinterpret_cast<float*>(L.reg) : part_out;
+#pragma unroll
+    for (int u = 0; u < N::ROUNDS; ++u)
+        if (L.wave + u * NWAVES < N::ITEMS) L.put_tile(to + (L.wave + u * NWAVES) * 1024, acc[u]);
+    if constexpr (N::PARTS > 1) {
+        __syncthreads();
+        float v[2 * N::NM];
+        L.sum_tiles(to, N::PARTS, v);
+#pragma unroll
+        for (int m = 0; m < 2 * N::NM; ++m) part_out[m * 512 + threadIdx.x] = v[m];
+    }
+    for (int c = threadIdx.x; c < 2 * N::DP * cpr; c += NW_T) {
+        const int row = c / cpr, q = c - row * cpr;
+        *reinterpret_cast<u32x4_t*>(xg + (int64_t)c * 16) = *reinterpret_cast<const u32x4_t*>(L.x + row * L.xs + q * 16);
+    }
 }
 
 // ---- host -----------------------------------------------------------------------------------------------------------------
+struct Tiles { int sym, upd; };                // tile edges of the symmetric and the update products
 struct Layout {
-    int64_t table, part, planes, total;      // byte offsets
-    int parts, sym, upd, pack;
+    int64_t table, firsts, part, planes, total;      // byte offsets
+    int64_t plane_elems;
+    int count, parts, maxW, tiles[GRIDS];
 };
+int esize(int dt) { return dt == POET_F32 ? 4 : 2; }
 int up(int v, int m) { return (v + m - 1) / m * m; }
 
-int tile_of(const int* rows, const int* cols, int n) {
-    // 128 x 128 tiles halve the operand traffic per product, 64 x 64 tiles make four times as many workgroups: the large tiles once they
-    // fill half the chip in the update products
-    int64_t tiles = 0;
-    for (int i = 0; i < n; ++i) tiles += (int64_t)cdiv(rows[i], 128) * cdiv(cols[i], 128);
-    return tiles >= 128 ? 128 : 64;
+// How a matrix is worked on, from its own shape alone (so that its result does not depend on what else is in the list):
+// 0 = the chain, D = one workgroup (d <= 32 D), MAX_D + D = slabs
+constexpr int GROUPS = 2 * MAX_D + 1;
+int group_of(int rows, int cols, int& W) {
+    const int d = rows < cols ? rows : cols, n = rows < cols ? cols : rows, D = cdiv(d, 32);
+    W = 0;
+    if (D > MAX_D) return 0;
+    const int slabs = cdiv(n, W_MAX[D]);
+    if (slabs > MAX_SLABS) return 0;
+    W = up(cdiv(n, slabs), 32);
+    return slabs == 1 ? D : MAX_D + D;
 }
 
-// fills the shape-dependent members of rec (when given) and the layout; false: too large
-bool layout(const int* rows, const int* cols, int n, int T, Layout& L, Rec* rec) {
-    int64_t planes = 0, sym = 0, upd = 0, pack = 0, parts = 0;
+Tiles tiles_of(const int* rows, const int* cols, int n) {
+    // 128 x 128 tiles halve the operand traffic per product, 64 x 64 tiles make (up to) four times as many workgroups: the large ones once
+    // they fill the chip: 2048 x 2048, 256 update tiles: 930 us against 1011; 180 tiles (an encoder's 30 matrices): 296 against 289; symmetric
+    // products twice (two workgroups a CU): 4 x 4096 x 1024, 144 tiles: 1509 against 1374
+    int64_t sym = 0, upd = 0;
     for (int i = 0; i < n; ++i) {
+        int W;
+        if (group_of(rows[i], cols[i], W)) continue;
+        const int64_t td = cdiv(rows[i] < cols[i] ? rows[i] : cols[i], 128);
+        sym += td * (td + 1) / 2;
+        upd += (int64_t)cdiv(rows[i], 128) * cdiv(cols[i], 128);
+    }
+    return {sym >= 512 ? 128 : 64, upd >= 256 ? 128 : 64};
+}
+
+// the records of one group among matrices [first, n) (at most `most` of them): shape-dependent members into rec (when given), sizes into L;
+// returns the index behind the last one taken, or -1: too large
+int layout(const int* rows, const int* cols, int first, int n, int group, Tiles T, int most, Layout& L, Rec* rec) {
+    const int P = T.sym > T.upd ? T.sym : T.upd;             // planes hold whole tiles of either kind
+    int64_t planes = 0, parts = 0, tiles[GRIDS] = {0, 0, 0};
+    int i = first, count = 0;
+    L.maxW = 0;
+    for (; i < n && count < most; ++i) {
         Rec r = {};
+        if (group_of(rows[i], cols[i], r.W) != group) continue;
         r.rows = rows[i];
         r.cols = cols[i];
         r.turned = rows[i] > cols[i];
         r.d = r.turned ? cols[i] : rows[i];
         r.n = r.turned ? rows[i] : cols[i];
-        r.dp = up(r.d, T);
-        r.np = up(r.n, T);
-        r.x0 = planes;
-        r.x1 = r.x0 + 2 * (int64_t)r.dp * r.np;
-        r.am = r.x1 + 2 * (int64_t)r.dp * r.np;
-        r.bm = r.am + 2 * (int64_t)r.dp * r.dp;
-        planes = r.bm + 2 * (int64_t)r.dp * r.dp;
         const int64_t e = (int64_t)r.rows * r.cols;
         r.nb = (int)(e > 256ll * NORM_ELEMS ? 256 : cdiv(e, NORM_ELEMS));
-        const int64_t td = r.dp / T, tn = r.np / T;
-        if (sym + td * (td + 1) / 2 > (1 << 29) || upd + td * tn > (1 << 29) || pack + (int64_t)(r.dp / 64) * (r.np / 64) > (1 << 29)) return false;
+        int64_t mine[GRIDS] = {0, 0, 0};
+        r.x0 = planes;
+        if (group == 0) {
+            r.dp = up(r.d, P);
+            r.np = up(r.n, P);
+            r.x1 = r.x0 + 2 * (int64_t)r.dp * r.np;
+            r.am = r.x1 + 2 * (int64_t)r.dp * r.np;
+            r.bm = r.am + 2 * (int64_t)r.dp * r.dp;
+            planes = r.bm + 2 * (int64_t)r.dp * r.dp;
+            const int64_t td = cdiv(r.d, T.sym);
+            mine[SYM] = td * (td + 1) / 2;
+            mine[UPD] = (int64_t)cdiv(r.d, T.upd) * (r.np / T.upd);
+            mine[PACK] = (int64_t)(r.dp / 64) * (r.np / 64);
+        } else if (group > MAX_D) {
+            const int D = group - MAX_D, slabs = cdiv(r.n, r.W);
+            const int64_t gram = (int64_t)slabs * D * (D + 1) / 2 * 2048;       // fp32 partial tiles, in 16-bit elements
+            r.am = r.x0 + (int64_t)slabs * 2 * 32 * D * r.W;
+            r.bm = r.am + gram;
+            planes = r.bm + gram;
+            mine[SYM] = slabs;
+        }
+        if (r.W > L.maxW) L.maxW = r.W;
         r.part0 = (int)parts;
-        r.sym0 = (int)sym;
-        r.upd0 = (int)upd;
-        r.pack0 = (int)pack;
         parts += r.nb;
-        sym += td * (td + 1) / 2;
-        upd += td * tn;
-        pack += (int64_t)(r.dp / 64) * (r.np / 64);
-        if (rec) rec[i] = r;
+        for (int k = 0; k < GRIDS; ++k) {
+            if (tiles[k] + mine[k] > (1 << 29)) return -1;
+            r.first[k] = (int)tiles[k];
+            tiles[k] += mine[k];
+        }
+        if (rec) rec[count] = r;
+        ++count;
     }
+    L.count = count;
     L.parts = (int)parts;
-    L.sym = (int)sym;
-    L.upd = (int)upd;
-    L.pack = (int)pack;
+    L.plane_elems = planes;
+    for (int k = 0; k < GRIDS; ++k) L.tiles[k] = (int)tiles[k];
     L.table = 0;
-    L.part = ((int64_t)n * sizeof(Rec) + 15) / 16 * 16;
+    L.firsts = ((int64_t)count * sizeof(Rec) + 15) / 16 * 16;
+    L.part = (L.firsts + (int64_t)count * GRIDS * 4 + 15) / 16 * 16;
     L.planes = (L.part + parts * 8 + 255) / 256 * 256;
-    L.total = L.planes + planes * 2;
-    return true;
+    L.total = (L.planes + planes * 2 + 255) / 256 * 256;
+    if (group > 0 && group <= MAX_D) L.total = 0;            // (all in LDS)
+    return i;
 }
 
 // exponents that keep X_k, A and q of every step within a quarter of fp16's range; false: the iteration leaves any useful range
@@ -519,35 +1131,89 @@ struct Job {
     const float* sqnorm;
 };
 
-template <int T, int BK> void chain(const Layout& L, const Job& j, const Steps& S, char* ws, hipStream_t st) {
+template <int Q> void sym_product(int T, const StageP& p, hipStream_t st) {
+    if (T == 128) hipLaunchKernelGGL((muon_sym_kernel<128, 32, Q>), dim3(p.total), dim3(NT), 0, st, p);
+    else hipLaunchKernelGGL((muon_sym_kernel<64, 64, Q>), dim3(p.total), dim3(NT), 0, st, p);
+}
+template <bool LAST> void update_product(int T, const StageP& p, hipStream_t st) {
+    if (T == 128) hipLaunchKernelGGL((muon_update_kernel<128, 32, LAST>), dim3(p.total), dim3(NT), 0, st, p);
+    else hipLaunchKernelGGL((muon_update_kernel<64, 64, LAST>), dim3(p.total), dim3(NT), 0, st, p);
+}
+StageP stage_params(const Layout& L, const Job& j, const Steps& S, char* ws) {
     StageP p = {};
     p.table = (const Rec*)(ws + L.table);
+    p.firsts = (const int*)(ws + L.firsts);
     p.part = (const double*)(ws + L.part);
     p.planes = (_Float16*)(ws + L.planes);
-    p.count = j.n;
+    p.count = L.count;
     p.g_dtype = j.g_dtype; p.o_dtype = j.o_dtype; p.muon = j.muon; p.nesterov = j.nesterov;
     p.mu = (float)j.mu; p.omu = (float)(1.0 - j.mu); p.eps = j.eps; p.gscale = j.gscale; p.max_norm = j.max_norm; p.sqnorm = j.sqnorm;
     p.lr = j.lr; p.wd = j.wd;
     p.out_exp = pow2(S.ex[0]);
-    hipLaunchKernelGGL(muon_pack_kernel, dim3(L.pack), dim3(NT), 0, st, p);
+    return p;
+}
+void chain(Tiles T, const Layout& L, const Job& j, const Steps& S, char* ws, hipStream_t st) {
+    StageP p = stage_params(L, j, S, ws);
+    hipLaunchKernelGGL(muon_pack_kernel, dim3(L.tiles[PACK]), dim3(NT), 0, st, p);
     for (int k = 0; k < j.steps; ++k) {
         p.flip = k & 1;
-        p.total = L.sym;
+        p.total = L.tiles[SYM];
         p.in_scale = pow2(-2 * S.ex[k]);
         p.out_exp = pow2(S.ea[k]);
-        hipLaunchKernelGGL((muon_sym_kernel<T, BK, 0>), dim3(L.sym), dim3(NT), 0, st, p);
+        sym_product<0>(T.sym, p, st);
         p.a = (float)j.coeffs[3 * k];
         p.b = (float)(j.coeffs[3 * k + 1] * pow2(-S.ea[k]));
         p.c = (float)j.coeffs[3 * k + 2];
         p.in_scale = pow2(-2 * S.ea[k]);
         p.out_exp = pow2(S.eq[k]);
-        hipLaunchKernelGGL((muon_sym_kernel<T, BK, 1>), dim3(L.sym), dim3(NT), 0, st, p);
-        p.total = L.upd;
+        sym_product<1>(T.sym, p, st);
+        p.total = L.tiles[UPD];
         p.in_scale = pow2(-S.eq[k] - S.ex[k]);
         p.out_exp = pow2(S.ex[k + 1]);
-        if (k + 1 < j.steps) hipLaunchKernelGGL((muon_update_kernel<T, BK, false>), dim3(L.upd), dim3(NT), 0, st, p);
-        else hipLaunchKernelGGL((muon_update_kernel<T, BK, true>), dim3(L.upd), dim3(NT), 0, st, p);
+        if (k + 1 < j.steps) update_product<false>(T.upd, p, st);
+        else update_product<true>(T.upd, p, st);
     }
+}
+NarrowP narrow_params(const Layout& L, const Job& j, const Steps& S, char* ws) {
+    NarrowP p = {};
+    p.s = stage_params(L, j, S, ws);
+    p.steps = j.steps;
+    for (int k = 0; k < j.steps; ++k) {
+        p.a[k] = (float)j.coeffs[3 * k];
+        p.b[k] = (float)(j.coeffs[3 * k + 1] * pow2(-S.ea[k]));
+        p.c[k] = (float)(j.coeffs[3 * k + 2] * pow2(-2 * S.ea[k]));
+        p.ascale[k] = pow2(S.ea[k] - 2 * S.ex[k]);
+        p.qscale[k] = pow2(S.eq[k]);
+        p.xscale[k] = pow2((k + 1 < j.steps ? S.ex[k + 1] : 0) - S.eq[k] - S.ex[k]);
+    }
+    return p;
+}
+template <int D> int narrow_lds(int W) { return Narrow<D>::REGION + 2 * Narrow<D>::DP * (W * 2 + 16); }
+template <int D> void narrow_single(const NarrowP& p, const Recs& recs, int count, int W, hipStream_t st) {
+    static unsigned long long done = 0;
+    static_assert(Narrow<D>::REGION + 2 * Narrow<D>::DP * (W_MAX[D] * 2 + 16) + 256 <= 160 * 1024, "LDS");
+    lds_attr_once((const void*)muon_narrow_kernel<D>, narrow_lds<D>(W_MAX[D]), done);
+    hipLaunchKernelGGL((muon_narrow_kernel<D>), dim3(count), dim3(NW_T), narrow_lds<D>(W), st, p, recs);
+}
+template <int D> void narrow_slabs(NarrowP p, const Layout& L, hipStream_t st) {
+    static unsigned long long done = 0;
+    lds_attr_once((const void*)muon_slab_kernel<D>, narrow_lds<D>(W_MAX[D]), done);
+    for (int k = -1; k < p.steps; ++k) {
+        p.mode = k < 0 ? N_INIT : k + 1 < p.steps ? N_STEP : N_LAST;
+        p.k = k < 0 ? 0 : k;
+        hipLaunchKernelGGL((muon_slab_kernel<D>), dim3(L.tiles[SYM]), dim3(NW_T), narrow_lds<D>(L.maxW), st, p);
+    }
+}
+
+// bytes of all groups (at least one aligned block), -1: too large
+int64_t workspace_of(const int* rows, const int* cols, int n, Tiles T) {
+    int64_t need = 0;
+    for (int group = 0; group < GROUPS; ++group) {
+        Layout L;
+        if (layout(rows, cols, 0, n, group, T, n, L, nullptr) < 0) return -1;
+        need += L.total;
+    }
+    return need > 256 ? need : 256;
 }
 
 int run_job(const char* what, const Job& j, void* ws, int64_t ws_bytes, void* stream) {
@@ -561,50 +1227,75 @@ int run_job(const char* what, const Job& j, void* ws, int64_t ws_bytes, void* st
     }
     Steps S;
     POET_CHECK(ranges(j.coeffs, j.steps, S), POET_ERR_ARG, "%s: these coefficients leave the range the iteration can hold", what);
-    const int T = tile_of(j.rows, j.cols, j.n);
-    Layout L;
-    POET_CHECK(layout(j.rows, j.cols, j.n, T, L, nullptr), POET_ERR_UNSUPPORTED, "%s: too many tiles", what);
-    POET_CHECK(ws && ((uintptr_t)ws % 256) == 0 && ws_bytes >= L.total, POET_ERR_ARG, "%s: workspace of %lld bytes needed (256-byte aligned), %lld given", what,
-               (long long)L.total, (long long)ws_bytes);
+    const Tiles T = tiles_of(j.rows, j.cols, j.n);
+    const int64_t need = workspace_of(j.rows, j.cols, j.n, T);
+    POET_CHECK(need >= 0, POET_ERR_UNSUPPORTED, "%s: too many tiles", what);
+    POET_CHECK(ws && ((uintptr_t)ws % 256) == 0 && ws_bytes >= need, POET_ERR_ARG, "%s: workspace of %lld bytes needed (256-byte aligned), %lld given", what,
+               (long long)need, (long long)ws_bytes);
     hipStream_t st = (hipStream_t)stream;
-    NormP np = {};
-    np.table = (Rec*)((char*)ws + L.table);
-    np.part = (double*)((char*)ws + L.part);
-    np.g_dtype = j.g_dtype; np.muon = j.muon; np.nesterov = j.nesterov;
-    np.mu = (float)j.mu; np.omu = (float)(1.0 - j.mu); np.gscale = j.gscale; np.max_norm = j.max_norm; np.sqnorm = j.sqnorm;
-    int64_t base[4] = {0, 0, 0, 0};                       // planes, partials | tiles before this chunk
-    int sym = 0, upd = 0, pack = 0;
-    for (int f = 0; f < j.n; f += CHUNK) {
-        Recs recs = {};
-        const int c = j.n - f < CHUNK ? j.n - f : CHUNK;
-        Layout C;
-        layout(j.rows + f, j.cols + f, c, T, C, recs.r);
-        int blocks = 0;
-        for (int i = 0; i < c; ++i) {
-            Rec& r = recs.r[i];
-            r.x0 += base[0]; r.x1 += base[0]; r.am += base[0]; r.bm += base[0];
-            r.part0 += (int)base[1];
-            r.sym0 += sym; r.upd0 += upd; r.pack0 += pack;
-            r.g = j.g[f + i];
-            r.o = j.o[f + i];
-            r.mom = j.muon ? j.mom[f + i] : nullptr;
-            r.p16 = j.p16 ? j.p16[f + i] : nullptr;
-            r.p16lo = j.p16lo ? j.p16lo[f + i] : nullptr;
-            r.lr_scale = j.lr_scale ? j.lr_scale[f + i] : nullptr;
-            r.ldg = j.ldg ? j.ldg[f + i] : r.cols;
-            r.ldo = j.ldo ? j.ldo[f + i] : r.cols;
-            r.out_scale = j.out_scale ? j.out_scale[f + i] : 1.f;
-            blocks += r.nb;
+    char* base = (char*)ws;
+    for (int group = 0; group < GROUPS; ++group) {
+        Layout L;
+        layout(j.rows, j.cols, 0, j.n, group, T, j.n, L, nullptr);
+        if (!L.count) continue;
+        const bool single = group > 0 && group <= MAX_D;
+        NormP np = {};
+        np.table = (Rec*)(base + L.table);
+        np.firsts = (int*)(base + L.firsts);
+        np.part = (double*)(base + L.part);
+        np.n = L.count;
+        np.g_dtype = j.g_dtype; np.muon = j.muon; np.nesterov = j.nesterov;
+        np.mu = (float)j.mu; np.omu = (float)(1.0 - j.mu); np.gscale = j.gscale; np.max_norm = j.max_norm; np.sqnorm = j.sqnorm;
+        const NarrowP narrow = narrow_params(L, j, S, base);
+        int64_t planes = 0;                                   // of the chunks before this one
+        int parts = 0, tiles[GRIDS] = {0, 0, 0};
+        for (int at = 0; np.first < L.count;) {
+            Recs recs = {};
+            Layout C;
+            const int from = at;
+            at = layout(j.rows, j.cols, from, j.n, group, T, CHUNK, C, recs.r);
+            int blocks = 0;
+            for (int i = from, c = 0; c < C.count; ++i) {
+                int W;
+                if (group_of(j.rows[i], j.cols[i], W) != group) continue;
+                Rec& r = recs.r[c++];
+                r.x0 += planes; r.x1 += planes; r.am += planes; r.bm += planes;
+                r.part0 += parts;
+                for (int k = 0; k < GRIDS; ++k) r.first[k] += tiles[k];
+                r.g = j.g[i];
+                r.o = j.o[i];
+                r.mom = j.muon ? j.mom[i] : nullptr;
+                r.p16 = j.p16 ? j.p16[i] : nullptr;
+                r.p16lo = j.p16lo ? j.p16lo[i] : nullptr;
+                r.lr_scale = j.lr_scale ? j.lr_scale[i] : nullptr;
+                r.ldg = j.ldg ? j.ldg[i] : r.cols;
+                r.ldo = j.ldo ? j.ldo[i] : r.cols;
+                r.out_scale = j.out_scale ? j.out_scale[i] : 1.f;
+                const int ge = esize(j.g_dtype), oe = esize(j.o_dtype), gw = 16 / ge;
+                r.gvec = r.ldg == r.cols && (int64_t)r.rows * r.cols % gw == 0 && ((uintptr_t)r.g | (uintptr_t)r.mom) % 16 == 0;
+                r.ovec = r.cols % 4 == 0 && r.ldo % 4 == 0 && (uintptr_t)r.o % (4 * oe) == 0 && ((uintptr_t)r.p16 | (uintptr_t)r.p16lo) % 8 == 0;
+                blocks += r.nb;
+            }
+            np.count = C.count;
+            if (!single) hipLaunchKernelGGL(muon_norm_kernel, dim3(blocks), dim3(NT), 0, st, np, recs);
+            else if (group == 1) narrow_single<1>(narrow, recs, C.count, C.maxW, st);
+            else if (group == 2) narrow_single<2>(narrow, recs, C.count, C.maxW, st);
+            else if (group == 3) narrow_single<3>(narrow, recs, C.count, C.maxW, st);
+            else if (group == 4) narrow_single<4>(narrow, recs, C.count, C.maxW, st);
+            else narrow_single<5>(narrow, recs, C.count, C.maxW, st);
+            planes += C.plane_elems;
+            parts += C.parts;
+            for (int k = 0; k < GRIDS; ++k) tiles[k] += C.tiles[k];
+            np.first += C.count;
         }
-        np.first = f;
-        np.count = c;
-        hipLaunchKernelGGL(muon_norm_kernel, dim3(blocks), dim3(NT), 0, st, np, recs);
-        base[0] += (C.total - C.planes) / 2;
-        base[1] += C.parts;
-        sym += C.sym; upd += C.upd; pack += C.pack;
+        if (group == 0) chain(T, L, j, S, base, st);
+        else if (group == MAX_D + 1) narrow_slabs<1>(narrow, L, st);
+        else if (group == MAX_D + 2) narrow_slabs<2>(narrow, L, st);
+        else if (group == MAX_D + 3) narrow_slabs<3>(narrow, L, st);
+        else if (group == MAX_D + 4) narrow_slabs<4>(narrow, L, st);
+        else if (group == MAX_D + 5) narrow_slabs<5>(narrow, L, st);
+        base += L.total;
     }
-    if (T == 128) chain<128, 32>(L, j, S, (char*)ws, st);
-    else chain<64, 64>(L, j, S, (char*)ws, st);
     POET_LAUNCH_CHECK();
     return POET_OK;
 }
@@ -619,9 +1310,9 @@ extern "C" int64_t poet_muon_workspace(const int* rows_host, const int* cols_hos
     POET_CHECK(rows_host && cols_host && n > 0, POET_ERR_ARG, "muon_workspace: null list or no matrices");
     for (int i = 0; i < n; ++i)
         POET_CHECK(rows_host[i] > 0 && cols_host[i] > 0 && rows_host[i] <= (1 << 20) && cols_host[i] <= (1 << 20), POET_ERR_ARG, "muon_workspace: matrix %d is %d x %d", i, rows_host[i], cols_host[i]);
-    Layout L;
-    POET_CHECK(layout(rows_host, cols_host, n, tile_of(rows_host, cols_host, n), L, nullptr), POET_ERR_UNSUPPORTED, "muon_workspace: too many tiles");
-    return L.total;
+    const int64_t need = workspace_of(rows_host, cols_host, n, tiles_of(rows_host, cols_host, n));
+    POET_CHECK(need >= 0, POET_ERR_UNSUPPORTED, "muon_workspace: too many tiles");
+    return need;
 }
 
 extern "C" int poet_orthogonalize(const void* const* g_host, const int64_t* ldg_host, void* const* o_host, const int64_t* ldo_host, const int* rows_host,
