@@ -65,22 +65,38 @@ struct NormP {
     float mu, omu, gscale, max_norm;       // momentum, 1 - momentum (each rounded once)
     const float* sqnorm;
 };
-struct StageP {
-    const Rec* table;
-    const int* firsts;
-    const double* part;
+// what a product needs of a record
+struct Shape {
+    int64_t x0, x1, am, bm;
+    int d, n, dp, np;
+};
+struct StageP {                            // (what every launch of a chain reads first lies in its first 128 bytes: two lines of the scalar cache)
     _Float16* planes;
-    int count, total;                      // matrices, workgroups
-    int g_dtype, o_dtype, muon, nesterov;
-    float mu, omu, eps;
-    float gscale, max_norm;
-    const float* sqnorm;
+    int64_t stride;                        // > 0: all matrices are of the shape `uniform` (the first one's), matrix k's planes lie k * stride further
+    Shape uniform;
+    int per[2];                            // ... and has this many tiles (SYM, UPD)
+    int total;                             // workgroups
+    int flip;                              // which X buffer holds the input
     float in_scale;                        // 2^-(exponents of the two operands)
     float out_exp;                         // 2^(exponent of the result)
     float a, b, c;                         // q stage; b carries A's exponent
-    int flip;                              // which X buffer holds the input
-    float lr, wd;
+    int count;                             // matrices
+    const Rec* table;
+    const int* firsts;
+    const double* part;
+    const float* sqnorm;
+    int g_dtype, o_dtype, muon, nesterov;
+    float mu, omu, eps, gscale, max_norm, lr, wd;
 };
+
+// a / b for 0 <= a < 2^30, 0 < b, and the remainder (the compiler's exact division costs a launch of these sizes several hundred cycles)
+__device__ __forceinline__ int divide(int a, int b, int& rem) {
+    int q = (int)((float)a * __builtin_amdgcn_rcpf((float)b));
+    rem = a - q * b;
+    while (rem < 0) --q, rem += b;
+    while (rem >= b) ++q, rem -= b;
+    return q;
+}
 
 template <typename T> __device__ __forceinline__ float ld1(const void* p, int64_t i) { return io<T>::ld((const T*)p + i); }
 __device__ __forceinline__ float ld_any(const void* p, int64_t i, int dt) {
@@ -176,6 +192,20 @@ __device__ __forceinline__ const Rec& find(const Rec* table, const int* firsts, 
     }
     return table[__builtin_amdgcn_readfirstlane(k)];
 }
+// the shape behind workgroup b of grid G, and its tile; with one shape for all, two dependent loads less at the head of every launch
+template <int G> __device__ __forceinline__ Shape locate(const StageP& p, int b, int& tile) {
+    if (p.stride) {
+        const int k = __builtin_amdgcn_readfirstlane(divide(b, p.per[G], tile));
+        tile = __builtin_amdgcn_readfirstlane(tile);
+        Shape s = p.uniform;
+        const int64_t o = k * p.stride;
+        s.x0 += o; s.x1 += o; s.am += o; s.bm += o;
+        return s;
+    }
+    const Rec& r = find(p.table, p.firsts + G * p.count, p.count, b);
+    tile = b - r.first[G];
+    return {r.x0, r.x1, r.am, r.bm, r.d, r.n, r.dp, r.np};
+}
 __device__ __forceinline__ int xcd_order(int b, int total) {          // workgroup b runs on XCD b % 8: give each a contiguous range of tiles
     const int q = total >> 3, rem = total & 7, x = b & 7;
     return x * q + min(x, rem) + (b >> 3);
@@ -247,15 +277,17 @@ template <int ROWB> __device__ __forceinline__ int swz_col(int krow) {
     else return ((krow >> 1) & 1) | (((krow >> 3) & 1) << 1);
 }
 
-// acc[f][s][r] += sum_k first[f 16 + 4 (lane / 16) + r][k] second[s 16 + lane % 16][k] over a T x T tile, 4 waves of T/2 x T/2.
+// SETS > 1: stage k of BK goes to accumulator set k % SETS, so that the sum has the order of the split kernels below.
+// acc[set][f][s][r] += sum_k first[f 16 + 4 (lane / 16) + r][k] second[s 16 + lane % 16][k] over a T x T tile, 4 waves of T/2 x T/2.
 // second: rows of K contiguous elements.  first: the same, or (KM) stored [k][column].  K % BK == 0; every row / column read exists
 // (planes are padded to whole tiles).
-template <int T, int BK, bool KM> struct Core {
+template <int T, int BK, bool KM, int SETS> struct Core {
     static constexpr int ROWB = BK * 2, CPR = BK / 8, F = T / 32, PLANE = T * BK * 2, STAGE = 4 * PLANE;
     static constexpr int NL = PLANE / 16 / NT;                                            // 16-byte loads per thread and plane
     static constexpr int COLB = T * 2, CPC = T / 8;
+    static constexpr int AHEAD = T == 64 && SETS == 1 ? 4 : 2, UNROLL = SETS > AHEAD ? SETS : AHEAD;      // stages in registers on their way to LDS
     static __device__ __forceinline__ void run(const _Float16* fh, const _Float16* fl, int64_t ldf, const _Float16* sh, const _Float16* sl, int64_t lds_,
-                                               int K, char* smem, f32x4_t (&acc)[F][F]) {
+                                               int K, char* smem, f32x4_t (&acc)[SETS][F][F]) {
         const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wf = (wave >> 1) * (T / 2), ws = (wave & 1) * (T / 2);
         const int m16 = lane & 15, kc = lane >> 4;
         int64_t go[NL], so[NL];
@@ -274,72 +306,75 @@ template <int T, int BK, bool KM> struct Core {
                 lo_f[q] = lo_s[q];
             }
         }
-        u32x4_t rf[2][NL], rs[2][NL];
-        auto fetch = [&](int k) {
+        u32x4_t rf[AHEAD][2][NL], rs[AHEAD][2][NL];
+        auto fetch = [&](int k, u32x4_t (&f)[2][NL], u32x4_t (&s)[2][NL]) {
             const int64_t kf = KM ? (int64_t)k * ldf : k;
 #pragma unroll
             for (int q = 0; q < NL; ++q) {
-                rf[0][q] = *reinterpret_cast<const u32x4_t*>(fh + go[q] + kf);
-                rf[1][q] = *reinterpret_cast<const u32x4_t*>(fl + go[q] + kf);
-                rs[0][q] = *reinterpret_cast<const u32x4_t*>(sh + so[q] + k);
-                rs[1][q] = *reinterpret_cast<const u32x4_t*>(sl + so[q] + k);
+                f[0][q] = *reinterpret_cast<const u32x4_t*>(fh + go[q] + kf);
+                f[1][q] = *reinterpret_cast<const u32x4_t*>(fl + go[q] + kf);
+                s[0][q] = *reinterpret_cast<const u32x4_t*>(sh + so[q] + k);
+                s[1][q] = *reinterpret_cast<const u32x4_t*>(sl + so[q] + k);
             }
         };
-        auto store = [&](char* st) {
+        auto store = [&](char* st, const u32x4_t (&f)[2][NL], const u32x4_t (&s)[2][NL]) {
 #pragma unroll
             for (int q = 0; q < NL; ++q) {
-                *reinterpret_cast<u32x4_t*>(st + lo_f[q]) = rf[0][q];
-                *reinterpret_cast<u32x4_t*>(st + PLANE + lo_f[q]) = rf[1][q];
-                *reinterpret_cast<u32x4_t*>(st + 2 * PLANE + lo_s[q]) = rs[0][q];
-                *reinterpret_cast<u32x4_t*>(st + 3 * PLANE + lo_s[q]) = rs[1][q];
+                *reinterpret_cast<u32x4_t*>(st + lo_f[q]) = f[0][q];
+                *reinterpret_cast<u32x4_t*>(st + PLANE + lo_f[q]) = f[1][q];
+                *reinterpret_cast<u32x4_t*>(st + 2 * PLANE + lo_s[q]) = s[0][q];
+                *reinterpret_cast<u32x4_t*>(st + 3 * PLANE + lo_s[q]) = s[1][q];
             }
         };
-        fetch(0);
-        store(smem);
-        __syncthreads();
-        int cur = 0;
-        for (int k = 0; k < K; k += BK) {
-            const bool more = k + BK < K;
-            if (more) fetch(k + BK);
-            const char* st = smem + cur * STAGE;
 #pragma unroll
-            for (int h = 0; h < BK / 32; ++h) {
-                f16x8_t fhv[F], flv[F];
+        for (int a = 0; a < AHEAD; ++a)
+            if (a * BK < K) fetch(a * BK, rf[a], rs[a]);
+        for (int k0 = 0; k0 < K; k0 += UNROLL * BK) {
 #pragma unroll
-                for (int f = 0; f < F; ++f) {
-                    if constexpr (KM) {
-                        const int kr = h * 32 + 8 * kc + (m16 >> 2), piece = (wf >> 4) + f;
-                        const int a0 = kr * COLB + ((piece ^ swz_col<COLB>(kr)) * 32) + (m16 & 3) * 8;
-                        const int a1 = (kr + 4) * COLB + ((piece ^ swz_col<COLB>(kr + 4)) * 32) + (m16 & 3) * 8;
-                        struct { v4s_t lo, hi; } u;
-                        u.lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s_t*)(st + a0));
-                        u.hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s_t*)(st + a1));
-                        fhv[f] = __builtin_bit_cast(f16x8_t, u);
-                        u.lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s_t*)(st + PLANE + a0));
-                        u.hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s_t*)(st + PLANE + a1));
-                        flv[f] = __builtin_bit_cast(f16x8_t, u);
-                    } else {
-                        const int row = wf + f * 16 + m16, a = row * ROWB + (((h * 4 + kc) ^ swz_row<ROWB>(row)) & (CPR - 1)) * 16;
-                        fhv[f] = *reinterpret_cast<const f16x8_t*>(st + a);
-                        flv[f] = *reinterpret_cast<const f16x8_t*>(st + PLANE + a);
-                    }
-                }
+            for (int a = 0; a < UNROLL; ++a) {
+                const int k = k0 + a * BK;
+                if (k >= K) break;
+                char* st = smem + (a & 1) * STAGE;
+                store(st, rf[a % AHEAD], rs[a % AHEAD]);          // (this slot's readers, two stages back, passed the barrier of the stage between)
+                __syncthreads();
+                if (k + AHEAD * BK < K) fetch(k + AHEAD * BK, rf[a % AHEAD], rs[a % AHEAD]);
+                stage(st, acc[a % SETS], wf, ws, m16, kc);
+            }
+        }
+    }
+    static __device__ __forceinline__ void stage(const char* st, f32x4_t (&acc)[F][F], int wf, int ws, int m16, int kc) {
 #pragma unroll
-                for (int s = 0; s < F; ++s) {
-                    const int row = ws + s * 16 + m16, a = row * ROWB + (((h * 4 + kc) ^ swz_row<ROWB>(row)) & (CPR - 1)) * 16;
-                    const f16x8_t shv = *reinterpret_cast<const f16x8_t*>(st + 2 * PLANE + a), slv = *reinterpret_cast<const f16x8_t*>(st + 3 * PLANE + a);
+        for (int h = 0; h < BK / 32; ++h) {
+            f16x8_t fhv[F], flv[F];
 #pragma unroll
-                    for (int f = 0; f < F; ++f) acc[f][s] = __builtin_amdgcn_mfma_f32_16x16x32_f16(flv[f], shv, acc[f][s], 0, 0, 0);
-#pragma unroll
-                    for (int f = 0; f < F; ++f) acc[f][s] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fhv[f], slv, acc[f][s], 0, 0, 0);
-#pragma unroll
-                    for (int f = 0; f < F; ++f) acc[f][s] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fhv[f], shv, acc[f][s], 0, 0, 0);
+            for (int f = 0; f < F; ++f) {
+                if constexpr (KM) {
+                    const int kr = h * 32 + 8 * kc + (m16 >> 2), piece = (wf >> 4) + f;
+                    const int a0 = kr * COLB + ((piece ^ swz_col<COLB>(kr)) * 32) + (m16 & 3) * 8;
+                    const int a1 = (kr + 4) * COLB + ((piece ^ swz_col<COLB>(kr + 4)) * 32) + (m16 & 3) * 8;
+                    struct { v4s_t lo, hi; } u;
+                    u.lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s_t*)(st + a0));
+                    u.hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s_t*)(st + a1));
+                    fhv[f] = __builtin_bit_cast(f16x8_t, u);
+                    u.lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s_t*)(st + PLANE + a0));
+                    u.hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s_t*)(st + PLANE + a1));
+                    flv[f] = __builtin_bit_cast(f16x8_t, u);
+                } else {
+                    const int row = wf + f * 16 + m16, a = row * ROWB + (((h * 4 + kc) ^ swz_row<ROWB>(row)) & (CPR - 1)) * 16;
+                    fhv[f] = *reinterpret_cast<const f16x8_t*>(st + a);
+                    flv[f] = *reinterpret_cast<const f16x8_t*>(st + PLANE + a);
                 }
             }
-            if (more) {
-                store(smem + (cur ^ 1) * STAGE);       // (the slot's readers passed the barrier that ended the last step)
-                __syncthreads();
-                cur ^= 1;
+#pragma unroll
+            for (int s = 0; s < F; ++s) {
+                const int row = ws + s * 16 + m16, a = row * ROWB + (((h * 4 + kc) ^ swz_row<ROWB>(row)) & (CPR - 1)) * 16;
+                const f16x8_t shv = *reinterpret_cast<const f16x8_t*>(st + 2 * PLANE + a), slv = *reinterpret_cast<const f16x8_t*>(st + 3 * PLANE + a);
+#pragma unroll
+                for (int f = 0; f < F; ++f) acc[f][s] = __builtin_amdgcn_mfma_f32_16x16x32_f16(flv[f], shv, acc[f][s], 0, 0, 0);
+#pragma unroll
+                for (int f = 0; f < F; ++f) acc[f][s] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fhv[f], slv, acc[f][s], 0, 0, 0);
+#pragma unroll
+                for (int f = 0; f < F; ++f) acc[f][s] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fhv[f], shv, acc[f][s], 0, 0, 0);
             }
         }
     }
@@ -347,193 +382,384 @@ template <int T, int BK, bool KM> struct Core {
 
 union H4 { _Float16 h[4]; uint2 u; };
 
-// A wave's T/2 x T/2 part of the tile, restaged through LDS so that results leave in whole rows of either orientation (straight from the
-// accumulators a lane owns 4 consecutive columns of one row, the mirror image would leave in 2-byte stores).  16-byte pieces of row i are
-// XORed with i / 4: both the rows and the columns of 4 read back without bank conflicts.
-template <int T> struct Sub {
-    static constexpr int S = T / 2;
-    static __device__ __forceinline__ int at(int i, int piece) { return i * S + ((piece ^ (i >> 2)) & (S / 4 - 1)) * 4; }
-    static __device__ __forceinline__ float* put(char* smem, const f32x4_t (&acc)[T / 32][T / 32], int wave, int lane) {
-        float* sub = reinterpret_cast<float*>(smem) + wave * S * S;
+__device__ __forceinline__ uint2 pack4(const f32x4_t& v, uint2& lo) {          // hi parts; lo: what they leave
+    const uint2 hi = make_uint2(pack_h2(v[0], v[1]), pack_h2(v[2], v[3]));
+    lo = make_uint2(pack_h2(v[0] - h_lo(hi.x), v[1] - h_hi(hi.x)), pack_h2(v[2] - h_lo(hi.y), v[3] - h_hi(hi.y)));
+    return hi;
+}
+__device__ __forceinline__ void store_some(_Float16* o, _Float16* ol, const uint2& hi, const uint2& lo, int first, int last) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (e >= first && e <= last) {
+            reinterpret_cast<uint16_t*>(o)[e] = (uint16_t)((e & 2 ? hi.y : hi.x) >> (e & 1) * 16);
+            reinterpret_cast<uint16_t*>(ol)[e] = (uint16_t)((e & 2 ? lo.y : lo.x) >> (e & 1) * 16);
+        }
+}
+// A T x T fp32 tile in LDS, 16-byte pieces XORed so that rows and columns of 4 read without conflicts.  A workgroup's threads hold it as
+// pieces: piece u of a thread is row u (NT / P) + threadIdx / P, columns 4 (threadIdx % P) .. + 3, P = T / 4.
+template <int T> struct Meet {
+    static constexpr int P = T / 4, U = T * P / NT, F = T / 16;
+    static __device__ __forceinline__ int at(int i, int piece) { return i * T + ((piece ^ (i >> 2)) & (P - 1)) * 4; }
+    static __device__ __forceinline__ int row(int u) { return u * (NT / P) + threadIdx.x / P; }
+    static __device__ __forceinline__ int col() { return (threadIdx.x % P) * 4; }
+    // the tile in the accumulators of four waves of T / 2 x T / 2 -> this thread's pieces
+    static __device__ __forceinline__ void share(float* part, const f32x4_t (&acc)[T / 32][T / 32], int wf, int ws, int m16, int kc, f32x4_t (&v)[U]) {
         __syncthreads();                                                      // (the last stage's operands have been read)
 #pragma unroll
         for (int f = 0; f < T / 32; ++f)
 #pragma unroll
-            for (int s = 0; s < T / 32; ++s) *reinterpret_cast<f32x4_t*>(sub + at(s * 16 + (lane & 15), f * 4 + (lane >> 4))) = acc[f][s];
+            for (int s = 0; s < T / 32; ++s) *reinterpret_cast<f32x4_t*>(part + at(ws + s * 16 + m16, ((wf + f * 16) >> 2) + kc)) = acc[f][s];
         __syncthreads();
-        return sub;
-    }
-    static __device__ __forceinline__ f32x4_t row(const float* sub, int i, int j) { return *reinterpret_cast<const f32x4_t*>(sub + at(i, j >> 2)); }
-    static __device__ __forceinline__ f32x4_t col(const float* sub, int i, int j) {       // elements (i .. i + 3, j)
-        f32x4_t v;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = sub[at(i + e, j >> 2) + (j & 3)];
-        return v;
+        for (int u = 0; u < U; ++u) v[u] = *reinterpret_cast<const f32x4_t*>(part + at(row(u), col() >> 2));
+    }
+    // the partial tiles of the four waves -> this thread's pieces of their sum
+    static __device__ __forceinline__ void sum(float* part, const f32x4_t (&acc)[F][F], int wave, int m16, int kc, f32x4_t (&v)[U]) {
+        float* mine = part + wave * T * T;
+#pragma unroll
+        for (int q = 0; q < F * F; ++q) *reinterpret_cast<f32x4_t*>(mine + at((q % F) * 16 + m16, (q / F) * 4 + kc)) = acc[q / F][q % F];
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const float* t = part + at(row(u), col() >> 2);
+            v[u] = (*reinterpret_cast<const f32x4_t*>(t) + *reinterpret_cast<const f32x4_t*>(t + T * T)) +
+                   (*reinterpret_cast<const f32x4_t*>(t + 2 * T * T) + *reinterpret_cast<const f32x4_t*>(t + 3 * T * T));
+        }
+    }
+    // ... and turned: afterwards v[u][e] is element (col() + e, row(u)).  (Each thread rewrites the pieces that it alone read there.)
+    static __device__ __forceinline__ void turn(float* part, f32x4_t (&v)[U]) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) *reinterpret_cast<f32x4_t*>(part + at(row(u), col() >> 2)) = v[u];
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[u][e] = part[at(col() + e, row(u) >> 2) + (row(u) & 3)];
     }
 };
-
-// A = X X^T (Q = 0), or q = a I + b A + c A A (Q = 1): tiles on and below the diagonal, written twice
-template <int T, int BK, int Q> __global__ __launch_bounds__(NT, 2) void muon_sym_kernel(const StageP p) {
-    __shared__ __attribute__((aligned(16))) char smem[2 * Core<T, BK, false>::STAGE];
-    constexpr int F = T / 32;
-    const int b = xcd_order(blockIdx.x, p.total);
-    const Rec r = find(p.table, p.firsts + SYM * p.count, p.count, b);
-    const int t = b - r.first[SYM], dp = r.dp;
-    int bi = (int)((sqrtf(8.f * (float)t + 1.f) - 1.f) * 0.5f);
-    while ((bi + 1) * (bi + 2) / 2 <= t) ++bi;
-    while (bi * (bi + 1) / 2 > t) --bi;
-    const int i0 = bi * T, j0 = (t - bi * (bi + 1) / 2) * T;
-    const int64_t ld = Q ? dp : r.np, plane = (int64_t)dp * ld;
-    const _Float16* in = p.planes + (Q ? r.am : p.flip ? r.x1 : r.x0);
-    const int K = Q ? (r.d + BK - 1) / BK * BK : (r.n + BK - 1) / BK * BK;
-    f32x4_t acc[F][F];
+// columns col .. col + 3 of a row of the output matrix, or of the weight update
+__device__ __forceinline__ void write4(const Rec& m, const StageP& p, float lr, int row, int col, const f32x4_t& v) {
+    if (row >= m.rows || col >= m.cols) return;
+    const int64_t at = row * m.ldo + col;
+    if (p.muon) {
+        float* w = (float*)m.o + at;
+        if (m.ovec) {                                                         // (cols % 4 == 0)
+            f32x4_t o = *reinterpret_cast<f32x4_t*>(w);
 #pragma unroll
-    for (int f = 0; f < F; ++f)
-#pragma unroll
-        for (int s = 0; s < F; ++s) acc[f][s] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    Core<T, BK, false>::run(in + j0 * ld, in + plane + j0 * ld, ld, in + i0 * ld, in + plane + i0 * ld, ld, K, smem, acc);
-
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wf = (wave >> 1) * (T / 2), ws = (wave & 1) * (T / 2);
-    const int64_t sq = (int64_t)dp * dp;
-    const _Float16* am = p.planes + r.am;
-    _Float16* out = p.planes + (Q ? r.bm : r.am);
-    float* sub = Sub<T>::put(smem, acc, wave, lane);
-    constexpr int LPR = Sub<T>::S / 4;                                        // lanes per row of 4-element pieces
-#pragma unroll
-    for (int it = 0; it < Sub<T>::S * LPR / 64; ++it) {
-        const int li = it * (64 / LPR) + lane / LPR, lj = (lane % LPR) * 4, i = i0 + ws + li, j = j0 + wf + lj;
-        if (i < j) continue;                                                  // (pieces on and below the diagonal; pieces start at multiples of 4)
-        const f32x4_t v = Sub<T>::row(sub, li, lj);
-        H4 h, l;
-        if constexpr (Q) {
-            H4 ah, al;
-            ah.u = *reinterpret_cast<const uint2*>(am + (int64_t)i * dp + j);
-            al.u = *reinterpret_cast<const uint2*>(am + sq + (int64_t)i * dp + j);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                float w = fmaf(p.c * p.in_scale, v[e], p.b * ((float)ah.h[e] + (float)al.h[e]));
-                if (i == j + e && i < r.d) w += p.a;
-                split16(w * p.out_exp, h.h[e], l.h[e]);
+            for (int e = 0; e < 4; ++e) o[e] = fmaf(-lr * m.out_scale, v[e], o[e] - lr * p.wd * o[e]);
+            *reinterpret_cast<f32x4_t*>(w) = o;
+            if (m.p16) {
+                const uint2 hi = make_uint2(pack_bf2(o[0], o[1]), pack_bf2(o[2], o[3]));
+                *reinterpret_cast<uint2*>(m.p16 + at) = hi;
+                if (m.p16lo)
+                    *reinterpret_cast<uint2*>(m.p16lo + at) =
+                        make_uint2(pack_bf2(o[0] - __uint_as_float(hi.x << 16), o[1] - __uint_as_float(hi.x & 0xffff0000u)),
+                                   pack_bf2(o[2] - __uint_as_float(hi.y << 16), o[3] - __uint_as_float(hi.y & 0xffff0000u)));
             }
-        } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) split16(v[e] * (p.in_scale * p.out_exp), h.h[e], l.h[e]);
-        }
-        _Float16* o = out + (int64_t)i * dp + j;
-        if (i >= j + 3) {
-            *reinterpret_cast<uint2*>(o) = h.u;
-            *reinterpret_cast<uint2*>(o + sq) = l.u;
-        } else
-#pragma unroll
-            for (int e = 0; e < 3; ++e)
-                if (i >= j + e) o[e] = h.h[e], o[sq + e] = l.h[e];
-    }
-    // the mirror image: row j of the result, columns i .. i + 3
-#pragma unroll
-    for (int it = 0; it < Sub<T>::S * LPR / 64; ++it) {
-        const int lj = it * (64 / LPR) + lane / LPR, li = (lane % LPR) * 4, i = i0 + ws + li, j = j0 + wf + lj;
-        if (i + 3 <= j) continue;
-        const f32x4_t v = Sub<T>::col(sub, li, lj);
-        H4 h, l, ah, al;
-        if constexpr (Q) {                                                    // (A is symmetric to the bit)
-            ah.u = *reinterpret_cast<const uint2*>(am + (int64_t)j * dp + i);
-            al.u = *reinterpret_cast<const uint2*>(am + sq + (int64_t)j * dp + i);
+            return;
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            if constexpr (Q) split16(fmaf(p.c * p.in_scale, v[e], p.b * ((float)ah.h[e] + (float)al.h[e])) * p.out_exp, h.h[e], l.h[e]);
-            else split16(v[e] * (p.in_scale * p.out_exp), h.h[e], l.h[e]);
+            if (col + e >= m.cols) break;
+            const float nw = fmaf(-lr * m.out_scale, v[e], w[e] - lr * p.wd * w[e]);
+            w[e] = nw;
+            if (m.p16) {
+                const bf16_t hi = f2bf(nw);
+                m.p16[at + e] = hi;
+                if (m.p16lo) m.p16lo[at + e] = f2bf(nw - bf2f(hi));
+            }
         }
-        _Float16* o = out + (int64_t)j * dp + i;
-        if (i > j) {
-            *reinterpret_cast<uint2*>(o) = h.u;
-            *reinterpret_cast<uint2*>(o + sq) = l.u;
-        } else
+    } else if (m.ovec && p.o_dtype == POET_F32) *reinterpret_cast<f32x4_t*>((float*)m.o + at) = v;
+    else if (m.ovec) {
+        const float o[4] = {v[0], v[1], v[2], v[3]};
+        if (p.o_dtype == POET_BF16) vec<bf16_t, 4>::st((bf16_t*)m.o + at, o);
+        else vec<f16_t, 4>::st((f16_t*)m.o + at, o);
+    } else {
 #pragma unroll
-            for (int e = 1; e < 4; ++e)
-                if (i + e > j) o[e] = h.h[e], o[sq + e] = l.h[e];
+        for (int e = 0; e < 4; ++e)
+            if (col + e < m.cols) st_any(m.o, at + e, v[e], p.o_dtype);
     }
 }
 
+// A tile of A or of q (from A's pieces ah, al), written twice: as it is, and its mirror image
+template <int T, int Q> __device__ __forceinline__ void leave_sym(const StageP& p, const Shape& r, int i0, int j0, float* part, f32x4_t (&v)[Meet<T>::U],
+                                                                  const uint2 (&ah)[Meet<T>::U], const uint2 (&al)[Meet<T>::U]) {
+    typedef Meet<T> M;
+    const int dp = r.dp;
+    const int64_t sq = (int64_t)dp * dp;
+    const float cs = (Q ? p.c : 1.f) * p.in_scale * p.out_exp, bs = p.b * p.out_exp, as = p.a * p.out_exp;
+    const bool diagonal = i0 == j0;
+    _Float16* out = p.planes + (Q ? r.bm : r.am) + (int64_t)i0 * dp + j0;
+#pragma unroll
+    for (int u = 0; u < M::U; ++u) {
+        v[u] *= cs;
+        if constexpr (Q) {
+            const float aa[4] = {h_lo(ah[u].x) + h_lo(al[u].x), h_hi(ah[u].x) + h_hi(al[u].x), h_lo(ah[u].y) + h_lo(al[u].y), h_hi(ah[u].y) + h_hi(al[u].y)};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[u][e] = fmaf(bs, aa[e], v[u][e]);
+            if (diagonal) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (M::row(u) == M::col() + e && i0 + M::row(u) < r.d) v[u][e] += as;
+            }
+        }
+        uint2 lo;
+        const uint2 hi = pack4(v[u], lo);
+        _Float16* o = out + (M::row(u) * dp + M::col());
+        if (!diagonal) {
+            *reinterpret_cast<uint2*>(o) = hi;
+            *reinterpret_cast<uint2*>(o + sq) = lo;
+        } else store_some(o, o + sq, hi, lo, 0, M::row(u) - M::col());
+    }
+    M::turn(part, v);
+    out = p.planes + (Q ? r.bm : r.am) + (int64_t)j0 * dp + i0;
+#pragma unroll
+    for (int u = 0; u < M::U; ++u) {
+        uint2 lo;
+        const uint2 hi = pack4(v[u], lo);
+        _Float16* o = out + (M::row(u) * dp + M::col());
+        if (!diagonal) {
+            *reinterpret_cast<uint2*>(o) = hi;
+            *reinterpret_cast<uint2*>(o + sq) = lo;
+        } else store_some(o, o + sq, hi, lo, M::row(u) - M::col() + 1, 3);
+    }
+}
+template <int T> __device__ __forceinline__ void a_pieces(const StageP& p, const Shape& r, int i0, int j0, uint2 (&ah)[Meet<T>::U], uint2 (&al)[Meet<T>::U]) {
+    const _Float16* a = p.planes + r.am + (int64_t)i0 * r.dp + j0;
+    const int64_t sq = (int64_t)r.dp * r.dp;
+#pragma unroll
+    for (int u = 0; u < Meet<T>::U; ++u) {
+        const _Float16* at = a + (Meet<T>::row(u) * r.dp + Meet<T>::col());
+        ah[u] = *reinterpret_cast<const uint2*>(at);
+        al[u] = *reinterpret_cast<const uint2*>(at + sq);
+    }
+}
+// A tile of X' into its planes, or of the result (LAST)
+template <int T, bool LAST> __device__ __forceinline__ void leave_update(const StageP& p, const Shape& r, int b, int i0, int j0, float* part, f32x4_t (&v)[Meet<T>::U]) {
+    typedef Meet<T> M;
+    if constexpr (!LAST) {
+        const int np = r.np;
+        const int64_t plane = (int64_t)r.dp * np;
+        _Float16* out = p.planes + (p.flip ? r.x0 : r.x1) + (int64_t)i0 * np + j0;
+#pragma unroll
+        for (int u = 0; u < M::U; ++u) {
+            uint2 lo;
+            const uint2 hi = pack4(v[u] * (p.in_scale * p.out_exp), lo);
+            _Float16* o = out + (M::row(u) * np + M::col());
+            *reinterpret_cast<uint2*>(o) = hi;
+            *reinterpret_cast<uint2*>(o + plane) = lo;
+        }
+    } else {
+        const Rec m = find(p.table, p.firsts + UPD * p.count, p.count, b);
+        const float lr = p.lr * (m.lr_scale ? fabsf(*m.lr_scale) : 1.f);
+        if (m.turned) M::turn(part, v);                                       // output rows are X's columns
+#pragma unroll
+        for (int u = 0; u < M::U; ++u) write4(m, p, lr, (m.turned ? j0 : i0) + M::row(u), (m.turned ? i0 : j0) + M::col(), v[u] * p.in_scale);
+    }
+}
+__device__ __forceinline__ void triangle(int t, int& bi, int& bj) {           // tile t < 2^29 of the lower triangle
+    int i = (int)((__builtin_amdgcn_sqrtf(8.f * (float)t + 1.f) - 1.f) * 0.5f);
+    while ((i + 1) * (i + 2) / 2 <= t) ++i;
+    while (i * (i + 1) / 2 > t) --i;
+    bi = __builtin_amdgcn_readfirstlane(i);
+    bj = __builtin_amdgcn_readfirstlane(t - i * (i + 1) / 2);
+}
+__device__ __forceinline__ void rectangle(int t, int tn, int& bi, int& bj) {  // tile t of rows of tn tiles
+    int j;
+    bi = __builtin_amdgcn_readfirstlane(divide(t, tn, j));
+    bj = __builtin_amdgcn_readfirstlane(j);
+}
+template <int SETS, int F> __device__ __forceinline__ void zero(f32x4_t (&acc)[SETS][F][F]) {
+#pragma unroll
+    for (int q = 0; q < SETS * F * F; ++q) acc[q / (F * F)][q / F % F][q % F] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+}
+template <int SETS, int F> __device__ __forceinline__ void fold_sets(f32x4_t (&acc)[SETS][F][F]) {
+    if constexpr (SETS == 4) {
+#pragma unroll
+        for (int q = 0; q < F * F; ++q) acc[0][q / F][q % F] = (acc[0][q / F][q % F] + acc[1][q / F][q % F]) + (acc[2][q / F][q % F] + acc[3][q / F][q % F]);
+    }
+}
+
+// A = X X^T (Q = 0), or q = a I + b A + c A A (Q = 1): tiles on and below the diagonal
+template <int T, int BK, int SETS, int Q> __global__ __launch_bounds__(NT, 2) void muon_sym_kernel(const StageP p) {
+    typedef Core<T, BK, false, SETS> C;
+    typedef Meet<T> M;
+    static_assert(2 * C::STAGE >= T * T * 4, "the tile fits the stages' LDS");
+    __shared__ __attribute__((aligned(16))) char smem[2 * C::STAGE];
+    int t, bi, bj;
+    const Shape r = locate<SYM>(p, xcd_order(blockIdx.x, p.total), t);
+    triangle(t, bi, bj);
+    const int i0 = bi * T, j0 = bj * T, dp = r.dp;
+    const int64_t ld = Q ? dp : r.np, plane = (int64_t)dp * ld;
+    const _Float16* in = p.planes + (Q ? r.am : p.flip ? r.x1 : r.x0);
+    const int K = Q ? (r.d + BK - 1) / BK * BK : (r.n + BK - 1) / BK * BK;
+    f32x4_t acc[SETS][C::F][C::F];
+    zero(acc);
+    uint2 ah[M::U], al[M::U];
+    if constexpr (Q && T == 64) a_pieces<T>(p, r, i0, j0, ah, al);            // (ahead of the product: 16 registers)
+    C::run(in + j0 * ld, in + plane + j0 * ld, ld, in + i0 * ld, in + plane + i0 * ld, ld, K, smem, acc);
+    if constexpr (Q && T != 64) a_pieces<T>(p, r, i0, j0, ah, al);
+    fold_sets(acc);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    f32x4_t v[M::U];
+    M::share(reinterpret_cast<float*>(smem), acc[0], (wave >> 1) * (T / 2), (wave & 1) * (T / 2), lane & 15, lane >> 4, v);
+    leave_sym<T, Q>(p, r, i0, j0, reinterpret_cast<float*>(smem), v, ah, al);
+}
+
 // X' = q X; the last step leaves the planes: the output matrix, or the weight update
-template <int T, int BK, bool LAST> __global__ __launch_bounds__(NT, 2) void muon_update_kernel(const StageP p) {
-    __shared__ __attribute__((aligned(16))) char smem[2 * Core<T, BK, true>::STAGE];
-    constexpr int F = T / 32;
+template <int T, int BK, int SETS, bool LAST> __global__ __launch_bounds__(NT, 2) void muon_update_kernel(const StageP p) {
+    typedef Core<T, BK, true, SETS> C;
+    typedef Meet<T> M;
+    __shared__ __attribute__((aligned(16))) char smem[2 * C::STAGE];
+    int t;
     const int b = xcd_order(blockIdx.x, p.total);
-    const Rec r = find(p.table, p.firsts + UPD * p.count, p.count, b);
-    const int t = b - r.first[UPD], tn = r.np / T, i0 = (t / tn) * T, j0 = (t % tn) * T, dp = r.dp;
+    const Shape r = locate<UPD>(p, b, t);
+    int bi, bj;
+    rectangle(t, r.np / T, bi, bj);
+    const int i0 = bi * T, j0 = bj * T, dp = r.dp;
     const int64_t np = r.np, plane = (int64_t)dp * np, sq = (int64_t)dp * dp;
     const _Float16* x = p.planes + (p.flip ? r.x1 : r.x0);
     const _Float16* qm = p.planes + r.bm;
-    f32x4_t acc[F][F];
-#pragma unroll
-    for (int f = 0; f < F; ++f)
-#pragma unroll
-        for (int s = 0; s < F; ++s) acc[f][s] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    Core<T, BK, true>::run(x + j0, x + plane + j0, np, qm + (int64_t)i0 * dp, qm + sq + (int64_t)i0 * dp, dp, (r.d + BK - 1) / BK * BK, smem, acc);
+    f32x4_t acc[SETS][C::F][C::F];
+    zero(acc);
+    C::run(x + j0, x + plane + j0, np, qm + (int64_t)i0 * dp, qm + sq + (int64_t)i0 * dp, dp, (r.d + BK - 1) / BK * BK, smem, acc);
+    fold_sets(acc);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    f32x4_t v[M::U];
+    M::share(reinterpret_cast<float*>(smem), acc[0], (wave >> 1) * (T / 2), (wave & 1) * (T / 2), lane & 15, lane >> 4, v);
+    leave_update<T, LAST>(p, r, b, i0, j0, reinterpret_cast<float*>(smem), v);
+}
 
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wf = (wave >> 1) * (T / 2), ws = (wave & 1) * (T / 2);
-    float* sub = Sub<T>::put(smem, acc, wave, lane);
-    constexpr int LPR = Sub<T>::S / 4;
-    const float lr = p.lr * (r.lr_scale ? fabsf(*r.lr_scale) : 1.f);
+// ---- 3b: the same products for short lists of matrices with d <= 256: 32 x 32 tiles, K split over the waves -------------------------
+// With K = d <= 256 a launch is a few microseconds of latency: of the 64 x 64 tiles above, staged through LDS, a K = 256 product is
+// store - barrier - read - multiply in turn with one wave per SIMD, and 128 KB of operands pass one CU's port.  Here the tile is a quarter, so that
+// four times as many CUs pull operands, and every wave multiplies the whole tile over its own steps of 32 k, its fragments loaded straight
+// into registers (a lane's 16 bytes of a row are the fragment), all in flight at once, no barrier; the partial tiles meet once in LDS.  Four
+// 256 x 256 matrices: 116 -> 89 us.  Half as much reuse of every operand byte, and 64-byte pieces of rows instead of 128: ten 1024 x 256
+// take 231 us this way against 189 with the staged tiles (and as much with 64 x 64 tiles that load like these).
+template <int F> struct Frags { f16x8_t h[F], l[F]; };
+template <int F> __device__ __forceinline__ void mfma_tile(f32x4_t (&acc)[F][F], const Frags<F>& f, const Frags<F>& s) {
 #pragma unroll
-    for (int it = 0; it < Sub<T>::S * LPR / 64; ++it) {
-        const int la = it * (64 / LPR) + lane / LPR, lb = (lane % LPR) * 4;
-        if constexpr (!LAST) {
-            const f32x4_t v = Sub<T>::row(sub, la, lb);
-            _Float16* out = p.planes + (p.flip ? r.x0 : r.x1) + (int64_t)(i0 + ws + la) * np + j0 + wf + lb;
-            H4 h, l;
+    for (int q = 0; q < F * F; ++q) acc[q / F][q % F] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.l[q / F], s.h[q % F], acc[q / F][q % F], 0, 0, 0);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) split16(v[e] * (p.in_scale * p.out_exp), h.h[e], l.h[e]);
-            *reinterpret_cast<uint2*>(out) = h.u;
-            *reinterpret_cast<uint2*>(out + plane) = l.u;
-        } else {
-            // output rows: X's rows, or X's columns when turned
-            f32x4_t v = r.turned ? Sub<T>::col(sub, lb, la) : Sub<T>::row(sub, la, lb);
-            const int row = r.turned ? j0 + wf + la : i0 + ws + la, col = r.turned ? i0 + ws + lb : j0 + wf + lb;
-            if (row >= r.rows || col >= r.cols) continue;
-            const int64_t at = row * r.ldo + col;
-            v *= p.in_scale;
-            if (p.muon) {
-                float* w = (float*)r.o + at;
-                if (r.ovec) {                                                 // (cols % 4 == 0)
-                    f32x4_t o = *reinterpret_cast<f32x4_t*>(w);
+    for (int q = 0; q < F * F; ++q) acc[q / F][q % F] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.h[q / F], s.l[q % F], acc[q / F][q % F], 0, 0, 0);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) o[e] = fmaf(-lr * r.out_scale, v[e], o[e] - lr * p.wd * o[e]);
-                    *reinterpret_cast<f32x4_t*>(w) = o;
-                    if (r.p16) {
-                        const uint2 hi = make_uint2(pack_bf2(o[0], o[1]), pack_bf2(o[2], o[3]));
-                        *reinterpret_cast<uint2*>(r.p16 + at) = hi;
-                        if (r.p16lo)
-                            *reinterpret_cast<uint2*>(r.p16lo + at) =
-                                make_uint2(pack_bf2(o[0] - __uint_as_float(hi.x << 16), o[1] - __uint_as_float(hi.x & 0xffff0000u)),
-                                           pack_bf2(o[2] - __uint_as_float(hi.y << 16), o[3] - __uint_as_float(hi.y & 0xffff0000u)));
-                    }
-                    continue;
-                }
+    for (int q = 0; q < F * F; ++q) acc[q / F][q % F] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.h[q / F], s.h[q % F], acc[q / F][q % F], 0, 0, 0);
+}
+// 16 F rows of a plane pair, k .. k + 31 (base: this lane's row and 16-byte piece)
+template <int F> __device__ __forceinline__ void rows_of(Frags<F>& f, const _Float16* base, int ld16, int64_t plane, int k) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    if (col + e >= r.cols) break;
-                    const float nw = fmaf(-lr * r.out_scale, v[e], w[e] - lr * p.wd * w[e]);
-                    w[e] = nw;
-                    if (r.p16) {
-                        const bf16_t hi = f2bf(nw);
-                        r.p16[at + e] = hi;
-                        if (r.p16lo) r.p16lo[at + e] = f2bf(nw - bf2f(hi));
-                    }
-                }
-            } else if (r.ovec && p.o_dtype == POET_F32) *reinterpret_cast<f32x4_t*>((float*)r.o + at) = v;
-            else if (r.ovec) {
-                float o[4] = {v[0], v[1], v[2], v[3]};
-                if (p.o_dtype == POET_BF16) vec<bf16_t, 4>::st((bf16_t*)r.o + at, o);
-                else vec<f16_t, 4>::st((f16_t*)r.o + at, o);
-            } else {
+    for (int q = 0; q < F; ++q) {
+        f.h[q] = *reinterpret_cast<const f16x8_t*>(base + (q * ld16 + k));
+        f.l[q] = *reinterpret_cast<const f16x8_t*>(base + plane + (q * ld16 + k));
+    }
+}
+// wave w's steps of 32 k: 2 w, 2 w + 1, 2 w + 8, ... (pairs share the 128-byte lines of a row)
+__device__ __forceinline__ int step_k(int wave, int u) { return ((u >> 1) * 8 + wave * 2 + (u & 1)) * 32; }
+
+template <int Q> __global__ __launch_bounds__(NT, 2) void muon_sym_split_kernel(const StageP p) {
+    constexpr int T = 32;
+    typedef Meet<T> M;
+    __shared__ __attribute__((aligned(16))) float part[NT / 64 * T * T];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), m16 = lane & 15, kc = lane >> 4;
+    int t, bi, bj;
+    const Shape r = locate<SYM>(p, xcd_order(blockIdx.x, p.total), t);
+    triangle(t, bi, bj);
+    const int i0 = bi * T, j0 = bj * T, dp = r.dp;
+    const int64_t ld = Q ? dp : r.np, plane = (int64_t)dp * ld;
+    const _Float16* in = p.planes + (Q ? r.am : p.flip ? r.x1 : r.x0);
+    const int K = ((Q ? r.d : r.n) + 31) / 32 * 32, ld16 = (int)ld * 16;
+    const _Float16* fb = in + (j0 + m16) * ld + kc * 8;
+    const _Float16* sb = in + (i0 + m16) * ld + kc * 8;
+    constexpr int AHEAD = Q ? 2 : 4;                                          // (K <= 256: two steps a wave)
+    Frags<2> f[AHEAD], s[AHEAD];
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (col + e < r.cols) st_any(r.o, at + e, v[e], p.o_dtype);
-            }
+    for (int u = 0; u < AHEAD; ++u)
+        if (const int k = step_k(wave, u); k < K) rows_of(f[u], fb, ld16, plane, k), rows_of(s[u], sb, ld16, plane, k);
+    uint2 ah[M::U], al[M::U];
+    if constexpr (Q) a_pieces<T>(p, r, i0, j0, ah, al);
+    f32x4_t acc[1][2][2];
+    zero(acc);
+    for (int u0 = 0; step_k(wave, u0) < K; u0 += AHEAD) {
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            if (step_k(wave, u0 + u) >= K) break;
+            mfma_tile<2>(acc[0], f[u], s[u]);
+            if (const int k = step_k(wave, u0 + u + AHEAD); k < K) rows_of(f[u], fb, ld16, plane, k), rows_of(s[u], sb, ld16, plane, k);
         }
     }
+    f32x4_t v[M::U];
+    M::sum(part, acc[0], wave, m16, kc, v);
+    leave_sym<T, Q>(p, r, i0, j0, part, v, ah, al);
+}
+
+// between a wave's LDS stores and its loads of what other lanes stored: these complete in order, so only the compiler has to keep it
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+// X' = q X.  X is stored [k][column]: a wave's steps of 32 rows x 32 columns pass through its quarter of the LDS for the transposing read
+// (32-byte pieces of the 64-byte rows XORed with bit 3 of the row: the 8 rows of a read meet all banks once)
+template <bool LAST> __global__ __launch_bounds__(NT, 2) void muon_update_split_kernel(const StageP p) {
+    constexpr int T = 32, ROWB = T * 2;
+    typedef Meet<T> M;
+    __shared__ __attribute__((aligned(16))) float part[NT / 64 * T * T];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), m16 = lane & 15, kc = lane >> 4;
+    const int b = xcd_order(blockIdx.x, p.total);
+    int t;
+    const Shape r = locate<UPD>(p, b, t);
+    int bi, bj;
+    rectangle(t, r.np / T, bi, bj);
+    const int i0 = bi * T, j0 = bj * T, dp = r.dp, K = (r.d + 31) / 32 * 32;
+    const int64_t np = r.np, plane = (int64_t)dp * np;
+    const int xrow = lane >> 2, xc = lane & 3;
+    const _Float16* x = p.planes + (p.flip ? r.x1 : r.x0) + xrow * np + j0 + xc * 8;
+    const _Float16* sb = p.planes + r.bm + (i0 + m16) * dp + kc * 8;
+    Frags<2> s[2];
+    u32x4_t xr[2][2][2];                                                      // step, plane, rows k + 16 h + lane / 4
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+        if (const int k = step_k(wave, u); k < K) {                           // (K <= 256: two steps a wave)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                xr[u][0][h] = *reinterpret_cast<const u32x4_t*>(x + (k + h * 16) * np);
+                xr[u][1][h] = *reinterpret_cast<const u32x4_t*>(x + plane + (k + h * 16) * np);
+            }
+            rows_of(s[u], sb, dp * 16, dp * dp, k);
+        }
+    f32x4_t acc[1][2][2];
+    zero(acc);
+    static_assert(2 * 32 * ROWB <= T * T * 4, "a step's two planes fit the wave's partial tile");
+    char* mine = reinterpret_cast<char*>(part + wave * T * T);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        if (step_k(wave, u) >= K) break;
+        wave_sync();
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int row = h * 16 + xrow, at = row * ROWB + ((xc >> 1) ^ ((row >> 3) & 1)) * 32 + (xc & 1) * 16;
+            *reinterpret_cast<u32x4_t*>(mine + at) = xr[u][0][h];
+            *reinterpret_cast<u32x4_t*>(mine + 32 * ROWB + at) = xr[u][1][h];
+        }
+        wave_sync();
+        Frags<2> f;
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {                                         // (bit 3 of rows 8 kc .. 8 kc + 7: kc & 1)
+            const char* a = mine + (8 * kc + (m16 >> 2)) * ROWB + ((q ^ (kc & 1)) * 32) + (m16 & 3) * 8;
+            struct { v4s_t lo, hi; } w;
+            w.lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s_t*)(a));
+            w.hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s_t*)(a + 4 * ROWB));
+            f.h[q] = __builtin_bit_cast(f16x8_t, w);
+            w.lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s_t*)(a + 32 * ROWB));
+            w.hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s_t*)(a + 36 * ROWB));
+            f.l[q] = __builtin_bit_cast(f16x8_t, w);
+        }
+        mfma_tile<2>(acc[0], f, s[u]);
+    }
+    wave_sync();
+    f32x4_t v[M::U];
+    M::sum(part, acc[0], wave, m16, kc, v);
+    leave_update<T, LAST>(p, r, b, i0, j0, part, v);
 }
 
 // ---- narrow matrices: d <= 160 ------------------------------------------------------------------------------------------------
@@ -547,7 +773,7 @@ template <int T, int BK, bool LAST> __global__ __launch_bounds__(NT, 2) void muo
 // diagonal (each fragment read serves two tiles; a diagonal one reads its fragments once), the update in PAIRS of 16-column strips (each
 // fragment of q serves both), rewritten in place by the wave that owns them.  Rows of the LDS images are padded by 16 bytes: an odd number
 // of 16-byte pieces, so that the 16 rows of a fragment read start in different banks.
-constexpr int NW_T = 512, NWAVES = NW_T / 64, MAX_SLABS = 8, MAX_D = 5;
+constexpr int NW_T = 512, NWAVES = NW_T / 64, MAX_SLABS = 8, MAX_D = 5, MAX_SLAB_D = 2;
 template <int D> struct Narrow {
     static constexpr int DP = 32 * D, NM = D * (D + 1) / 2;
     static constexpr int PARTS = D == 1 ? 8 : D == 2 ? 2 : 1;             // few macro tiles: the columns in PARTS ranges, so that all waves have some
@@ -990,6 +1216,7 @@ template <int D> __global__ __launch_bounds__(NW_T, 2) void muon_slab_kernel(con
 
 // ---- host -----------------------------------------------------------------------------------------------------------------
 struct Tiles { int sym, upd; };                // tile edges of the symmetric and the update products
+struct Choice { Tiles large, small; };         // ... of the matrices with d > 256, and of the others
 struct Layout {
     int64_t table, firsts, part, planes, total;      // byte offsets
     int64_t plane_elems;
@@ -999,37 +1226,51 @@ int esize(int dt) { return dt == POET_F32 ? 4 : 2; }
 int up(int v, int m) { return (v + m - 1) / m * m; }
 
 // How a matrix is worked on, from its own shape alone (so that its result does not depend on what else is in the list):
-// 0 = the chain, D = one workgroup (d <= 32 D), MAX_D + D = slabs
-constexpr int GROUPS = 2 * MAX_D + 1;
+// 0 = the chain, SMALL = the chain of small tiles (d <= 256), D = one workgroup (d <= 32 D), MAX_D + D = slabs
+constexpr int SMALL = MAX_D + MAX_SLAB_D + 1, GROUPS = SMALL + 1;
 int group_of(int rows, int cols, int& W) {
     const int d = rows < cols ? rows : cols, n = rows < cols ? cols : rows, D = cdiv(d, 32);
     W = 0;
-    if (D > MAX_D) return 0;
-    const int slabs = cdiv(n, W_MAX[D]);
-    if (slabs > MAX_SLABS) return 0;
+    if (d > 256) return 0;
+    if (D <= MAX_D && n <= W_MAX[D]) {                       // (66 x 256: 61 us against 85 with the chain; 60 x 300: 50 against 89)
+        W = up(n, 32);
+        return D;
+    }
+    // slabs of 256 columns (at most 8, wider then): 20 x 2000: 73 us against 143 with the chain, 60 x 1500: 106 against 120; with three tiles of
+    // rows and more the chain wins (90 x 400: 96 against 81, 131 x 257: 115 against 81)
+    if (D > MAX_SLAB_D || n > MAX_SLABS * W_MAX[D]) return SMALL;
+    const int slabs = cdiv(n, 256) < MAX_SLABS ? cdiv(n, 256) : MAX_SLABS;
     W = up(cdiv(n, slabs), 32);
-    return slabs == 1 ? D : MAX_D + D;
+    return MAX_D + D;
 }
 
-Tiles tiles_of(const int* rows, const int* cols, int n) {
-    // 128 x 128 tiles halve the operand traffic per product, 64 x 64 tiles make (up to) four times as many workgroups: the large ones once
-    // they fill the chip: 2048 x 2048, 256 update tiles: 930 us against 1011; 180 tiles (an encoder's 30 matrices): 296 against 289; symmetric
-    // products twice (two workgroups a CU): 4 x 4096 x 1024, 144 tiles: 1509 against 1374
-    int64_t sym = 0, upd = 0;
+Choice tiles_of(const int* rows, const int* cols, int n) {
+    // d > 256: 128 x 128 tiles halve the operand traffic per product, 64 x 64 tiles make (up to) four times as many workgroups: the large
+    // ones once they fill the chip (2048 x 2048, 256 update tiles: 930 us against 1011), in the symmetric products twice, two workgroups
+    // a CU (4 x 4096 x 1024, 144 tiles: 1509 us against 1374 with the small ones).  d <= 256: 32 x 32 tiles while they fit the chip once (twice
+    // in the update): four 256 x 256 87 us against 116; sixteen 144 against 120, ten 1024 x 256 231 against 189.
+    int64_t sym = 0, upd = 0, ssym = 0, supd = 0;
     for (int i = 0; i < n; ++i) {
         int W;
-        if (group_of(rows[i], cols[i], W)) continue;
-        const int64_t td = cdiv(rows[i] < cols[i] ? rows[i] : cols[i], 128);
-        sym += td * (td + 1) / 2;
-        upd += (int64_t)cdiv(rows[i], 128) * cdiv(cols[i], 128);
+        const int group = group_of(rows[i], cols[i], W), d = rows[i] < cols[i] ? rows[i] : cols[i];
+        if (group == 0) {
+            const int64_t td = cdiv(d, 128);
+            sym += td * (td + 1) / 2;
+            upd += (int64_t)cdiv(rows[i], 128) * cdiv(cols[i], 128);
+        } else if (group == SMALL) {
+            const int64_t td = cdiv(d, 32);
+            ssym += td * (td + 1) / 2;
+            supd += (int64_t)cdiv(rows[i], 32) * cdiv(cols[i], 32);
+        }
     }
-    return {sym >= 512 ? 128 : 64, upd >= 256 ? 128 : 64};
+    return {{sym >= 512 ? 128 : 64, upd >= 256 ? 128 : 64}, {ssym > 256 ? 64 : 32, supd > 512 ? 64 : 32}};
 }
 
 // the records of one group among matrices [first, n) (at most `most` of them): shape-dependent members into rec (when given), sizes into L;
 // returns the index behind the last one taken, or -1: too large
-int layout(const int* rows, const int* cols, int first, int n, int group, Tiles T, int most, Layout& L, Rec* rec) {
-    const int P = T.sym > T.upd ? T.sym : T.upd;             // planes hold whole tiles of either kind
+int layout(const int* rows, const int* cols, int first, int n, int group, const Choice& choice, int most, Layout& L, Rec* rec) {
+    const Tiles T = group == SMALL ? choice.small : choice.large;
+    const int P = T.sym == 128 || T.upd == 128 ? 128 : 64;   // planes hold whole tiles of every kind
     int64_t planes = 0, parts = 0, tiles[GRIDS] = {0, 0, 0};
     int i = first, count = 0;
     L.maxW = 0;
@@ -1045,18 +1286,21 @@ int layout(const int* rows, const int* cols, int first, int n, int group, Tiles 
         r.nb = (int)(e > 256ll * NORM_ELEMS ? 256 : cdiv(e, NORM_ELEMS));
         int64_t mine[GRIDS] = {0, 0, 0};
         r.x0 = planes;
-        if (group == 0) {
+        if (group == 0 || group == SMALL) {
             r.dp = up(r.d, P);
             r.np = up(r.n, P);
             r.x1 = r.x0 + 2 * (int64_t)r.dp * r.np;
             r.am = r.x1 + 2 * (int64_t)r.dp * r.np;
             r.bm = r.am + 2 * (int64_t)r.dp * r.dp;
             planes = r.bm + 2 * (int64_t)r.dp * r.dp;
-            const int64_t td = cdiv(r.d, T.sym);
+            // Staged 64 x 64 tiles run k in steps of 64, so that next to 32 x 32 ones the rows up to a multiple of 64 must be there (as zeros):
+            // one kind of product writes what the other reads
+            const int rows_of_tiles = group == SMALL && (T.sym == 64 || T.upd == 64) ? r.dp : r.d;
+            const int64_t td = cdiv(rows_of_tiles, T.sym);
             mine[SYM] = td * (td + 1) / 2;
-            mine[UPD] = (int64_t)cdiv(r.d, T.upd) * (r.np / T.upd);
+            mine[UPD] = (int64_t)cdiv(rows_of_tiles, T.upd) * (r.np / T.upd);
             mine[PACK] = (int64_t)(r.dp / 64) * (r.np / 64);
-        } else if (group > MAX_D) {
+        } else if (group > MAX_D) {           // slabs
             const int D = group - MAX_D, slabs = cdiv(r.n, r.W);
             const int64_t gram = (int64_t)slabs * D * (D + 1) / 2 * 2048;       // fp32 partial tiles, in 16-bit elements
             r.am = r.x0 + (int64_t)slabs * 2 * 32 * D * r.W;
@@ -1131,13 +1375,18 @@ struct Job {
     const float* sqnorm;
 };
 
-template <int Q> void sym_product(int T, const StageP& p, hipStream_t st) {
-    if (T == 128) hipLaunchKernelGGL((muon_sym_kernel<128, 32, Q>), dim3(p.total), dim3(NT), 0, st, p);
-    else hipLaunchKernelGGL((muon_sym_kernel<64, 64, Q>), dim3(p.total), dim3(NT), 0, st, p);
+// split: d <= 256, where sums have four parts whichever tile is taken
+template <int Q> void sym_product(int T, bool split, const StageP& p, hipStream_t st) {
+    if (T == 32) hipLaunchKernelGGL((muon_sym_split_kernel<Q>), dim3(p.total), dim3(NT), 0, st, p);
+    else if (split) hipLaunchKernelGGL((muon_sym_kernel<64, 64, 4, Q>), dim3(p.total), dim3(NT), 0, st, p);
+    else if (T == 128) hipLaunchKernelGGL((muon_sym_kernel<128, 32, 1, Q>), dim3(p.total), dim3(NT), 0, st, p);
+    else hipLaunchKernelGGL((muon_sym_kernel<64, 64, 1, Q>), dim3(p.total), dim3(NT), 0, st, p);
 }
-template <bool LAST> void update_product(int T, const StageP& p, hipStream_t st) {
-    if (T == 128) hipLaunchKernelGGL((muon_update_kernel<128, 32, LAST>), dim3(p.total), dim3(NT), 0, st, p);
-    else hipLaunchKernelGGL((muon_update_kernel<64, 64, LAST>), dim3(p.total), dim3(NT), 0, st, p);
+template <bool LAST> void update_product(int T, bool split, const StageP& p, hipStream_t st) {
+    if (T == 32) hipLaunchKernelGGL((muon_update_split_kernel<LAST>), dim3(p.total), dim3(NT), 0, st, p);
+    else if (split) hipLaunchKernelGGL((muon_update_kernel<64, 64, 4, LAST>), dim3(p.total), dim3(NT), 0, st, p);
+    else if (T == 128) hipLaunchKernelGGL((muon_update_kernel<128, 32, 1, LAST>), dim3(p.total), dim3(NT), 0, st, p);
+    else hipLaunchKernelGGL((muon_update_kernel<64, 64, 1, LAST>), dim3(p.total), dim3(NT), 0, st, p);
 }
 StageP stage_params(const Layout& L, const Job& j, const Steps& S, char* ws) {
     StageP p = {};
@@ -1152,26 +1401,32 @@ StageP stage_params(const Layout& L, const Job& j, const Steps& S, char* ws) {
     p.out_exp = pow2(S.ex[0]);
     return p;
 }
-void chain(Tiles T, const Layout& L, const Job& j, const Steps& S, char* ws, hipStream_t st) {
+void chain(Tiles T, bool split, const Rec& first, bool one_shape, const Layout& L, const Job& j, const Steps& S, char* ws, hipStream_t st) {
     StageP p = stage_params(L, j, S, ws);
+    if (one_shape) {
+        p.uniform = {first.x0, first.x1, first.am, first.bm, first.d, first.n, first.dp, first.np};
+        p.stride = L.plane_elems / L.count;
+        p.per[SYM] = L.tiles[SYM] / L.count;
+        p.per[UPD] = L.tiles[UPD] / L.count;
+    }
     hipLaunchKernelGGL(muon_pack_kernel, dim3(L.tiles[PACK]), dim3(NT), 0, st, p);
     for (int k = 0; k < j.steps; ++k) {
         p.flip = k & 1;
         p.total = L.tiles[SYM];
         p.in_scale = pow2(-2 * S.ex[k]);
         p.out_exp = pow2(S.ea[k]);
-        sym_product<0>(T.sym, p, st);
+        sym_product<0>(T.sym, split, p, st);
         p.a = (float)j.coeffs[3 * k];
         p.b = (float)(j.coeffs[3 * k + 1] * pow2(-S.ea[k]));
         p.c = (float)j.coeffs[3 * k + 2];
         p.in_scale = pow2(-2 * S.ea[k]);
         p.out_exp = pow2(S.eq[k]);
-        sym_product<1>(T.sym, p, st);
+        sym_product<1>(T.sym, split, p, st);
         p.total = L.tiles[UPD];
         p.in_scale = pow2(-S.eq[k] - S.ex[k]);
         p.out_exp = pow2(S.ex[k + 1]);
-        if (k + 1 < j.steps) update_product<false>(T.upd, p, st);
-        else update_product<true>(T.upd, p, st);
+        if (k + 1 < j.steps) update_product<false>(T.upd, split, p, st);
+        else update_product<true>(T.upd, split, p, st);
     }
 }
 NarrowP narrow_params(const Layout& L, const Job& j, const Steps& S, char* ws) {
@@ -1206,7 +1461,7 @@ template <int D> void narrow_slabs(NarrowP p, const Layout& L, hipStream_t st) {
 }
 
 // bytes of all groups (at least one aligned block), -1: too large
-int64_t workspace_of(const int* rows, const int* cols, int n, Tiles T) {
+int64_t workspace_of(const int* rows, const int* cols, int n, const Choice& T) {
     int64_t need = 0;
     for (int group = 0; group < GROUPS; ++group) {
         Layout L;
@@ -1227,7 +1482,7 @@ int run_job(const char* what, const Job& j, void* ws, int64_t ws_bytes, void* st
     }
     Steps S;
     POET_CHECK(ranges(j.coeffs, j.steps, S), POET_ERR_ARG, "%s: these coefficients leave the range the iteration can hold", what);
-    const Tiles T = tiles_of(j.rows, j.cols, j.n);
+    const Choice T = tiles_of(j.rows, j.cols, j.n);
     const int64_t need = workspace_of(j.rows, j.cols, j.n, T);
     POET_CHECK(need >= 0, POET_ERR_UNSUPPORTED, "%s: too many tiles", what);
     POET_CHECK(ws && ((uintptr_t)ws % 256) == 0 && ws_bytes >= need, POET_ERR_ARG, "%s: workspace of %lld bytes needed (256-byte aligned), %lld given", what,
@@ -1249,6 +1504,8 @@ int run_job(const char* what, const Job& j, void* ws, int64_t ws_bytes, void* st
         const NarrowP narrow = narrow_params(L, j, S, base);
         int64_t planes = 0;                                   // of the chunks before this one
         int parts = 0, tiles[GRIDS] = {0, 0, 0};
+        Rec shape = {};
+        bool one_shape = true;
         for (int at = 0; np.first < L.count;) {
             Recs recs = {};
             Layout C;
@@ -1259,6 +1516,8 @@ int run_job(const char* what, const Job& j, void* ws, int64_t ws_bytes, void* st
                 int W;
                 if (group_of(j.rows[i], j.cols[i], W) != group) continue;
                 Rec& r = recs.r[c++];
+                if (np.first + c == 1) shape = r;
+                one_shape = one_shape && r.d == shape.d && r.n == shape.n;
                 r.x0 += planes; r.x1 += planes; r.am += planes; r.bm += planes;
                 r.part0 += parts;
                 for (int k = 0; k < GRIDS; ++k) r.first[k] += tiles[k];
@@ -1288,12 +1547,10 @@ int run_job(const char* what, const Job& j, void* ws, int64_t ws_bytes, void* st
             for (int k = 0; k < GRIDS; ++k) tiles[k] += C.tiles[k];
             np.first += C.count;
         }
-        if (group == 0) chain(T, L, j, S, base, st);
+        if (group == 0) chain(T.large, false, shape, one_shape, L, j, S, base, st);
+        else if (group == SMALL) chain(T.small, true, shape, one_shape, L, j, S, base, st);
         else if (group == MAX_D + 1) narrow_slabs<1>(narrow, L, st);
         else if (group == MAX_D + 2) narrow_slabs<2>(narrow, L, st);
-        else if (group == MAX_D + 3) narrow_slabs<3>(narrow, L, st);
-        else if (group == MAX_D + 4) narrow_slabs<4>(narrow, L, st);
-        else if (group == MAX_D + 5) narrow_slabs<5>(narrow, L, st);
         base += L.total;
     }
     POET_LAUNCH_CHECK();

@@ -118,6 +118,20 @@ def test_list_equals_single_calls(ops):
     assert all(torch.equal(p, q) for p, q in zip(outs, ops.orthogonalize(gs)))
 
 
+@pytest.mark.parametrize("shape,count", [((200, 200), 3), ((200, 200), 10), ((200, 200), 14), ((200, 400), 8), ((70, 300), 60), ((300, 300), 4), ((1100, 1030), 2)])
+def test_every_tile_choice_on_a_dirty_workspace(ops, shape, count):
+    """Both kinds of product with either tile edge, at sizes that end inside a tile; what the padding of the planes held before the call
+    (here NaN) does not reach a result, and the result is that of a call of its own."""
+    gs = [matrix(*shape, seed=i).cuda() for i in range(count)]
+    torch.full((1 << 27,), float("nan"), device="cuda")                       # freed at once: the workspaces below come out of it
+    outs = ops.orthogonalize(gs)
+    for g, o in zip(gs, outs):
+        check(o, g, f"{shape} x {count}")
+    for i in (0, count - 1):
+        torch.full((1 << 27,), float("nan"), device="cuda")
+        assert torch.equal(outs[i], ops.orthogonalize(gs[i]))
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_batches_views_and_out(ops, dtype):
     dt = DT[dtype]
