@@ -454,7 +454,8 @@ int poet_adamw(float* p, const float* g, float* m, float* v, uint16_t* p_bf16, u
                const float* sqnorm, float max_norm, float grad_scale,
                const uint32_t* step_dev /* optional: the step count is read from this device word instead of `step` */,
                const float* lr_scale /* optional: lr multiplier per block of 64 elements, ceil(n/64) floats (the 0.1x group of
-                                        main.py:41,253-271 inside one contiguous range) */,
+                                        main.py:41,253-271 inside one contiguous range); where its sign bit is set (-0 too) the block
+                                        belongs to another optimiser (poet_muon_step) and is left alone: p, m, v, images */,
                void* stream);
 /* ------------------------------------------------------------------------------------------------
  * Orthogonalised updates of weight matrices (the Muon optimiser), a LIST of n matrices of any shapes in one chain of launches.

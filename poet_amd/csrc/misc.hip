@@ -625,7 +625,11 @@ __global__ __launch_bounds__(256) void adamw_kernel(float* __restrict__ p, const
                                                     const uint32_t* __restrict__ step_dev, const float* __restrict__ lr_scale, int vec4) {
     const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
     if (i >= n) return;
-    if (lr_scale) lr *= lr_scale[i >> 6];                    // per-64-element learning-rate multiplier (LR groups inside one range)
+    if (lr_scale) {                                          // per-64-element learning-rate multiplier (LR groups inside one range)
+        const float s = lr_scale[i >> 6];
+        if (__float_as_uint(s) >> 31) return;                // (the sign marks a block of another optimiser's, also at a rate of -0)
+        lr *= s;
+    }
     if (step_dev) {                                          // graph replay: bias corrections from the device-side step
         const float t = (float)(*step_dev);
         bc1 = 1.f - powf(b1, t);

@@ -54,10 +54,15 @@ class ParamArena:
     Parameters that never receive a gradient in this configuration (transformer.reference_points.*
     in bbox mode; the reason the reference needs find_unused_parameters=True) stay outside, exactly as
     torch.optim.AdamW skips parameters whose .grad is None.
+    muon: options of ops.MuonPlan.step / its `scale` (or True) -- the weight matrices (MUON_SKIP: not the embeddings and tables, not the
+    heads' output layers) step by orthogonalised updates instead of AdamW, their first Adam moment being the momentum; learning rate,
+    schedule, clip and weight decay are AdamW's (scale "rms" by default: steps of AdamW's size).  Self-attention's stacked in-projection
+    counts as three matrices.  lr_scale is negative over their blocks (poet_adamw leaves those alone).
     """
+    MUON_SKIP = re.compile(r"level_embed|query_embed|^backbone\.|_head\w*\.\d+\.layers\.2\.")
 
     def __init__(self, model: nn.Module, lr=2e-4, lr_proj_mult=0.1, proj_names=("reference_points", "sampling_offsets"),
-                 weight_decay=1e-4, betas=(0.9, 0.999), eps=1e-8, exclude=("transformer.reference_points",), lr_backbone_mult=0.1):
+                 weight_decay=1e-4, betas=(0.9, 0.999), eps=1e-8, exclude=("transformer.reference_points",), lr_backbone_mult=0.1, muon=None):
         named = [(n, p) for n, p in model.named_parameters() if p.requires_grad and not any(e in n for e in exclude)]
         # Only the hot path's own parameters live here (their gradients are written by the HIP backward programs).  Anything
         # else that is trainable -- e.g. a real backbone, which the reference trains at lr_backbone (main.py:253-271) -- would
@@ -148,6 +153,11 @@ class ParamArena:
         # Learning rate = base_lr (a host scalar baked into captured graphs) x this per-64-element DEVICE table: the table
         # carries the 0.1x group of sampling_offsets AND the schedule (set_lr rescales it in place, so a replayed graph
         # follows a StepLR exactly like the eager path does; main.py:278 lr_scheduler.step()).
+        self.muon_names = [n for n, p, _ in self.entries if p.dim() >= 2 and not self.MUON_SKIP.search(n)] if muon else []
+        for n, p, o in self.entries if muon else ():
+            if n in set(self.muon_names):
+                for i in range(o // ALIGN, (o + p.numel() + ALIGN - 1) // ALIGN):
+                    scale[i] = -scale[i]
         self.lr_scale_base = torch.tensor(scale, dtype=torch.float32, device=dev)
         self.lr_scale = self.lr_scale_base.clone()
         self.base_lr = self.lr = float(lr)
@@ -158,8 +168,25 @@ class ParamArena:
         self.step_count = 0
         self.step_word = torch.zeros(1, dtype=torch.int32, device=dev)       # device copy of step_count (graph replays bump it)
         self.world = 1
+        self.muon = None
+        if muon:
+            opts = {} if muon is True else dict(muon)
+            self.muon = (self._muon_plan(opts.pop("scale", "rms")), opts)
         # model.load_state_dict copies into the fp32 arena views in place; the bf16 operand shadow must follow
         model.register_load_state_dict_post_hook(lambda module, incompatible: self.refresh_shadow())
+
+    def _muon_plan(self, scale):
+        if not self.flat.is_cuda:
+            raise ValueError("ParamArena: Muon updates need the model on the GPU")
+        mats = []
+        for n, p, o in self.entries:
+            if n in set(self.muon_names):
+                parts = 3 if n.endswith("in_proj_weight") and p.shape[0] % 3 == 0 else 1
+                r, c = p.shape[0] // parts, p.numel() // p.shape[0]
+                mats += [(o + i * r * c, r, c, o // ALIGN) for i in range(parts)]
+        view = lambda flat: [flat[o:o + r * c].view(r, c) for o, r, c, _ in mats]       # noqa: E731
+        return ops.MuonPlan(view(self.flat), view(self.grad), view(self.m), scale=scale, p_bf16=view(self.flat_bf16), p_bf16_lo=view(self.flat_bf16_lo),
+                            lr_scale=[self.lr_scale[b:b + 1] for _, _, _, b in mats])
 
     def set_lr(self, lr: float):
         """Scheduler entry (the reference's StepLR, main.py:277-278): effective from the next optimiser launch, eager or
@@ -175,12 +202,17 @@ class ParamArena:
         """What the reference checkpoints as 'optimizer' + 'lr_scheduler' (main.py:293-301,364-372): Adam moments, step, lr."""
         if self.step_word.is_cuda:
             self.step_count = max(self.step_count, int(self.step_word.item()))
-        return {"m": self.m.detach().cpu().clone(), "v": self.v.detach().cpu().clone(), "step": self.step_count,
-                "lr": self.lr, "base_lr": self.base_lr, "names": [n for n, _, _ in self.entries]}
+        sd = {"m": self.m.detach().cpu().clone(), "v": self.v.detach().cpu().clone(), "step": self.step_count,
+              "lr": self.lr, "base_lr": self.base_lr, "names": [n for n, _, _ in self.entries]}
+        if self.muon_names:
+            sd["muon"] = list(self.muon_names)
+        return sd
 
     def load_state_dict(self, sd):
         if list(sd["names"]) != [n for n, _, _ in self.entries]:
             raise ValueError("ParamArena.load_state_dict: parameter layout differs from the checkpoint's")
+        if list(sd.get("muon", [])) != self.muon_names:
+            raise ValueError("ParamArena.load_state_dict: the checkpoint's moments belong to another choice of optimiser (muon)")
         self.m.copy_(sd["m"]); self.v.copy_(sd["v"])
         self.step_count = int(sd["step"])
         self.step_word.fill_(self.step_count)
@@ -256,6 +288,9 @@ class ParamArena:
                           self.eps, self.weight_decay, self.step_count, sqnorm_buf=sq, max_norm=max_norm, grad_scale=gs,
                           p_bf16=self.flat_bf16[a:b], step_dev=step_dev, lr_scale=self.lr_scale[a // ALIGN:],
                           p_bf16_lo=self.flat_bf16_lo[a:b])
+        if self.muon is not None:
+            plan, opts = self.muon
+            plan.step(**{"lr": self.groups[0][2], "weight_decay": self.weight_decay, "sqnorm_buf": sq, "max_norm": max_norm, "grad_scale": gs, **opts})
 
     def grad_norm(self) -> torch.Tensor:
         return torch.sqrt(self.sq[0]) / self.world
@@ -778,12 +813,13 @@ class Trainer:
     """One training step == engine.py:55-81 (forward, loss, zero_grad, backward, clip, AdamW)."""
 
     def __init__(self, model: nn.Module, criterion: SetCriterion, lr=2e-4, weight_decay=1e-4, max_norm=0.1,
-                 distributed: Optional[bool] = None):
+                 distributed: Optional[bool] = None, muon=None):
+        """muon: orthogonalised updates of the weight matrices (ParamArena)."""
         self.model, self.criterion, self.max_norm = model, criterion, max_norm
         # transformer.reference_points only receives a gradient with learned reference points (else it stays outside, as
         # torch.optim.AdamW skips parameters whose .grad is None)
         exclude = () if getattr(model, "ref_points_mode", "bbox") == "learned" else ("transformer.reference_points",)
-        self.arena = ParamArena(model, lr=lr, weight_decay=weight_decay, exclude=exclude)
+        self.arena = ParamArena(model, lr=lr, weight_decay=weight_decay, exclude=exclude, muon=muon)
         if distributed is None:
             distributed = dist.is_available() and dist.is_initialized() and (dist.get_world_size() > 1 or collectives_forced())
         self.reducer = BucketReducer(self.arena) if distributed else None
@@ -901,7 +937,7 @@ class GraphedTrainer(Trainer):
     Requirements: fixed batch size / image geometry, model in train() mode for the whole run."""
 
     def __init__(self, model, criterion, lr=2e-4, weight_decay=1e-4, max_norm=0.1, warm=3, segment_backward=None,
-                 persistent_inputs=False):
+                 persistent_inputs=False, muon=None):
         """persistent_inputs=True: the caller promises that the feature / mask tensors it passes are the SAME buffers on every
         step (a backbone writing into fixed outputs); they are then used as the graphs' static inputs without a copy.  The
         default keeps private static buffers and copies every step's inputs into them -- the trainer never writes into a
@@ -909,7 +945,7 @@ class GraphedTrainer(Trainer):
         # the base class broadcasts the parameters and owns the bucket reducer used by the EAGER warm-up steps (without it
         # the ranks would drift apart before the graphs are captured); the captured steps all-reduce the whole arena
         # themselves (see _Replay.backward) and run with the reducer detached
-        super().__init__(model, criterion, lr=lr, weight_decay=weight_decay, max_norm=max_norm, distributed=None)
+        super().__init__(model, criterion, lr=lr, weight_decay=weight_decay, max_norm=max_norm, distributed=None, muon=muon)
         self.world = dist.get_world_size() if dist.is_available() and dist.is_initialized() else 1
         self.arena.world = self.world
         self.warm, self.calls, self.ready = warm, 0, False

@@ -518,16 +518,28 @@ class HeadsRawFn(torch.autograd.Function):
 # ====================================================================================================
 # input_proj: 1x1 conv (+3x3 s2 conv for extra levels) + GroupNorm(32), written token-major
 # ====================================================================================================
+def _input_norm(pre, gw, gb, src, stats, groups, off, act, x16=None):
+    """GroupNorm [+ activation] of a projected level (N, HW, d) into rows [off, off + HW) of the token stream; x16: also pre in bf16."""
+    N, HW, d = pre.shape
+    if act is None:
+        ops.groupnorm_fwd(pre, gw, gb, src, stats, N, HW, d, groups, 0, HW, off, src.shape[1], x16=x16)
+        return
+    if x16 is not None:
+        ops.cast(pre, x16)
+    ops.groupnorm_act_fwd(pre, gw, gb, src[:, off:off + HW], groups, act, stats=stats)
+
+
 class InputProjFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, feats, geom, n_groups, dtypes, names, *params):
-        """feats: list of NCHW backbone maps (no grad).  Levels beyond len(feats) come from the 3x3 s2 conv of the
+        """dtypes: (branch, stream[, split weights[, activation behind the GroupNorm]]).  feats: list of NCHW backbone maps (no grad).  Levels beyond len(feats) come from the 3x3 s2 conv of the
         last backbone map (first extra level) or of the previous projected map (further ones)."""
         N = feats[0].shape[0]
         d = params[0].shape[0]
         S = geom.S
         act_dtype, stream_dtype = dtypes[:2]      # branch (conv output) dtype, residual-stream dtype
         split = len(dtypes) > 2 and bool(dtypes[2]) and act_dtype == torch.bfloat16     # fp32 conv weights as bf16 hi + lo
+        gn_act = dtypes[3] if len(dtypes) > 3 else None
         src = torch.empty((N, S, d), dtype=stream_dtype, device=feats[0].device)
         saved = []
         for lvl in range(geom.L):
@@ -554,7 +566,7 @@ class InputProjFn(torch.autograd.Function):
                         pre32 = torch.empty((N, HW, d), dtype=torch.float32, device=src.device)
                         ops.linear_fwd(f2, torch.cat([W.view(d, C), W.view(d, C)], 1), b, pre32.view(N * HW, d), split=True)
                         stats = torch.empty((N, n_groups, 2), dtype=torch.float32, device=src.device)
-                        ops.groupnorm_fwd(pre32, gw, gb, src, stats, N, HW, d, n_groups, 0, HW, geom.starts[lvl], S, x16=pre)      # (+ the bf16 copy backward reads)
+                        _input_norm(pre32, gw, gb, src, stats, n_groups, geom.starts[lvl], gn_act, x16=pre)      # (+ the bf16 copy backward reads)
                         saved.append((f2, None, pre, stats))
                         continue
                     f16 = torch.empty((N * HW, C), dtype=torch.bfloat16, device=src.device)
@@ -589,7 +601,7 @@ class InputProjFn(torch.autograd.Function):
                     col = torch.empty((N * HW, C * 9), dtype=torch.bfloat16, device=src.device)     # (backward's operand copy)
                     ops.cast(col32, col)
                     stats = torch.empty((N, n_groups, 2), dtype=torch.float32, device=src.device)
-                    ops.groupnorm_fwd(pre32, gw, gb, src, stats, N, HW, d, n_groups, 0, HW, geom.starts[lvl], S, x16=pre)
+                    _input_norm(pre32, gw, gb, src, stats, n_groups, geom.starts[lvl], gn_act, x16=pre)
                     saved.append((None, col, pre, stats))
                     continue
                 col = torch.empty((N * HW, C * 9), dtype=act_dtype, device=src.device)
@@ -597,10 +609,10 @@ class InputProjFn(torch.autograd.Function):
                 ops.linear_fwd(col, W.view(d, C * 9), b, pre, split=split)
                 f = None
             stats = torch.empty((N, n_groups, 2), dtype=torch.float32, device=src.device)
-            ops.groupnorm_fwd(pre, gw, gb, src, stats, N, HW, d, n_groups, 0, HW, geom.starts[lvl], S)
+            _input_norm(pre, gw, gb, src, stats, n_groups, geom.starts[lvl], gn_act)
             saved.append((f, col, pre, stats))
         ctx.saved, ctx.geom, ctx.n_groups, ctx.names, ctx.params, ctx.dims = saved, geom, n_groups, names, params, (N, S, d)
-        ctx.n_feats = len(feats)
+        ctx.n_feats, ctx.gn_act = len(feats), gn_act
         return src
 
     @staticmethod
@@ -618,8 +630,13 @@ class InputProjFn(torch.autograd.Function):
             HW = H * Wd
             gw = params[names.index(f"{lvl}.1.weight")]
             dpre = torch.empty_like(pre)
-            ops.groupnorm_bwd(dsrc, pre, stats, gw, dpre, G(f"{lvl}.1.weight"), G(f"{lvl}.1.bias"), N, HW, d, ctx.n_groups,
-                              0, HW, geom.starts[lvl], S)
+            if ctx.gn_act is None:
+                ops.groupnorm_bwd(dsrc, pre, stats, gw, dpre, G(f"{lvl}.1.weight"), G(f"{lvl}.1.bias"), N, HW, d, ctx.n_groups,
+                                  0, HW, geom.starts[lvl], S)
+            else:
+                o = geom.starts[lvl]
+                ops.groupnorm_act_bwd(dsrc[:, o:o + HW], pre, stats, gw, params[names.index(f"{lvl}.1.bias")], ctx.n_groups, ctx.gn_act, dx=dpre,
+                                      dgamma=G(f"{lvl}.1.weight"), dbeta=G(f"{lvl}.1.bias"), accumulate=True)
             gW = G(f"{lvl}.0.weight")
             if lvl > ctx.n_feats:                  # pose_estimation_transformer.py:327-330: input_proj[lvl](srcs[-1])
                 W = params[names.index(f"{lvl}.0.weight")]

@@ -427,8 +427,12 @@ class PoET(nn.Module):
 
     def __init__(self, backbone, transformer, num_queries, num_feature_levels, n_classes, bbox_mode="gt",
                  ref_points_mode="bbox", query_embedding_mode="bbox", rotation_mode="6d", class_mode="agnostic",
-                 aleatoric=False, aux_loss=True, backbone_type="yolo"):
+                 aleatoric=False, aux_loss=True, backbone_type="yolo", input_proj_act=None):
+        """input_proj_act: an activation behind the input projection's GroupNorm ("relu", "gelu", "silu"; the reference has none)."""
         super().__init__()
+        if input_proj_act is not None and input_proj_act not in ops.ACT:
+            raise ValueError(f"input_proj_act must be None or one of {sorted(ops.ACT)}, got {input_proj_act!r}")
+        self.input_proj_act = input_proj_act
         if bbox_mode not in ("gt", "jitter", "backbone"):
             raise NotImplementedError("PoET Bounding Box Mode not implemented!")
         if query_embedding_mode not in ("bbox", "learned"):
@@ -552,7 +556,7 @@ class PoET(nn.Module):
             masks.append(m)
         geom = LevelGeom(shapes)
         names, params = _named(self.input_proj)
-        src = Fn.InputProjFn.apply(feats, geom, 32, (act, stream, tr.split_w), names, *params)
+        src = Fn.InputProjFn.apply(feats, geom, 32, (act, stream, tr.split_w, self.input_proj_act), names, *params)
         self._last_src = src                          # autograd-node boundaries: the graphed trainer splits backward here
         lvl_embed = tr.level_embed.detach().contiguous()
         pe = self.backbone[1] if hasattr(self.backbone, "__getitem__") else None

@@ -1021,54 +1021,71 @@ def orthogonalize(g, out=None, steps=5, coeffs=NS_COEFFS, eps=1e-7):
 MUON_SCALES = {"spectral": lambda r, c: max(1.0, r / c) ** 0.5, "rms": lambda r, c: 0.2 * max(r, c) ** 0.5}
 
 
+class MuonPlan:
+    """A list of fp32 weight matrices with their gradients and moments (more than two dimensions: rows x the rest), checked once, for the
+    updates of a training run: `plan.step(lr, ...)` = muon_step on them.  The tensors are held, and have to stay where they are.
+    Optional, as of adamw: the bf16 images of the parameters (lists), lr_scale = one device word per matrix (its magnitude counts)."""
+
+    def __init__(self, params, grads, moments, scale="spectral", p_bf16=None, p_bf16_lo=None, lr_scale=None):
+        params, grads, moments = list(params), list(grads), list(moments)
+        self.n = n = len(params)
+        if not (len(grads) == len(moments) == n) or any(l is not None and len(l) != n for l in (p_bf16, p_bf16_lo, lr_scale)):
+            raise ValueError("poet_amd: a Muon update takes lists of one length")
+        if scale not in MUON_SCALES:
+            raise ValueError(f"poet_amd: scale must be one of {sorted(MUON_SCALES)}, got {scale!r}")
+        if p_bf16_lo is not None and p_bf16 is None:
+            raise ValueError("poet_amd: p_bf16_lo goes with p_bf16")
+        if n == 0:
+            return
+        dev = _req(params[0], "params").device
+        f32, bf16 = torch.float32, torch.bfloat16
+        for p, g, m in zip(params, grads, moments):
+            if not (p.dtype is f32 and g.dtype is f32 and m.dtype is f32 and p.is_contiguous() and g.is_contiguous() and m.is_contiguous()
+                    and p.device == dev and g.device == dev and m.device == dev and p.shape == g.shape == m.shape):
+                raise ValueError("poet_amd: parameter, gradient and moment of a matrix are contiguous fp32 tensors of one shape on one device")
+        for l, dt in ((p_bf16, bf16), (p_bf16_lo, bf16), (lr_scale, f32)):
+            if l is not None:
+                for p, t in zip(params, l):
+                    if t.dtype != dt or t.device != dev or not t.is_contiguous() or (t.numel() != p.numel() if dt is bf16 else t.numel() < 1):
+                        raise ValueError("poet_amd: bf16 images are contiguous bf16 tensors of the parameter's size, lr_scale fp32 words, on its device")
+        self.rows, self.cols = _muon_dims([p.shape for p in params])
+        pp, mp = [p.data_ptr() for p in params], [m.data_ptr() for m in moments]
+        if len(set(pp + mp)) != 2 * n:
+            raise ValueError("poet_amd: the same parameter or moment twice in one call")
+        ptrs = C.c_void_p * n
+        lst = lambda l: None if l is None else ptrs(*[t.data_ptr() for t in l])        # noqa: E731
+        fn = MUON_SCALES[scale]
+        self.arrays = (ptrs(*pp), lst(grads), ptrs(*mp), lst(p_bf16), lst(p_bf16_lo), lst(lr_scale),
+                       (C.c_float * n)(*[fn(r, c) for r, c in zip(self.rows, self.cols)]), self.rows, self.cols, n)
+        self.device, self.held = dev, (params, grads, moments, p_bf16, p_bf16_lo, lr_scale)
+
+    def step(self, lr, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5, coeffs=NS_COEFFS, eps=1e-7, sqnorm_buf=None, max_norm=0.0, grad_scale=1.0):
+        if not 0.0 <= momentum < 1.0:
+            raise ValueError(f"poet_amd: momentum must be in [0, 1), got {momentum}")
+        if not 1 <= steps <= 16:
+            raise ValueError(f"poet_amd: 1 .. 16 steps, got {steps}")
+        if self.n == 0:
+            return
+        if sqnorm_buf is not None and (sqnorm_buf.dtype != torch.float32 or sqnorm_buf.device != self.device):
+            raise ValueError("poet_amd: sqnorm_buf is an fp32 tensor on the parameters' device")
+        lib = _lib.load()
+        cf = _ns_coeffs(coeffs, steps)
+        with _on_device(self.held[0][0]) as stream:
+            ws = _muon_ws(lib, self.rows, self.cols, self.n, self.device)
+            _lib.check(lib.poet_muon_step(*self.arrays, lr, momentum, int(nesterov), weight_decay, steps, cf, eps, _ptr(sqnorm_buf), max_norm, grad_scale,
+                                          ws.data_ptr(), ws.numel(), stream), "poet_muon_step")
+
+
 def muon_step(params, grads, moments, lr, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5, coeffs=NS_COEFFS, eps=1e-7, scale="spectral",
               p_bf16=None, p_bf16_lo=None, lr_scale=None, sqnorm_buf=None, max_norm=0.0, grad_scale=1.0):
     """One Muon update, in place, of a list of fp32 weight matrices (more than two dimensions: rows x the rest):
         m <- momentum m + (1 - momentum) g;  u = momentum m + (1 - momentum) g (nesterov) or m;
         p <- p (1 - lr weight_decay) - lr s orthogonalize(u)
     s: "spectral" = sqrt(max(1, rows / cols)), "rms" = 0.2 sqrt(max(rows, cols)) (the step size of AdamW).  Optional, as of adamw: the
-    gradient scale and clip (sqnorm_buf, max_norm), the bf16 images of p (lists), lr_scale = one device word per matrix (its magnitude)."""
-    params, grads, moments = list(params), list(grads), list(moments)
-    n = len(params)
-    if not (len(grads) == len(moments) == n) or any(l is not None and len(l) != n for l in (p_bf16, p_bf16_lo, lr_scale)):
-        raise ValueError("poet_amd: muon_step takes lists of one length")
-    if scale not in MUON_SCALES:
-        raise ValueError(f"poet_amd: scale must be one of {sorted(MUON_SCALES)}, got {scale!r}")
-    if not 0.0 <= momentum < 1.0:
-        raise ValueError(f"poet_amd: momentum must be in [0, 1), got {momentum}")
-    if not 1 <= steps <= 16:
-        raise ValueError(f"poet_amd: 1 .. 16 steps, got {steps}")
-    if p_bf16_lo is not None and p_bf16 is None:
-        raise ValueError("poet_amd: p_bf16_lo goes with p_bf16")
-    if n == 0:
-        return
-    dev = _req(params[0], "params").device
-    f32, bf16 = torch.float32, torch.bfloat16
-    for p, g, m in zip(params, grads, moments):
-        if not (p.dtype == g.dtype == m.dtype == f32 and p.is_contiguous() and g.is_contiguous() and m.is_contiguous()
-                and p.device == g.device == m.device == dev and p.shape == g.shape == m.shape):
-            raise ValueError("poet_amd: parameter, gradient and moment of a matrix are contiguous fp32 tensors of one shape on one device")
-    for l, dt in ((p_bf16, bf16), (p_bf16_lo, bf16), (lr_scale, f32)):
-        if l is not None:
-            for p, t in zip(params, l):
-                if t.dtype != dt or t.device != dev or not t.is_contiguous() or (dt is bf16 and t.numel() != p.numel()):
-                    raise ValueError("poet_amd: bf16 images are contiguous bf16 tensors of the parameter's size, lr_scale fp32 words, on its device")
-    if sqnorm_buf is not None and (sqnorm_buf.dtype != f32 or sqnorm_buf.device != dev):
-        raise ValueError("poet_amd: sqnorm_buf is an fp32 tensor on the parameters' device")
-    rows, cols = _muon_dims([p.shape for p in params])
-    pp, mp = [p.data_ptr() for p in params], [m.data_ptr() for m in moments]
-    if len(set(pp + mp)) != 2 * n:
-        raise ValueError("poet_amd: the same parameter or moment twice in one call")
-    lib = _lib.load()
-    fn = MUON_SCALES[scale]
-    cf = _ns_coeffs(coeffs, steps)
-    ptrs = C.c_void_p * n
-    lst = lambda l: None if l is None else ptrs(*[t.data_ptr() for t in l])        # noqa: E731
-    with _on_device(params[0]) as stream:
-        ws = _muon_ws(lib, rows, cols, n, dev)
-        _lib.check(lib.poet_muon_step(ptrs(*pp), lst(grads), ptrs(*mp), lst(p_bf16), lst(p_bf16_lo), lst(lr_scale),
-                                      (C.c_float * n)(*[fn(r, c) for r, c in zip(rows, cols)]), rows, cols, n, lr, momentum, int(nesterov), weight_decay,
-                                      steps, cf, eps, _ptr(sqnorm_buf), max_norm, grad_scale, ws.data_ptr(), ws.numel(), stream), "poet_muon_step")
+    gradient scale and clip (sqnorm_buf, max_norm), the bf16 images of p (lists), lr_scale = one device word per matrix (its magnitude).
+    MuonPlan keeps the checked lists of a training run."""
+    MuonPlan(params, grads, moments, scale, p_bf16, p_bf16_lo, lr_scale).step(lr, momentum, nesterov, weight_decay, steps, coeffs, eps, sqnorm_buf, max_norm,
+                                                                              grad_scale)
 
 
 def counter_add(word, delta=1):
