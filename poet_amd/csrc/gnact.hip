@@ -18,9 +18,13 @@
 // Nothing is accumulated with atomics: results do not depend on the order of workgroups.
 #include "common.cuh"
 
+#include <type_traits>
+
 namespace poet {
 
 namespace {
+
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 
 constexpr int NT = 256;
 
@@ -32,6 +36,7 @@ struct GnaP {
     const float* beta;
     float* stats;                           // (N, G, 2) mean, rstd: written by forward, read by backward
     float2* part;                           // (N, G, T * P) partials of a group
+    float2* folded;                         // (N, G): forward (mean, rstd) -- the stats when asked for --, backward the two means over the group
     float2* cpart;                          // (N, T, C) backward: (sum dz, sum dz h) per channel
     float* dgamma;
     float* dbeta;
@@ -39,7 +44,8 @@ struct GnaP {
     int T, R;                               // row chunks of R rows
     int nslab, gps, P, cpp;                 // slabs of gps whole groups (P == 1), or a group in P pieces of cpp channels
     int tail;                               // backward, second launch: leading workgroups that reduce dgamma / dbeta
-    int accumulate;
+    int accumulate, act;
+    int reverse;                            // second pass: from the last row to the first
     float eps;
 };
 
@@ -95,6 +101,13 @@ struct Blk {
     int LPR, RP, r, l;                // lanes per row, rows per pass, this thread's row / lane
     bool active;
 };
+// Where the first pass read more than the memory-side cache keeps, the second takes the chunks, and their rows, in the opposite order, each on
+// the XCD (b % 8) of the first: what was read last is still there (backward, 8 x 19200 x 256 fp32, 315 MB: 171 -> 148 us; below the
+// cache's size the way back is 5 % slower)
+__device__ __forceinline__ int turned(const GnaP& p, int b, int total) {
+    const int q = total >> 3;
+    return p.reverse && b < q * 8 ? (q - 1 - (b >> 3)) * 8 + (b & 7) : b;
+}
 template <int V> __device__ __forceinline__ Blk decode(const GnaP& p, int b) {
     Blk k;
     k.t = b % p.T;
@@ -123,6 +136,17 @@ template <int V> __device__ __forceinline__ Blk decode(const GnaP& p, int b) {
     k.l = threadIdx.x - k.r * k.LPR;
     k.active = k.r < k.RP;
     return k;
+}
+
+constexpr int ROWS_AHEAD = 2;      // vectors of a thread in flight (4: 84 -> 94 us backward at 8 x 19200 x 256 fp16, GELU; 8: 104)
+// this thread's first row in the chunk (the last one of its strides of ROWS_AHEAD RP when reversed), and the stride
+__device__ __forceinline__ int first_row(const GnaP& p, const Blk& k, int& step) {
+    step = ROWS_AHEAD * k.RP;
+    const int n = k.row1 - k.row0 - k.r;
+    if (!p.reverse || n <= 0) return k.row0 + k.r;
+    const int last = k.row0 + k.r + (n - 1) / step * step;
+    step = -step;
+    return last;
 }
 
 // per-thread, per-channel values -> one sum per channel (chan) -> one per group of the slab (grp).  red: RP x Cs floats.
@@ -157,7 +181,6 @@ __device__ __forceinline__ void to_groups(const Blk& k, const float* chan, float
     __syncthreads();
 }
 
-constexpr int ROWS_AHEAD = 4;      // vectors of a thread in flight
 
 // ---- forward, 1: (mean, M2) per group of the chunk ------------------------------------------------------
 template <typename TX, int V> __global__ __launch_bounds__(NT) void gna_stats_kernel(const GnaP p) {
@@ -212,7 +235,8 @@ template <typename TX, typename TY, int V, int ACT>
 __device__ __forceinline__ void apply_rows(const GnaP& p, const Blk& k, const float* mean, const float* sc, const float* sh) {
     const TX* x = (const TX*)p.x + k.n * p.xn + k.c0 + k.l * V;
     TY* y = (TY*)p.y + k.n * p.yn + k.c0 + k.l * V;
-    for (int row = k.row0 + k.r; row < k.row1; row += ROWS_AHEAD * k.RP) {
+    int step;
+    for (int row = first_row(p, k, step); row < k.row1 && row >= k.row0; row += step) {
         float v[ROWS_AHEAD][V];
 #pragma unroll
         for (int u = 0; u < ROWS_AHEAD; ++u)
@@ -227,42 +251,51 @@ __device__ __forceinline__ void apply_rows(const GnaP& p, const Blk& k, const fl
     }
 }
 
-template <typename TX, typename TY, int V, int ACT> __global__ __launch_bounds__(NT) void gna_apply_kernel(const GnaP p) {
-    __shared__ float gm[NT * V], gr[NT * V];
-    const Blk k = decode<V>(p, blockIdx.x);
-    const int team = team_of(k.ng), per = NT / team, m = threadIdx.x & (team - 1), E = p.T * p.P;
+// a wave per (image, group): the partials of its chunks -> (mean, rstd), or backward (BWD) the two means of dx's formula
+template <bool BWD> __global__ __launch_bounds__(NT) void gna_fold_kernel(const GnaP p) {
+    const int64_t ng = (int64_t)blockIdx.x * (NT / 64) + (threadIdx.x >> 6);
+    if (ng >= (int64_t)p.N * p.G) return;
+    const int lane = threadIdx.x & 63, E = p.T * p.P;
     const float total = (float)p.HW * (float)p.cpg;
-    for (int b = 0; b < k.ng; b += per) {
-        const int g = b + threadIdx.x / team;
-        const float2* e = p.part + ((int64_t)k.n * p.G + k.g0 + (g < k.ng ? g : 0)) * E;
+    const float2* e = p.part + ng * E;
+    if constexpr (BWD) {
+        float s1 = 0.f, s2 = 0.f;
+#pragma unroll 4
+        for (int i = lane; i < E; i += 64) s1 += e[i].x, s2 += e[i].y;
+        s1 = team_sum(s1, 64);
+        s2 = team_sum(s2, 64);
+        if (lane == 0) p.folded[ng] = make_float2(s1 / total, s2 / total);
+    } else {
         auto weight = [&](int i) {
-            const int t = i / p.P, q = i - t * p.P;
+            const int t = p.P == 1 ? i : i / p.P, q = i - t * p.P;
             return (float)(min(p.HW, (t + 1) * p.R) - t * p.R) * (float)(p.P == 1 ? p.cpg : min(p.cpp, p.cpg - q * p.cpp));
         };
         const float m0 = e[0].x;
         float s = 0.f;
-        for (int i = m; i < E; i += team) s = fmaf(weight(i), e[i].x - m0, s);
-        const float mean = m0 + team_sum(s, team) / total;
+#pragma unroll 4
+        for (int i = lane; i < E; i += 64) s = fmaf(weight(i), e[i].x - m0, s);
+        const float mean = m0 + team_sum(s, 64) / total;
         float q = 0.f;
-        for (int i = m; i < E; i += team) {
+#pragma unroll 4
+        for (int i = lane; i < E; i += 64) {
             const float d = e[i].x - mean;
             q += fmaf(weight(i) * d, d, e[i].y);
         }
-        const float rstd = 1.f / sqrtf(team_sum(q, team) / total + p.eps);
-        if (g < k.ng && m == 0) {
-            gm[g] = mean;
-            gr[g] = rstd;
-            if (k.t == 0 && k.piece == 0 && p.stats) *reinterpret_cast<float2*>(p.stats + 2 * ((int64_t)k.n * p.G + k.g0 + g)) = make_float2(mean, rstd);
-        }
+        q = team_sum(q, 64);
+        if (lane == 0) p.folded[ng] = make_float2(mean, 1.f / sqrtf(q / total + p.eps));
     }
-    __syncthreads();
+}
+
+template <typename TX, typename TY, int V, int ACT> __global__ __launch_bounds__(NT) void gna_apply_kernel(const GnaP p) {
+    const Blk k = decode<V>(p, turned(p, blockIdx.x, gridDim.x));
     if (!k.active) return;
     float mean[V], sc[V], sh[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        const int c = k.l * V + i, g = c / k.cps;
-        mean[i] = gm[g];
-        sc[i] = p.gamma[k.c0 + c] * gr[g];
+        const int c = k.l * V + i;
+        const float2 st = p.folded[(int64_t)k.n * p.G + k.g0 + c / k.cps];
+        mean[i] = st.x;
+        sc[i] = p.gamma[k.c0 + c] * st.y;
         sh[i] = p.beta[k.c0 + c];
     }
     apply_rows<TX, TY, V, ACT>(p, k, mean, sc, sh);
@@ -352,34 +385,22 @@ __device__ __forceinline__ void reduce_params(const GnaP& p, int b) {
 
 template <typename TX, typename TY, int V, int ACT> __global__ __launch_bounds__(NT) void gna_bwd_apply_kernel(const GnaP p) {
     if ((int)blockIdx.x < p.tail) return reduce_params(p, blockIdx.x);
-    __shared__ float g1[NT * V], g2[NT * V];
-    const Blk k = decode<V>(p, blockIdx.x - p.tail);
-    const int team = team_of(k.ng), per = NT / team, m = threadIdx.x & (team - 1), E = p.T * p.P;
-    const float inv = 1.f / ((float)p.HW * (float)p.cpg);
-    for (int b = 0; b < k.ng; b += per) {
-        const int g = b + threadIdx.x / team;
-        const float2* e = p.part + ((int64_t)k.n * p.G + k.g0 + (g < k.ng ? g : 0)) * E;
-        float s1 = 0.f, s2 = 0.f;
-        for (int i = m; i < E; i += team) s1 += e[i].x, s2 += e[i].y;
-        s1 = team_sum(s1, team);
-        s2 = team_sum(s2, team);
-        if (g < k.ng && m == 0) g1[g] = s1 * inv, g2[g] = s2 * inv;
-    }
-    __syncthreads();
+    const Blk k = decode<V>(p, turned(p, blockIdx.x - p.tail, gridDim.x - p.tail));
     if (!k.active) return;
     Chan ch[V];
     load_chan<V>(p, k, ch);
     float k2[V], k3[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        const int g = (k.l * V + i) / k.cps;
-        k2[i] = -ch[i].rstd * g1[g];
-        k3[i] = -ch[i].rstd * g2[g];
+        const float2 m = p.folded[(int64_t)k.n * p.G + k.g0 + (k.l * V + i) / k.cps];
+        k2[i] = -ch[i].rstd * m.x;
+        k3[i] = -ch[i].rstd * m.y;
     }
     const TX* x = (const TX*)p.x + k.n * p.xn + k.c0 + k.l * V;
     const TY* dy = (const TY*)p.dy + k.n * p.dn + k.c0 + k.l * V;
     TX* dx = (TX*)p.y + k.n * p.yn + k.c0 + k.l * V;
-    for (int row = k.row0 + k.r; row < k.row1; row += ROWS_AHEAD * k.RP) {
+    int step;
+    for (int row = first_row(p, k, step); row < k.row1 && row >= k.row0; row += step) {
         float v[ROWS_AHEAD][V], w[ROWS_AHEAD][V];
 #pragma unroll
         for (int u = 0; u < ROWS_AHEAD; ++u)
@@ -401,7 +422,247 @@ template <typename TX, typename TY, int V, int ACT> __global__ __launch_bounds__
     }
 }
 
+// ---- whole images in registers: one launch ------------------------------------------------------------------------------------
+// Where the rows of a few groups of an image fit a workgroup's registers (up to 192 KB), x is read once, the statistics are plain two-pass
+// sums over registers, and a forward pass is ONE launch: what small calls cost is launches, and a level of 4800 rows saves its re-read.  Needs
+// whole vectors in a group.  A workgroup takes gpw neighbouring groups: lanes l of a row's LPR = gpw * cpg / V, rows threadIdx / LPR + u RP.
+template <typename T, int V> struct Raw {
+    u32x4_t w;
+    __device__ __forceinline__ void ld(const T* p) { w = *reinterpret_cast<const u32x4_t*>(p); }
+    __device__ __forceinline__ void get(float* o) const {
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[i] = __uint_as_float(w[i]);
+        } else if constexpr (std::is_same<T, bf16_t>::value) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[2 * i] = __uint_as_float(w[i] << 16), o[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[2 * i] = h_lo(w[i]), o[2 * i + 1] = h_hi(w[i]);
+        }
+    }
+};
+template <typename T> struct Raw<T, 1> {
+    float w;
+    __device__ __forceinline__ void ld(const T* p) { w = io<T>::ld(p); }
+    __device__ __forceinline__ void get(float* o) const { o[0] = w; }
+};
+// sum of v over the workgroup's threads that share this thread's group (lanes lg * g .. of every LPR): lg and LPR powers of two up to 64, or
+// one group for the whole workgroup
+template <int BT> __device__ __forceinline__ float group_sum(float v, float* sh, int lg, int LPR, bool one, int grp) {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1)
+        if (one || o < lg || o >= LPR) v += __shfl_xor(v, o, 64);
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    __syncthreads();
+    if (one ? lane == 0 : lane < LPR && (lane & (lg - 1)) == 0) sh[wave * 64 + (one ? 0 : lane / lg)] = v;
+    __syncthreads();
+    float s = 0.f;
+#pragma unroll
+    for (int w = 0; w < BT / 64; ++w) s += sh[w * 64 + grp];
+    return s;
+}
+struct Fit {                            // where this thread works
+    int n, g0, c, grp, l, r, LPR, RP, lg;
+    bool one, active;
+};
+template <int BT, int V> __device__ __forceinline__ Fit fit_of(const GnaP& p) {
+    Fit f;
+    const int b = blockIdx.x, total = gridDim.x, q = total >> 3, rem = total & 7, x = b & 7;
+    const int k = x * q + min(x, rem) + (b >> 3);          // neighbouring groups share 128-byte lines: the same XCD, at about the same time
+    const int per = p.G / p.gps;
+    f.n = k / per;
+    f.g0 = (k - f.n * per) * p.gps;
+    f.lg = p.cpg / V;
+    f.LPR = f.lg * p.gps;
+    f.RP = BT / f.LPR;
+    f.r = threadIdx.x / f.LPR;
+    f.l = threadIdx.x - f.r * f.LPR;
+    f.one = p.gps == 1;
+    f.grp = f.one ? 0 : f.l / f.lg;
+    f.c = f.g0 * p.cpg + f.l * V;
+    f.active = f.r < f.RP;
+    return f;
+}
+
+template <typename TX, int V, int BT, int NR> __global__ __launch_bounds__(BT) void gna_fit_kernel(const GnaP p) {
+    __shared__ float sh[BT / 64 * 64];
+    const Fit f = fit_of<BT, V>(p);
+    const TX* x = (const TX*)p.x + f.n * p.xn + f.c;
+    Raw<TX, V> raw[NR];
+    float s = 0.f, first = 0.f;                            // (sums against the thread's first value: a mean far from 0 costs no digits)
+    const int rows = f.active ? p.HW : 0;
+#pragma unroll
+    for (int u = 0; u < NR; ++u)
+        if (f.r + u * f.RP < rows) raw[u].ld(x + (f.r + u * f.RP) * p.xr);
+    int cnt = 0;
+#pragma unroll
+    for (int u = 0; u < NR; ++u)
+        if (f.r + u * f.RP < rows) {
+            float v[V];
+            raw[u].get(v);
+            if (u == 0) first = v[0];
+            cnt += V;
+#pragma unroll
+            for (int i = 0; i < V; ++i) s += v[i] - first;
+        }
+    s = fmaf((float)cnt, first, s);
+    const float inv = 1.f / ((float)p.HW * (float)p.cpg);
+    const float mean = group_sum<BT>(s, sh, f.lg, f.LPR, f.one, f.grp) * inv;
+    s = 0.f;
+#pragma unroll
+    for (int u = 0; u < NR; ++u)
+        if (f.r + u * f.RP < rows) {
+            float v[V];
+            raw[u].get(v);
+#pragma unroll
+            for (int i = 0; i < V; ++i) s = fmaf(v[i] - mean, v[i] - mean, s);
+        }
+    const float rstd = 1.f / sqrtf(group_sum<BT>(s, sh, f.lg, f.LPR, f.one, f.grp) * inv + p.eps);
+    if (p.stats && f.r == 0 && f.l % f.lg == 0) *reinterpret_cast<float2*>(p.stats + 2 * ((int64_t)f.n * p.G + f.g0 + f.grp)) = make_float2(mean, rstd);
+    if (!f.active) return;
+    float sc[V], b[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) sc[i] = p.gamma[f.c + i] * rstd, b[i] = p.beta[f.c + i];
+    TX* y = (TX*)p.y + f.n * p.yn + f.c;
+    auto rest = [&](auto act) {
+#pragma unroll
+        for (int u = 0; u < NR; ++u)
+            if (f.r + u * f.RP < rows) {
+                float v[V];
+                raw[u].get(v);
+#pragma unroll
+                for (int i = 0; i < V; ++i) v[i] = act_f<decltype(act)::value>(fmaf(v[i] - mean, sc[i], b[i]));
+                stv<TX, V>(y + (f.r + u * f.RP) * p.yr, v);
+            }
+    };
+    if (p.act == A_NONE) rest(std::integral_constant<int, A_NONE>());
+    else if (p.act == A_RELU) rest(std::integral_constant<int, A_RELU>());
+    else if (p.act == A_GELU) rest(std::integral_constant<int, A_GELU>());
+    else rest(std::integral_constant<int, A_SILU>());
+}
+
+// backward: x and dy stay in registers; leaves the channel sums of the image in cpart (N, C), or in dgamma / dbeta when N == 1
+template <typename TX, int V, int BT, int NR> __global__ __launch_bounds__(BT) void gna_fit_bwd_kernel(const GnaP p) {
+    constexpr int W = BT / 64;
+    __shared__ float red[BT * V], tot[64 * V][2];
+    const Fit f = fit_of<BT, V>(p);
+    const TX* x = (const TX*)p.x + f.n * p.xn + f.c;
+    const TX* dy = (const TX*)p.dy + f.n * p.dn + f.c;
+    Raw<TX, V> raw[NR], rdy[NR];
+    const int rows = f.active ? p.HW : 0;
+#pragma unroll
+    for (int u = 0; u < NR; ++u)
+        if (f.r + u * f.RP < rows) {
+            raw[u].ld(x + (f.r + u * f.RP) * p.xr);
+            rdy[u].ld(dy + (f.r + u * f.RP) * p.dr);
+        }
+    const float2 st = *reinterpret_cast<const float2*>(p.stats + 2 * ((int64_t)f.n * p.G + f.g0 + f.grp));
+    const float mean = st.x, rstd = st.y;
+    float ga[V], be[V], a[V], b[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) ga[i] = p.gamma[f.c + i], be[i] = p.beta[f.c + i], a[i] = b[i] = 0.f;
+    auto sums = [&](auto act) {
+#pragma unroll
+        for (int u = 0; u < NR; ++u)
+            if (f.r + u * f.RP < rows) {
+                float v[V], w[V];
+                raw[u].get(v);
+                rdy[u].get(w);
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    const float h = (v[i] - mean) * rstd, dz = act_df<decltype(act)::value>(fmaf(h, ga[i], be[i]), w[i]);
+                    a[i] += dz;
+                    b[i] = fmaf(dz, h, b[i]);
+                }
+            }
+    };
+    if (p.act == A_NONE) sums(std::integral_constant<int, A_NONE>());
+    else if (p.act == A_RELU) sums(std::integral_constant<int, A_RELU>());
+    else if (p.act == A_GELU) sums(std::integral_constant<int, A_GELU>());
+    else sums(std::integral_constant<int, A_SILU>());
+    // rows -> one sum per channel.  LPR a power of two: lanes of one column meet by exchanges; else every thread's own go through LDS
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, Cs = f.LPR * V;
+    const bool pow2 = (f.LPR & (f.LPR - 1)) == 0;          // (LPR <= 64)
+    if (pow2) {
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1)
+            if (o >= f.LPR) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) a[i] += __shfl_xor(a[i], o, 64), b[i] += __shfl_xor(b[i], o, 64);
+            }
+    }
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        const float* v = q ? b : a;
+        __syncthreads();
+        if (pow2) {
+            if (lane < f.LPR)
+#pragma unroll
+                for (int i = 0; i < V; ++i) red[wave * Cs + lane * V + i] = v[i];
+        } else if (f.active) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) red[threadIdx.x * V + i] = v[i];
+        }
+        __syncthreads();
+        if (pow2) {
+            for (int c = threadIdx.x; c < Cs; c += BT) {
+                float s = 0.f;
+#pragma unroll
+                for (int w = 0; w < W; ++w) s += red[w * Cs + c];
+                tot[c][q] = s;
+            }
+        } else {
+            for (int c = wave; c < Cs; c += W) {           // a wave per channel
+                float s = 0.f;
+                for (int r = lane; r < f.RP; r += 64) s += red[r * Cs + c];
+                s = team_sum(s, 64);
+                if (lane == 0) tot[c][q] = s;
+            }
+        }
+    }
+    __syncthreads();
+    if (p.dgamma)
+        for (int c = threadIdx.x; c < Cs; c += BT) {
+            const int cc = f.g0 * p.cpg + c;
+            if (p.N == 1) {
+                p.dbeta[cc] = (p.accumulate ? p.dbeta[cc] : 0.f) + tot[c][0];
+                p.dgamma[cc] = (p.accumulate ? p.dgamma[cc] : 0.f) + tot[c][1];
+            } else p.cpart[(int64_t)f.n * p.C + cc] = make_float2(tot[c][0], tot[c][1]);
+        }
+    if (!p.y || !f.active) return;
+    float s1 = 0.f, s2 = 0.f;
+    for (int c = f.grp * p.cpg; c < (f.grp + 1) * p.cpg; ++c) {
+        const float g = p.gamma[f.g0 * p.cpg + c];
+        s1 = fmaf(g, tot[c][0], s1);
+        s2 = fmaf(g, tot[c][1], s2);
+    }
+    const float inv = rstd / ((float)p.HW * (float)p.cpg), k2 = -s1 * inv, k3 = -s2 * inv;
+    TX* dx = (TX*)p.y + f.n * p.yn + f.c;
+    auto rest = [&](auto act) {
+#pragma unroll
+        for (int u = 0; u < NR; ++u)
+            if (f.r + u * f.RP < rows) {
+                float v[V], w[V];
+                raw[u].get(v);
+                rdy[u].get(w);
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    const float h = (v[i] - mean) * rstd, dz = act_df<decltype(act)::value>(fmaf(h, ga[i], be[i]), w[i]);
+                    v[i] = fmaf(ga[i] * rstd, dz, fmaf(k3, h, k2));
+                }
+                stv<TX, V>(dx + (f.r + u * f.RP) * p.yr, v);
+            }
+    };
+    if (p.act == A_NONE) rest(std::integral_constant<int, A_NONE>());
+    else if (p.act == A_RELU) rest(std::integral_constant<int, A_RELU>());
+    else if (p.act == A_GELU) rest(std::integral_constant<int, A_GELU>());
+    else rest(std::integral_constant<int, A_SILU>());
+}
+__global__ __launch_bounds__(NT) void gna_params_kernel(const GnaP p) { reduce_params(p, blockIdx.x); }
+
 // ---- host ----------------------------------------------------------------------------------------------
+constexpr int FIT_BLOCKS = 256;
 bool aligned16(const void* p, int64_t a, int64_t b, int esz) { return ((uintptr_t)p % 16) == 0 && (a * esz) % 16 == 0 && (b * esz) % 16 == 0; }
 int esize(int dt) { return dt == POET_F32 ? 4 : 2; }
 
@@ -439,7 +700,7 @@ bool plan(GnaP& p, int V) {
     return true;
 }
 
-int64_t ws_need(const GnaP& p, bool bwd) { return 8 * ((int64_t)p.N * p.G * p.T * p.P + (bwd ? (int64_t)p.N * p.T * p.C : 0)); }
+int64_t ws_need(const GnaP& p, bool bwd) { return 8 * ((int64_t)p.N * p.G * (p.T * p.P + 1) + (bwd ? (int64_t)p.N * p.T * p.C : 0)); }
 
 template <template <typename, typename, int, int> class L, typename TX, typename TY, int V> void by_act(const GnaP& p, int act, hipStream_t s) {
     if (act == A_NONE) L<TX, TY, V, A_NONE>::go(p, s);
@@ -462,10 +723,12 @@ template <template <typename, typename, int, int> class L> bool by_type(const Gn
     return true;
 }
 int blocks(const GnaP& p) { return p.N * p.nslab * p.T; }
+int fold_blocks(const GnaP& p) { return cdiv((int64_t)p.N * p.G, NT / 64); }
 
 template <typename TX, typename TY, int V, int ACT> struct Fwd {
     static void go(const GnaP& p, hipStream_t s) {
         hipLaunchKernelGGL((gna_stats_kernel<TX, V>), dim3(blocks(p)), dim3(NT), 0, s, p);
+        hipLaunchKernelGGL((gna_fold_kernel<false>), dim3(fold_blocks(p)), dim3(NT), 0, s, p);
         hipLaunchKernelGGL((gna_apply_kernel<TX, TY, V, ACT>), dim3(blocks(p)), dim3(NT), 0, s, p);
     }
 };
@@ -473,15 +736,65 @@ template <typename TX, typename TY, int V, int ACT> struct Bwd {
     static void go(const GnaP& p, hipStream_t s) {
         hipLaunchKernelGGL((gna_bwd_stats_kernel<TX, TY, V, ACT>), dim3(blocks(p)), dim3(NT), 0, s, p);
         const int main = p.y ? blocks(p) : 0;
+        if (main) hipLaunchKernelGGL((gna_fold_kernel<true>), dim3(fold_blocks(p)), dim3(NT), 0, s, p);
         if (main + p.tail) hipLaunchKernelGGL((gna_bwd_apply_kernel<TX, TY, V, ACT>), dim3(main + p.tail), dim3(NT), 0, s, p);
     }
 };
+
+// Whether the rows of some groups of an image fit a workgroup (`most` vectors), and how many groups: enough neighbouring ones for 64-byte pieces
+// of a row as long as that leaves two workgroups a CU.  Vectors of V, or single elements for a small image.
+bool fit(GnaP& p, int& V, int esz, int most) {
+    if (p.cpg % V) V = 1;
+    const int lg = p.cpg / V;
+    if ((int64_t)p.HW * lg > most || lg > 64) return false;
+    if ((int64_t)p.N * p.G > (1 << 30)) return false;
+    p.gps = 1;
+    p.T = 1;
+    if ((lg & (lg - 1)) == 0)
+        while (p.G % (2 * p.gps) == 0 && p.gps * lg * V * esz < 64 && 2 * p.gps * lg <= 64 && (int64_t)p.HW * lg * p.gps * 2 <= most &&
+               (int64_t)p.N * (p.G / (2 * p.gps)) >= FIT_BLOCKS)
+            p.gps *= 2;
+    return true;
+}
+template <typename T, int V, int BT, int NR> void go_fit(const GnaP& p, bool bwd, hipStream_t s) {
+    const int blocks = p.N * (p.G / p.gps);
+    if (bwd) {
+        if constexpr (NR <= 6) hipLaunchKernelGGL((gna_fit_bwd_kernel<T, V, BT, NR>), dim3(blocks), dim3(BT), 0, s, p);
+    } else hipLaunchKernelGGL((gna_fit_kernel<T, V, BT, NR>), dim3(blocks), dim3(BT), 0, s, p);
+}
+template <typename T, int V> void fit_size(const GnaP& p, bool bwd, hipStream_t s) {
+    auto holds = [&](int bt, int nr) { return (int64_t)(bt / (p.cpg / V * p.gps)) * nr >= p.HW; };
+    if (holds(256, 2)) go_fit<T, V, 256, 2>(p, bwd, s);
+    else if (holds(256, 6)) go_fit<T, V, 256, 6>(p, bwd, s);
+    else if (holds(1024, 3)) go_fit<T, V, 1024, 3>(p, bwd, s);
+    else if (holds(1024, 6)) go_fit<T, V, 1024, 6>(p, bwd, s);
+    else go_fit<T, V, 1024, 12>(p, bwd, s);
+}
+template <typename T> void fit_vec(const GnaP& p, int V, bool bwd, hipStream_t s) {
+    if (V == 1) fit_size<T, 1>(p, bwd, s);
+    else fit_size<T, 16 / (int)sizeof(T)>(p, bwd, s);
+}
+bool launch_fit(GnaP& p, int xt, int yt, bool wide_ok, bool bwd, hipStream_t s) {
+    if (xt != yt || (xt != POET_F32 && xt != POET_BF16 && xt != POET_F16)) return false;
+    GnaP f = p;
+    int V = !wide_ok ? 1 : xt == POET_F32 ? 4 : 8;
+    // (lanes of a row that do not divide the workgroup leave up to LPR - 1 threads idle: 60 of 64 rows of 3 lanes still hold)
+    const int most = bwd ? 6 * 960 : 12 * 960;
+    if (!fit(f, V, esize(xt), most)) return false;
+    // (16-byte pieces of 128-byte lines, twice: 16 x 4800 x 256 bf16 takes 52 us this way, 45 in chunks)
+    if (bwd && f.gps * (f.cpg / V) * V * esize(xt) < 32 && f.HW * (f.cpg / V) > 3 * 960) return false;
+    if (xt == POET_F32) fit_vec<float>(f, V, bwd, s);
+    else if (xt == POET_BF16) fit_vec<bf16_t>(f, V, bwd, s);
+    else fit_vec<f16_t>(f, V, bwd, s);
+    if (bwd && p.dgamma && p.N > 1) hipLaunchKernelGGL(gna_params_kernel, dim3(cdiv(p.C, 16)), dim3(NT), 0, s, f);
+    return true;
+}
 
 // the part of the checks and of the plan that both directions share; returns POET_OK or an error
 int setup(GnaP& p, const char* what, int N, int HW, int C, int G, int act, int x_dtype, int y_dtype, bool wide_ok, void* ws, int64_t ws_bytes, bool bwd, bool& wide) {
     POET_CHECK(N > 0 && HW > 0 && C > 0 && G > 0 && C % G == 0, POET_ERR_ARG, "%s: bad dims (N %d, HW %d, C %d, G %d)", what, N, HW, C, G);
     POET_CHECK(act >= A_NONE && act <= A_SILU, POET_ERR_ARG, "%s: unknown activation %d", what, act);
-    POET_CHECK(C <= (1 << 20) && HW <= (1 << 30), POET_ERR_UNSUPPORTED, "%s: C > 2^20 or HW > 2^30", what);
+    POET_CHECK(C <= (1 << 20) && HW <= (1 << 30) && (int64_t)N * G < (1ll << 30), POET_ERR_UNSUPPORTED, "%s: C > 2^20, HW > 2^30 or N G > 2^30", what);
     p.N = N; p.HW = HW; p.C = C; p.G = G; p.cpg = C / G;
     wide = wide_ok && plan(p, x_dtype == POET_F32 ? 4 : 8);
     if (!wide) plan(p, 1);
@@ -489,8 +802,10 @@ int setup(GnaP& p, const char* what, int N, int HW, int C, int G, int act, int x
     const int64_t need = ws_need(p, bwd);
     POET_CHECK(ws && ((uintptr_t)ws % 8) == 0 && ws_bytes >= need, POET_ERR_ARG, "%s: workspace of %lld bytes needed (8-byte aligned), %lld given", what,
                (long long)need, (long long)ws_bytes);
+    p.reverse = (int64_t)N * HW * C * (esize(x_dtype) + (bwd ? esize(y_dtype) : 0)) > (200ll << 20);
     p.part = (float2*)ws;
-    p.cpart = p.part + (int64_t)N * G * p.T * p.P;
+    p.folded = p.part + (int64_t)N * G * p.T * p.P;
+    p.cpart = p.folded + (int64_t)N * G;
     return POET_OK;
 }
 
@@ -517,13 +832,18 @@ extern "C" int poet_groupnorm_act_fwd(const void* x, int64_t x_n, int64_t x_r, c
     POET_CHECK(x && gamma && beta && y, POET_ERR_ARG, "groupnorm_act_fwd: null pointer");
     GnaP p = {};
     bool wide = false;
-    const int rc = setup(p, "groupnorm_act_fwd", N, HW, C, G, act, x_dtype, y_dtype,
-                         aligned16(x, x_n, x_r, esize(x_dtype)) && aligned16(y, y_n, y_r, esize(y_dtype)), workspace, workspace_bytes, false, wide);
+    const bool wide_ok = aligned16(x, x_n, x_r, esize(x_dtype)) && aligned16(y, y_n, y_r, esize(y_dtype));
+    const int rc = setup(p, "groupnorm_act_fwd", N, HW, C, G, act, x_dtype, y_dtype, wide_ok, workspace, workspace_bytes, false, wide);
     if (rc != POET_OK) return rc;
     POET_CHECK(!stats || ((uintptr_t)stats % 8) == 0, POET_ERR_ARG, "groupnorm_act_fwd: stats must be 8-byte aligned");
     p.x = x; p.xn = x_n; p.xr = x_r;
     p.y = y; p.yn = y_n; p.yr = y_r;
-    p.gamma = gamma; p.beta = beta; p.stats = stats; p.eps = eps;
+    p.gamma = gamma; p.beta = beta; p.stats = stats; p.eps = eps; p.act = act;
+    if (launch_fit(p, x_dtype, y_dtype, wide_ok, false, (hipStream_t)stream)) {
+        POET_LAUNCH_CHECK();
+        return POET_OK;
+    }
+    if (stats) p.folded = (float2*)stats;
     POET_CHECK(by_type<Fwd>(p, x_dtype, y_dtype, act, wide, (hipStream_t)stream), POET_ERR_UNSUPPORTED, "groupnorm_act_fwd: dtypes %d -> %d", x_dtype, y_dtype);
     POET_LAUNCH_CHECK();
     return POET_OK;
@@ -538,9 +858,8 @@ extern "C" int poet_groupnorm_act_bwd(const void* dy, int64_t dy_n, int64_t dy_r
     POET_CHECK(((uintptr_t)stats % 8) == 0, POET_ERR_ARG, "groupnorm_act_bwd: stats must be 8-byte aligned");
     GnaP p = {};
     bool wide = false;
-    const int rc = setup(p, "groupnorm_act_bwd", N, HW, C, G, act, x_dtype, y_dtype,
-                         aligned16(x, x_n, x_r, esize(x_dtype)) && aligned16(dy, dy_n, dy_r, esize(y_dtype)) && (!dx || aligned16(dx, dx_n, dx_r, esize(x_dtype))),
-                         workspace, workspace_bytes, true, wide);
+    const bool wide_ok = aligned16(x, x_n, x_r, esize(x_dtype)) && aligned16(dy, dy_n, dy_r, esize(y_dtype)) && (!dx || aligned16(dx, dx_n, dx_r, esize(x_dtype)));
+    const int rc = setup(p, "groupnorm_act_bwd", N, HW, C, G, act, x_dtype, y_dtype, wide_ok, workspace, workspace_bytes, true, wide);
     if (rc != POET_OK) return rc;
     p.x = x; p.xn = x_n; p.xr = x_r;
     p.dy = dy; p.dn = dy_n; p.dr = dy_r;
@@ -548,6 +867,11 @@ extern "C" int poet_groupnorm_act_bwd(const void* dy, int64_t dy_n, int64_t dy_r
     p.gamma = gamma; p.beta = beta; p.stats = const_cast<float*>(stats);
     p.dgamma = dgamma; p.dbeta = dbeta; p.accumulate = accumulate;
     p.tail = dgamma ? cdiv(C, 16) : 0;
+    p.act = act;
+    if (launch_fit(p, x_dtype, y_dtype, wide_ok, true, (hipStream_t)stream)) {
+        POET_LAUNCH_CHECK();
+        return POET_OK;
+    }
     POET_CHECK(by_type<Bwd>(p, x_dtype, y_dtype, act, wide, (hipStream_t)stream), POET_ERR_UNSUPPORTED, "groupnorm_act_bwd: dtypes %d, %d", x_dtype, y_dtype);
     POET_LAUNCH_CHECK();
     return POET_OK;

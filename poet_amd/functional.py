@@ -670,7 +670,7 @@ class GroupNormActFn(torch.autograd.Function):
     def forward(ctx, x, w, b, groups, act, eps):
         y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
         stats = torch.empty((x.shape[0], groups, 2), dtype=torch.float32, device=x.device)
-        ops.groupnorm_act_fwd(x, w, b, y, groups, act, stats=stats, eps=eps)
+        ops.groupnorm_act_fwd(x, w, b, y, groups, act, stats, eps)
         ctx.save_for_backward(x, stats, w, b)
         ctx.params, ctx.cfg = (w, b), (groups, act)
         return y
@@ -680,37 +680,39 @@ class GroupNormActFn(torch.autograd.Function):
     def backward(ctx, dy):
         x, stats, w, b = ctx.saved_tensors
         groups, act = ctx.cfg
-        if dy.stride(-1) != 1 and dy.shape[-1] > 1:
+        if not dy.is_contiguous() and dy.stride(-1) != 1 and dy.shape[-1] > 1:
             dy = dy.contiguous()
-        need_x, need_p = ctx.needs_input_grad[0], ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
         dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
-        views = [getattr(p, "_grad_view", None) for p in ctx.params]
-        arena = need_p and all(v is not None for v in views)
-        dw, db = (views if arena else (torch.empty_like(w), torch.empty_like(b))) if need_p else (None, None)
-        ops.groupnorm_act_bwd(dy, x, stats, w, b, groups, act, dx=dx, dgamma=dw, dbeta=db, accumulate=arena)
-        if arena:
-            dw = db = None
-        return dx, dw if ctx.needs_input_grad[1] else None, db if ctx.needs_input_grad[2] else None, None, None, None
+        if not (need_w or need_b):
+            ops.groupnorm_act_bwd(dy, x, stats, w, b, groups, act, dx)
+            return dx, None, None, None, None, None
+        pw, pb = ctx.params
+        dw, db = getattr(pw, "_grad_view", None), getattr(pb, "_grad_view", None)
+        if dw is not None and db is not None:
+            ops.groupnorm_act_bwd(dy, x, stats, w, b, groups, act, dx, dw, db, True)
+            return dx, None, None, None, None, None
+        dw, db = torch.empty((2, w.numel()), dtype=torch.float32, device=x.device).unbind(0)
+        ops.groupnorm_act_bwd(dy, x, stats, w, b, groups, act, dx, dw, db)
+        return dx, dw.view(w.shape) if need_w else None, db.view(b.shape) if need_b else None, None, None, None
 
 
 def group_norm_act(x, weight, bias, groups, act="none", eps=1e-5):
     """act(group_norm(x)) for channels-last x (N, ..., C) in fp32, bf16 or fp16; fp32 weight / bias (C).  act: "none", "relu", "gelu" (erf),
     "silu".  Differentiable once in x, weight and bias; the result has x's type.  Rows may be strided (a slice of a token buffer); x is
     copied only when its channels are not contiguous or its middle dimensions do not merge."""
-    if x.dim() < 2:
+    nd = x.dim()
+    if nd < 2:
         raise ValueError(f"poet_amd: x must be (N, ..., C), got {tuple(x.shape)}")
-    if x.dim() != 3:
-        x3 = x.flatten(1, -2) if x.dim() > 3 else x.unsqueeze(1)
-    else:
-        x3 = x
-    if x3.stride(-1) != 1 and x3.shape[-1] > 1:
+    x3 = x if nd == 3 else x.flatten(1, -2) if nd > 3 else x.unsqueeze(1)
+    if not x3.is_contiguous() and x3.stride(-1) != 1 and x3.shape[-1] > 1:
         x3 = x3.contiguous()
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or bias.requires_grad):
         y = GroupNormActFn.apply(x3, weight, bias, int(groups), act, float(eps))
     else:
         y = torch.empty(x3.shape, dtype=x.dtype, device=x.device)
-        ops.groupnorm_act_fwd(x3, weight, bias, y, int(groups), act, eps=float(eps))
-    return y if x.dim() == 3 else y.view(x.shape)
+        ops.groupnorm_act_fwd(x3, weight, bias, y, int(groups), act, None, float(eps))
+    return y if nd == 3 else y.view(x.shape)
 
 
 # ====================================================================================================

@@ -3,6 +3,7 @@ device buffers and the stream; every computation below is a libpoet_hip.so kerne
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import os
 from typing import Optional, Sequence
 
@@ -530,19 +531,27 @@ def groupnorm_bwd(dy, x, stats, gamma, dx, dgamma, dbeta, N, HW, Cc, G, x_off, x
 ACT = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}          # POET_ACT_*
 
 
-class _on_device:
-    """Launch context of the operators that allocate their own workspace: `with _on_device(t) as stream:` makes t's device current
-    (when it is not) and gives the raw handle of THAT device's current stream."""
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
 
-    def __init__(self, t):
-        self.dev = t.device.index
-        self.guard = None if self.dev == torch.cuda.current_device() else torch.cuda.device(self.dev)
+
+class _on_device:
+    """Launch context of the operators that allocate their own workspace: `with _on_device(device) as stream:` makes the tensors' device
+    current (when it is not) and gives the raw handle of THAT device's current stream."""
+    __slots__ = ("guard", "stream")
+
+    def __init__(self, device):
+        i = device.index
+        if i == torch.cuda.current_device():
+            self.guard, self.stream = None, _STREAM_OVERRIDE[0]
+            if self.stream is None:
+                self.stream = _raw_stream(i)
+        else:                                                     # (a pinned stream is one of the current device)
+            self.guard, self.stream = torch.cuda.device(i), _raw_stream(i)
 
     def __enter__(self):
-        if self.guard is None:
-            return _stream()
-        self.guard.__enter__()
-        return torch.cuda.current_stream().cuda_stream
+        if self.guard is not None:
+            self.guard.__enter__()
+        return self.stream
 
     def __exit__(self, *exc):
         return self.guard.__exit__(*exc) if self.guard is not None else False
@@ -550,94 +559,95 @@ class _on_device:
 
 def _rows3(t: torch.Tensor, name: str, N: int, HW: int, C: int, out: bool = False):
     """(image stride, row stride) of a channels-last (N, HW, C) tensor; an output must not write an element twice."""
-    if t.dim() != 3 or tuple(t.shape) != (N, HW, C):
+    if tuple(t.shape) != (N, HW, C):
         raise ValueError(f"poet_amd: {name} must be ({N}, {HW}, {C}), got {tuple(t.shape)}")
+    if t.is_contiguous():
+        return HW * C, C
     if t.numel() == 0:
         return 0, 0
-    if C > 1 and t.stride(2) != 1:
-        raise ValueError(f"poet_amd: {name} must hold its channels contiguously (stride {t.stride(2)})")
-    n, r = t.stride(0) if N > 1 else 0, t.stride(1) if HW > 1 else 0
+    n, r, c = t.stride()
+    if C > 1 and c != 1:
+        raise ValueError(f"poet_amd: {name} must hold its channels contiguously (stride {c})")
+    n, r = n if N > 1 else 0, r if HW > 1 else 0
     if out and not ((HW == 1 or r >= C) and (N == 1 or n >= (HW - 1) * r + C) or (N == 1 or n >= C) and (HW == 1 or r >= (N - 1) * n + C)):
         raise ValueError(f"poet_amd: rows of the output {name} overlap (strides {n}, {r})")
     return n, r
 
 
-def _chan_params(x, C, G, **params):
+def _gna_args(x, params, G, act):
+    """Checks what both directions share: (device, N, HW, C, activation code)."""
+    if not x.is_cuda:
+        _req(x, "x")
+    if x.dim() != 3:
+        raise ValueError(f"poet_amd: x must be (N, HW, C), got {tuple(x.shape)}")
+    N, HW, C = x.shape
     if G <= 0 or C % G:
         raise ValueError(f"poet_amd: {C} channels do not split into {G} groups")
-    for k, t in params.items():
-        if t is None:
-            continue
-        if t.dtype != torch.float32 or t.numel() != C or not t.is_contiguous():
-            raise ValueError(f"poet_amd: {k} must be a contiguous fp32 tensor of {C} elements")
-        if t.device != x.device:
-            raise ValueError(f"poet_amd: {k} lives on {t.device}, x on {x.device}")
+    dev, f32 = x.device, torch.float32
+    for t in params:
+        if t is not None and not (t.dtype is f32 and t.numel() == C and t.is_contiguous() and t.device == dev):
+            raise ValueError(f"poet_amd: scales, shifts and their gradients are contiguous fp32 tensors of {C} elements on x's device")
+    a = ACT.get(act)
+    if a is None:
+        raise ValueError(f"poet_amd: activation must be one of {sorted(ACT)}, got {act!r}")
+    return dev, N, HW, C, a
 
 
-def _act_code(act):
-    try:
-        return ACT[act]
-    except KeyError:
-        raise ValueError(f"poet_amd: activation must be one of {sorted(ACT)}, got {act!r}") from None
+@functools.lru_cache(maxsize=256)
+def _gna_ws(N, HW, C, G):
+    """Bytes of workspace for these sizes (a function of them alone)."""
+    n = _lib.load().poet_groupnorm_act_workspace(N, HW, C, G)
+    if n < 0:
+        _lib.check(int(n), "poet_groupnorm_act_workspace")
+    return n
 
 
 def groupnorm_act_fwd(x, gamma, beta, y, G, act="none", stats=None, eps=1e-5):
     """y = act(gamma (x - mean) rstd + beta), statistics over the rows and the C / G channels of each (image, group).  x, y (N, HW, C) with
     contiguous channels, any image / row strides (a level's rows of a token buffer); types: equal (fp32, bf16, fp16), or fp32 with bf16.
     stats: optional (N, G, 2) fp32 output (mean, rstd), what groupnorm_act_bwd reads.  y may be x."""
-    lib = _lib.load()
-    _req(x, "x")
-    if x.dim() != 3:
-        raise ValueError(f"poet_amd: x must be (N, HW, C), got {tuple(x.shape)}")
-    N, HW, C = x.shape
-    _chan_params(x, C, G, gamma=gamma, beta=beta)
+    dev, N, HW, C, a = _gna_args(x, (gamma, beta), G, act)
     (xn, xr), (yn, yr) = _rows3(x, "x", N, HW, C), _rows3(y, "y", N, HW, C, out=True)
-    xd, yd, a = dcode(x), dcode(y), _act_code(act)
-    if y.device != x.device or stats is not None and (stats.device != x.device or stats.dtype != torch.float32 or not stats.is_contiguous() or stats.numel() != 2 * N * G):
+    xd, yd = dcode(x), dcode(y)
+    if y.device != dev or stats is not None and not (stats.device == dev and stats.dtype is torch.float32 and stats.is_contiguous() and stats.numel() == 2 * N * G):
         raise ValueError("poet_amd: y and stats must live on x's device, stats as a contiguous fp32 (N, G, 2) tensor")
-    if x.numel() == 0:
+    if N == 0 or HW == 0:
         return y
-    with _on_device(x) as stream:
-        ws = torch.empty(_gna_ws(lib, N, HW, C, G), dtype=torch.uint8, device=x.device)
-        _lib.check(lib.poet_groupnorm_act_fwd(x.data_ptr(), xn, xr, gamma.data_ptr(), beta.data_ptr(), y.data_ptr(), yn, yr, _ptr(stats), N, HW, C, G,
-                                              eps, a, xd, yd, ws.data_ptr(), ws.numel(), stream), "poet_groupnorm_act_fwd")
+    with _on_device(dev) as stream:
+        n = _gna_ws(N, HW, C, G)
+        ws = torch.empty(n, dtype=torch.uint8, device=dev)
+        rc = _lib.load().poet_groupnorm_act_fwd(x.data_ptr(), xn, xr, gamma.data_ptr(), beta.data_ptr(), y.data_ptr(), yn, yr,
+                                                None if stats is None else stats.data_ptr(), N, HW, C, G, eps, a, xd, yd, ws.data_ptr(), n, stream)
+    if rc:
+        _lib.check(rc, "poet_groupnorm_act_fwd")
     return y
-
-
-def _gna_ws(lib, N, HW, C, G):
-    n = lib.poet_groupnorm_act_workspace(N, HW, C, G)
-    if n < 0:
-        _lib.check(int(n), "poet_groupnorm_act_workspace")
-    return n
 
 
 def groupnorm_act_bwd(dy, x, stats, gamma, beta, G, act="none", dx=None, dgamma=None, dbeta=None, accumulate=False):
     """Gradients of groupnorm_act_fwd from its input and stats (z is recomputed): dx in x's type, dgamma / dbeta fp32, overwritten or
     (accumulate) added to.  Any of them may be left out (dgamma and dbeta together)."""
-    lib = _lib.load()
-    _req(x, "x")
-    if x.dim() != 3:
-        raise ValueError(f"poet_amd: x must be (N, HW, C), got {tuple(x.shape)}")
-    N, HW, C = x.shape
-    _chan_params(x, C, G, gamma=gamma, beta=beta, dgamma=dgamma, dbeta=dbeta)
+    dev, N, HW, C, a = _gna_args(x, (gamma, beta, dgamma, dbeta), G, act)
     (xn, xr), (dn, dr) = _rows3(x, "x", N, HW, C), _rows3(dy, "dy", N, HW, C)
     on, orow = (0, 0) if dx is None else _rows3(dx, "dx", N, HW, C, out=True)
-    if dx is not None and (dx.dtype != x.dtype or dx.device != x.device) or dy.device != x.device:
+    if dx is not None and (dx.dtype != x.dtype or dx.device != dev) or dy.device != dev:
         raise ValueError("poet_amd: dx has x's type, and dy, dx live on x's device")
-    if stats.dtype != torch.float32 or stats.device != x.device or not stats.is_contiguous() or stats.numel() != 2 * N * G:
+    if not (stats.dtype is torch.float32 and stats.device == dev and stats.is_contiguous() and stats.numel() == 2 * N * G):
         raise ValueError("poet_amd: stats must be the contiguous fp32 (N, G, 2) tensor of the forward pass")
     if (dgamma is None) != (dbeta is None):
         raise ValueError("poet_amd: dgamma and dbeta go together")
-    xd, yd, a = dcode(x), dcode(dy), _act_code(act)
-    if x.numel() == 0 or dx is None and dgamma is None:
+    xd, yd = dcode(x), dcode(dy)
+    if N == 0 or HW == 0 or dx is None and dgamma is None:
         if dgamma is not None and not accumulate:
             dgamma.zero_(), dbeta.zero_()
         return dx, dgamma, dbeta
-    with _on_device(x) as stream:
-        ws = torch.empty(_gna_ws(lib, N, HW, C, G), dtype=torch.uint8, device=x.device)
-        _lib.check(lib.poet_groupnorm_act_bwd(dy.data_ptr(), dn, dr, x.data_ptr(), xn, xr, stats.data_ptr(), gamma.data_ptr(), beta.data_ptr(),
-                                              _ptr(dx), on, orow, _ptr(dgamma), _ptr(dbeta), int(accumulate), N, HW, C, G, a, xd, yd, ws.data_ptr(),
-                                              ws.numel(), stream), "poet_groupnorm_act_bwd")
+    with _on_device(dev) as stream:
+        n = _gna_ws(N, HW, C, G)
+        ws = torch.empty(n, dtype=torch.uint8, device=dev)
+        rc = _lib.load().poet_groupnorm_act_bwd(dy.data_ptr(), dn, dr, x.data_ptr(), xn, xr, stats.data_ptr(), gamma.data_ptr(), beta.data_ptr(),
+                                                None if dx is None else dx.data_ptr(), on, orow, None if dgamma is None else dgamma.data_ptr(),
+                                                None if dbeta is None else dbeta.data_ptr(), int(accumulate), N, HW, C, G, a, xd, yd, ws.data_ptr(), n, stream)
+    if rc:
+        _lib.check(rc, "poet_groupnorm_act_bwd")
     return dx, dgamma, dbeta
 
 
@@ -1011,7 +1021,7 @@ def orthogonalize(g, out=None, steps=5, coeffs=NS_COEFFS, eps=1e-7):
     dev = gs[0].device
     rows, cols = _muon_dims(shapes)
     ptrs, i64s = C.c_void_p * n, C.c_int64 * n
-    with _on_device(gs[0]) as stream:
+    with _on_device(dev) as stream:
         ws = _muon_ws(lib, rows, cols, n, dev)
         _lib.check(lib.poet_orthogonalize(ptrs(*gp), i64s(*gl), ptrs(*op), i64s(*ol), rows, cols, n, dcode(gs[0]), dcode(os_[0]), steps, cf, eps,
                                           ws.data_ptr(), ws.numel(), stream), "poet_orthogonalize")
@@ -1070,7 +1080,7 @@ class MuonPlan:
             raise ValueError("poet_amd: sqnorm_buf is an fp32 tensor on the parameters' device")
         lib = _lib.load()
         cf = _ns_coeffs(coeffs, steps)
-        with _on_device(self.held[0][0]) as stream:
+        with _on_device(self.device) as stream:
             ws = _muon_ws(lib, self.rows, self.cols, self.n, self.device)
             _lib.check(lib.poet_muon_step(*self.arrays, lr, momentum, int(nesterov), weight_decay, steps, cf, eps, _ptr(sqnorm_buf), max_norm, grad_scale,
                                           ws.data_ptr(), ws.numel(), stream), "poet_muon_step")

@@ -330,3 +330,33 @@ def test_refusals(fn, ops):
     (g,) = torch.autograd.grad(fn.group_norm_act(xg, w, b, 8, act="silu").sum(), xg, create_graph=True)
     with pytest.raises(RuntimeError):                       # differentiable once
         g.sum().backward()
+
+
+def test_more_than_the_cache_holds(ops):
+    """Over 200 MB the second pass runs from the last row to the first: the same results, image by image against float64 on the GPU."""
+    N, HW, C, G = 3, 70001, 256, 32
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.randn(N, HW, C, generator=g, device="cuda") + 1.5
+    dy = torch.randn(N, HW, C, generator=g, device="cuda") * 0.1
+    w, b = torch.rand(C, generator=g, device="cuda") + 0.5, torch.randn(C, generator=g, device="cuda") * 0.1
+    y, dx, st, dw, db = torch.empty_like(x), torch.empty_like(x), torch.empty(N, G, 2, device="cuda"), torch.empty_like(w), torch.empty_like(b)
+    ops.groupnorm_act_fwd(x, w, b, y, G, "silu", stats=st)
+    ops.groupnorm_act_bwd(dy, x, st, w, b, G, "silu", dx=dx, dgamma=dw, dbeta=db)
+    sw, sb = torch.zeros(C, dtype=torch.float64, device="cuda"), torch.zeros(C, dtype=torch.float64, device="cuda")
+    for n in range(N):
+        q = x[n].double().view(HW, G, C // G)
+        m = q.mean((0, 2), keepdim=True)
+        s = ((q - m).square().mean((0, 2), keepdim=True) + 1e-5).sqrt()
+        h = ((q - m) / s).view(HW, C)
+        z = h * w.double() + b.double()
+        sig = torch.sigmoid(z)
+        # (K u per element as above: K = 16 for y; the group's two means sum 560 008 terms, lanes of <= 64 rows and then trees)
+        assert (y[n].double() - z * sig).norm() <= 16 * U * (z * sig).norm()
+        dz = dy[n].double() * sig * (1 + z * (1 - sig))
+        p = (dz * w.double()).view(HW, G, C // G)
+        hg = h.view(HW, G, C // G)
+        want = ((p - p.mean((0, 2), keepdim=True) - hg * (p * hg).mean((0, 2), keepdim=True)) / s).view(HW, C)
+        assert (dx[n].double() - want).norm() <= 32 * U * want.norm()
+        sw += (dz * h).sum(0)
+        sb += dz.sum(0)
+    assert (dw.double() - sw).norm() <= 128 * U * HW ** 0.5 * sw.norm() and (db.double() - sb).norm() <= 128 * U * HW ** 0.5 * sb.norm()
