@@ -51,7 +51,7 @@ struct Rec {
     int nb, part0;                         // workgroups of the norm pass, first partial sum
     int first[GRIDS];                      // first tile of the matrix in each grid
     int W;                                 // narrow matrices: columns of a slab
-    int gvec, ovec;                        // 16-byte accesses of g (and the moment) as one flat range / of the output rows
+    int gvec, rows_vec, ovec;              // vectors of g and the moment as one flat range / of 4 columns of their rows / of the output rows
     float out_scale;                       // muon: the shape's learning-rate factor
 };
 struct Recs { Rec r[CHUNK]; };
@@ -233,30 +233,66 @@ __global__ __launch_bounds__(NT) void muon_pack_kernel(const StageP p) {
     const float gs = grad_scale_of(p.gscale, p.sqnorm, p.max_norm);
     const int t = b - r.first[PACK], tn = r.np >> 6, i0 = (t / tn) << 6, j0 = (t % tn) << 6;
     const int sr = r.turned ? j0 : i0, sc = r.turned ? i0 : j0;       // the tile's place in u
-    const int c = threadIdx.x & 63;
-    for (int q = threadIdx.x >> 6; q < 64; q += 4) {
-        const int row = sr + q, col = sc + c;
-        float v = 0.f;
-        if (row < r.rows && col < r.cols) {
-            if (p.muon) {
-                const int64_t i = (int64_t)row * r.cols + col;
-                const float m = r.mom[i];                              // (already this step's)
-                v = p.nesterov ? fmaf(p.mu, m, p.omu * (((const float*)r.g)[i] * gs)) : m;
-            } else v = ld_any(r.g, row * r.ldg + col, p.g_dtype);
+    const int c4 = (threadIdx.x & 15) * 4, q0 = threadIdx.x >> 4;     // 4 columns of rows q0 + 16 k
+    float v[4][4];
+    if (r.rows_vec && sr + 64 <= r.rows && sc + 64 <= r.cols) {       // a whole tile of aligned rows: 16-byte (8-byte) loads, all in flight
+        if (p.muon) {
+            f32x4_t g[4], m[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int64_t i = (int64_t)(sr + q0 + 16 * k) * r.cols + sc + c4;
+                g[k] = *reinterpret_cast<const f32x4_t*>((const float*)r.g + i);
+                m[k] = *reinterpret_cast<const f32x4_t*>(r.mom + i);                     // (already this step's)
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[k][e] = p.nesterov ? fmaf(p.mu, m[k][e], p.omu * (g[k][e] * gs)) : m[k][e];
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int64_t i = (sr + q0 + 16 * k) * r.ldg + sc + c4;
+                if (p.g_dtype == POET_F32) vec<float, 4>::ld((const float*)r.g + i, v[k]);
+                else if (p.g_dtype == POET_BF16) vec<bf16_t, 4>::ld((const bf16_t*)r.g + i, v[k]);
+                else vec<f16_t, 4>::ld((const f16_t*)r.g + i, v[k]);
+            }
         }
-        tile[q][c] = v;
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int row = sr + q0 + 16 * k, col = sc + c4 + e;
+                v[k][e] = 0.f;
+                if (row < r.rows && col < r.cols) {
+                    if (p.muon) {
+                        const int64_t i = (int64_t)row * r.cols + col;
+                        const float m = r.mom[i];
+                        v[k][e] = p.nesterov ? fmaf(p.mu, m, p.omu * (((const float*)r.g)[i] * gs)) : m;
+                    } else v[k][e] = ld_any(r.g, row * r.ldg + col, p.g_dtype);
+                }
+            }
     }
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) tile[q0 + 16 * k][c4 + e] = v[k][e];
     __syncthreads();
-    const double inv = s_inv;
+    int ex = 0;
+    const float inv = (float)frexp(s_inv, &ex);                       // (a mantissa and an exponent: the factor alone may leave fp32's range)
     _Float16* hi = p.planes + r.x0 + (int64_t)i0 * r.np + j0;
     _Float16* lo = hi + (int64_t)r.dp * r.np;
-    for (int q = threadIdx.x >> 6; q < 64; q += 4) {
-        const float v = (float)((double)(r.turned ? tile[c][q] : tile[q][c]) * inv);
-        const bool in = i0 + q < r.d && j0 + c < r.n;
-        _Float16 h, l;
-        split16(in ? v : 0.f, h, l);
-        hi[(int64_t)q * r.np + c] = h;
-        lo[(int64_t)q * r.np + c] = l;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const int q = q0 + 16 * k;
+        _Float16 h[4], l[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const bool in = i0 + q < r.d && j0 + c4 + e < r.n;        // (zeros behind the matrix, also when the factor is not a number)
+            split16(in ? ldexpf((r.turned ? tile[c4 + e][q] : tile[q][c4 + e]) * inv, ex) : 0.f, h[e], l[e]);
+        }
+        *reinterpret_cast<uint2*>(hi + (int64_t)q * r.np + c4) = *reinterpret_cast<const uint2*>(h);
+        *reinterpret_cast<uint2*>(lo + (int64_t)q * r.np + c4) = *reinterpret_cast<const uint2*>(l);
     }
 }
 
@@ -1532,6 +1568,7 @@ int run_job(const char* what, const Job& j, void* ws, int64_t ws_bytes, void* st
                 r.out_scale = j.out_scale ? j.out_scale[i] : 1.f;
                 const int ge = esize(j.g_dtype), oe = esize(j.o_dtype), gw = 16 / ge;
                 r.gvec = r.ldg == r.cols && (int64_t)r.rows * r.cols % gw == 0 && ((uintptr_t)r.g | (uintptr_t)r.mom) % 16 == 0;
+                r.rows_vec = r.cols % 4 == 0 && r.ldg % 4 == 0 && (uintptr_t)r.g % (4 * ge) == 0 && (uintptr_t)r.mom % 16 == 0;
                 r.ovec = r.cols % 4 == 0 && r.ldo % 4 == 0 && (uintptr_t)r.o % (4 * oe) == 0 && ((uintptr_t)r.p16 | (uintptr_t)r.p16lo) % 8 == 0;
                 blocks += r.nb;
             }
