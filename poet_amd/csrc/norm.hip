@@ -17,6 +17,12 @@ constexpr int LN_MAXIT = 4;   // d <= 1024
 // all-layer maximum of the 1280x960 golden went 4.3e-3 -> 1.17e-2 in the arena pass.)
 template <typename T> struct is_f16 { static constexpr bool value = false; };
 template <> struct is_f16<f16_t> { static constexpr bool value = true; };
+// sum + a b in two roundings: these sums keep the bits they had when their products were packed in pairs (a pair was multiplied and added, a
+// lone product fused, as the vectoriser happened to decide)
+__device__ __forceinline__ float add_mul(float sum, float a, float b) {
+#pragma clang fp contract(off)
+    return sum + a * b;
+}
 // res[e] of 4 consecutive elements: plain load, or bf16 head + fp16 remainder
 template <typename TR>
 __device__ __forceinline__ void ld_stream4(const TR* __restrict__ res, const bf16_t* __restrict__ hi, int64_t at, float* r) {
@@ -83,7 +89,7 @@ __global__ __launch_bounds__(256) void ln_fwd_kernel(const TX* __restrict__ x, c
         const int c = (lane + 64 * it) * 4;
         if (c < d) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) { const float t = v[it][e] - mu; q += t * t; }
+            for (int e = 0; e < 4; ++e) { const float t = v[it][e] - mu; q = add_mul(q, t, t); }
         }
     }
     const float rs = rsqrtf(wave_sum(q) / (float)d + eps);
@@ -162,7 +168,7 @@ __global__ __launch_bounds__(256) void ln_fwd256_kernel(const TX* __restrict__ x
         for (int k = 0; k < R; ++k) {
             q[k] = 0.f;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) { const float t = v[k][e] - mu[k]; q[k] += t * t; }
+            for (int e = 0; e < 4; ++e) { const float t = v[k][e] - mu[k]; q[k] = add_mul(q[k], t, t); }
         }
 #pragma unroll
         for (int k = 0; k < R; ++k) rs[k] = rsqrtf(wave_sum(q[k]) / (float)d + eps);
@@ -307,11 +313,11 @@ __global__ __launch_bounds__(256) void ln_bwd256_kernel(const TR* __restrict__ d
             for (int e = 0; e < 4; ++e) {
                 const float av = ok ? a[r][e] : 0.f;
                 xh[r][e] = (zz[r][e] - mu[r]) * rs[r];
-                ag[e] += av * xh[r][e];
+                ag[e] = add_mul(ag[e], av, xh[r][e]);
                 ab[e] += av;
                 g[r][e] = av * gm[e];
                 c1[r] += g[r][e];
-                c2[r] += g[r][e] * xh[r][e];
+                c2[r] = add_mul(c2[r], g[r][e], xh[r][e]);
             }
         }
 #pragma unroll
@@ -322,7 +328,7 @@ __global__ __launch_bounds__(256) void ln_bwd256_kernel(const TR* __restrict__ d
                 const int64_t row = row0 + r;
                 float o[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) o[e] = rs[r] * (g[r][e] - c1[r] - xh[r][e] * c2[r]);
+                for (int e = 0; e < 4; ++e) o[e] = rs[r] * add_mul(g[r][e] - c1[r], -xh[r][e], c2[r]);
                 vec<TRO, 4>::st(dz + row * d + c, o);
                 if (sep) {
                     if (thresh) {
@@ -401,7 +407,7 @@ __global__ __launch_bounds__(256) void gn_fwd_kernel(const T* __restrict__ x, co
     for (int hw = threadIdx.x; hw < HW; hw += 256) {
         float v[GN_MAXCPG];
         gn_ld<T>(xb + (int64_t)hw * C, v, cpg, vec8);
-        for (int c = 0; c < cpg; ++c) { s += v[c]; q += v[c] * v[c]; }
+        for (int c = 0; c < cpg; ++c) { s += v[c]; q = add_mul(q, v[c], v[c]); }
     }
     const float cnt = (float)HW * (float)cpg;
     const float mu = block_sum(s, sm) / cnt;
@@ -454,7 +460,7 @@ __global__ __launch_bounds__(256) void gn_bwd_kernel(const TY* __restrict__ dy, 
         float d[GN_MAXCPG], v[GN_MAXCPG];
         gn_ld<TY>(dy + ybase + (int64_t)hw * C, d, cpg, vec8);
         gn_ld<T>(x + base + (int64_t)hw * C, v, cpg, vec8);
-        for (int c = 0; c < cpg; ++c) v[c] = rs * (d[c] * gm[c] - m1 - (v[c] - mu) * rs * m2);
+        for (int c = 0; c < cpg; ++c) v[c] = rs * (add_mul(-m1, d[c], gm[c]) - (v[c] - mu) * rs * m2);
         gn_st<T>(dx + base + (int64_t)hw * C, v, cpg, vec8);
     }
 }
@@ -487,13 +493,13 @@ __global__ __launch_bounds__(256) void gn_rows_stats_kernel(const T* __restrict_
 #pragma unroll
         for (int u = 0; u < 4; ++u)
 #pragma unroll
-            for (int c = 0; c < 8; ++c) { s += v[u][c]; q += v[u][c] * v[u][c]; }
+            for (int c = 0; c < 8; ++c) { s += v[u][c]; q = add_mul(q, v[u][c], v[u][c]); }
     }
     for (; r < rend; r += 8) {
         float v[8];
         vec<T, 8>::ld(xb + (int64_t)r * 256, v);
 #pragma unroll
-        for (int c = 0; c < 8; ++c) { s += v[c]; q += v[c] * v[c]; }
+        for (int c = 0; c < 8; ++c) { s += v[c]; q = add_mul(q, v[c], v[c]); }
     }
     red[0][rl][g] = s; red[1][rl][g] = q;
     __syncthreads();
