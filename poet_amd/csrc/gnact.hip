@@ -663,6 +663,7 @@ __global__ __launch_bounds__(NT) void gna_params_kernel(const GnaP p) { reduce_p
 
 // ---- host ----------------------------------------------------------------------------------------------
 constexpr int FIT_BLOCKS = 256;
+constexpr int64_t MAX_THREADS = 1ll << 32;                // of a launch
 bool aligned16(const void* p, int64_t a, int64_t b, int esz) { return ((uintptr_t)p % 16) == 0 && (a * esz) % 16 == 0 && (b * esz) % 16 == 0; }
 int esize(int dt) { return dt == POET_F32 ? 4 : 2; }
 
@@ -747,7 +748,7 @@ bool fit(GnaP& p, int& V, int esz, int most) {
     if (p.cpg % V) V = 1;
     const int lg = p.cpg / V;
     if ((int64_t)p.HW * lg > most || lg > 64) return false;
-    if ((int64_t)p.N * p.G > (1 << 30)) return false;
+    if ((int64_t)p.N * p.G >= MAX_THREADS / 1024) return false;
     p.gps = 1;
     p.T = 1;
     if ((lg & (lg - 1)) == 0)
@@ -794,11 +795,12 @@ bool launch_fit(GnaP& p, int xt, int yt, bool wide_ok, bool bwd, hipStream_t s) 
 int setup(GnaP& p, const char* what, int N, int HW, int C, int G, int act, int x_dtype, int y_dtype, bool wide_ok, void* ws, int64_t ws_bytes, bool bwd, bool& wide) {
     POET_CHECK(N > 0 && HW > 0 && C > 0 && G > 0 && C % G == 0, POET_ERR_ARG, "%s: bad dims (N %d, HW %d, C %d, G %d)", what, N, HW, C, G);
     POET_CHECK(act >= A_NONE && act <= A_SILU, POET_ERR_ARG, "%s: unknown activation %d", what, act);
-    POET_CHECK(C <= (1 << 20) && HW <= (1 << 30) && (int64_t)N * G < (1ll << 30), POET_ERR_UNSUPPORTED, "%s: C > 2^20, HW > 2^30 or N G > 2^30", what);
+    POET_CHECK(C <= (1 << 20) && HW <= (1 << 30), POET_ERR_UNSUPPORTED, "%s: C > 2^20 or HW > 2^30", what);
     p.N = N; p.HW = HW; p.C = C; p.G = G; p.cpg = C / G;
     wide = wide_ok && plan(p, x_dtype == POET_F32 ? 4 : 8);
     if (!wide) plan(p, 1);
-    POET_CHECK((int64_t)N * p.nslab * p.T < (1ll << 30), POET_ERR_UNSUPPORTED, "%s: too many row chunks", what);
+    POET_CHECK((int64_t)N * p.nslab * p.T + cdiv(C, 16) < MAX_THREADS / NT && (int64_t)N * G < MAX_THREADS / 64, POET_ERR_UNSUPPORTED,
+               "%s: N %d, HW %d, C %d, G %d would need 2^32 threads", what, N, HW, C, G);
     const int64_t need = ws_need(p, bwd);
     POET_CHECK(ws && ((uintptr_t)ws % 8) == 0 && ws_bytes >= need, POET_ERR_ARG, "%s: workspace of %lld bytes needed (8-byte aligned), %lld given", what,
                (long long)need, (long long)ws_bytes);

@@ -360,3 +360,41 @@ def test_more_than_the_cache_holds(ops):
         sw += (dz * h).sum(0)
         sb += dz.sum(0)
     assert (dw.double() - sw).norm() <= 128 * U * HW ** 0.5 * sw.norm() and (db.double() - sb).norm() <= 128 * U * HW ** 0.5 * sb.norm()
+
+
+@pytest.mark.parametrize("N,HW,C,G", [(1, 30, 64, 8), (2, 5000, 64, 2)])
+def test_in_place(ops, N, HW, C, G):
+    """y on x; dx on x or on dy: the bits of the call with its own outputs, on both the one-launch and the chunked path."""
+    x, w, b, dy = make(N, HW, C, torch.float32)
+    y, stats = torch.empty_like(x), torch.empty(N, G, 2, device="cuda")
+    ops.groupnorm_act_fwd(x, w, b, y, G, "silu", stats)
+    dx, (dw, db) = torch.empty_like(x), torch.empty(2, C, device="cuda")
+    ops.groupnorm_act_bwd(dy, x, stats, w, b, G, "silu", dx, dw, db)
+    for own in (lambda: (x.clone(), dy.clone(), 0), lambda: (x.clone(), dy.clone(), 1)):
+        xc, dyc, which = own()
+        dw2, db2 = torch.empty(2, C, device="cuda")
+        ops.groupnorm_act_bwd(dyc, xc, stats, w, b, G, "silu", (xc, dyc)[which], dw2, db2)
+        assert torch.equal((xc, dyc)[which], dx) and torch.equal(dw2, dw) and torch.equal(db2, db)
+    xc = x.clone()
+    assert torch.equal(ops.groupnorm_act_fwd(xc, w, b, xc, G, "silu"), y)
+    big = torch.zeros(N, HW + 1, C, device="cuda")
+    big[:, :HW] = x
+    keep = big.clone()
+    with pytest.raises(ValueError):
+        ops.groupnorm_act_fwd(big[:, :HW], w, b, big[:, 1:], G, "silu")
+    with pytest.raises(ValueError):
+        ops.groupnorm_act_bwd(dy, big[:, :HW], stats, w, b, G, "silu", big[:, 1:])
+    with pytest.raises(ValueError):
+        ops.groupnorm_act_bwd(dy, x, stats, w, b, G, "silu", None, dw, dw)
+    assert torch.equal(big, keep)
+
+
+def test_more_images_than_one_launch_of_groups_holds(fn):
+    """2^17 images of 32 groups: past what the one-launch path may start, the chunked one takes over."""
+    x, w, b, dy = make(4, 1, 64, torch.float32)
+    n = (1 << 17) + 4
+    big = x.repeat(n // 4, 1, 1)
+    got = fn.group_norm_act(big, w, b, 32, act="gelu")
+    r = ref(x, w, b, 32, "gelu", 1e-5)
+    check(got[-4:], r["y"], r["tol_y"], "last images")
+    assert torch.equal(got.view(-1, 4, 1, 64), got[:4].expand(n // 4, 4, 1, 64))
