@@ -673,19 +673,19 @@ template <int T, int BK, int SETS, bool LAST> __global__ __launch_bounds__(NT, 2
 // into registers (a lane's 16 bytes of a row are the fragment), all in flight at once, no barrier; the partial tiles meet once in LDS.  Four
 // 256 x 256 matrices: 116 -> 89 us.  Half as much reuse of every operand byte, and 64-byte pieces of rows instead of 128: ten 1024 x 256
 // take 231 us this way against 189 with the staged tiles (and as much with 64 x 64 tiles that load like these).
-template <int F> struct Frags { f16x8_t h[F], l[F]; };
-template <int F> __device__ __forceinline__ void mfma_tile(f32x4_t (&acc)[F][F], const Frags<F>& f, const Frags<F>& s) {
+struct Frags { f16x8_t h[2], l[2]; };
+__device__ __forceinline__ void mfma_tile(f32x4_t (&acc)[2][2], const Frags& f, const Frags& s) {
 #pragma unroll
-    for (int q = 0; q < F * F; ++q) acc[q / F][q % F] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.l[q / F], s.h[q % F], acc[q / F][q % F], 0, 0, 0);
+    for (int q = 0; q < 4; ++q) acc[q >> 1][q & 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.l[q >> 1], s.h[q & 1], acc[q >> 1][q & 1], 0, 0, 0);
 #pragma unroll
-    for (int q = 0; q < F * F; ++q) acc[q / F][q % F] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.h[q / F], s.l[q % F], acc[q / F][q % F], 0, 0, 0);
+    for (int q = 0; q < 4; ++q) acc[q >> 1][q & 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.h[q >> 1], s.l[q & 1], acc[q >> 1][q & 1], 0, 0, 0);
 #pragma unroll
-    for (int q = 0; q < F * F; ++q) acc[q / F][q % F] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.h[q / F], s.h[q % F], acc[q / F][q % F], 0, 0, 0);
+    for (int q = 0; q < 4; ++q) acc[q >> 1][q & 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.h[q >> 1], s.h[q & 1], acc[q >> 1][q & 1], 0, 0, 0);
 }
-// 16 F rows of a plane pair, k .. k + 31 (base: this lane's row and 16-byte piece)
-template <int F> __device__ __forceinline__ void rows_of(Frags<F>& f, const _Float16* base, int ld16, int64_t plane, int k) {
+// 32 rows of a plane pair, k .. k + 31 (base: this lane's row and 16-byte piece)
+__device__ __forceinline__ void rows_of(Frags& f, const _Float16* base, int ld16, int64_t plane, int k) {
 #pragma unroll
-    for (int q = 0; q < F; ++q) {
+    for (int q = 0; q < 2; ++q) {
         f.h[q] = *reinterpret_cast<const f16x8_t*>(base + (q * ld16 + k));
         f.l[q] = *reinterpret_cast<const f16x8_t*>(base + plane + (q * ld16 + k));
     }
@@ -708,7 +708,7 @@ template <int Q> __global__ __launch_bounds__(NT, 2) void muon_sym_split_kernel(
     const _Float16* fb = in + (j0 + m16) * ld + kc * 8;
     const _Float16* sb = in + (i0 + m16) * ld + kc * 8;
     constexpr int AHEAD = Q ? 2 : 4;                                          // (K <= 256: two steps a wave)
-    Frags<2> f[AHEAD], s[AHEAD];
+    Frags f[AHEAD], s[AHEAD];
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u)
         if (const int k = step_k(wave, u); k < K) rows_of(f[u], fb, ld16, plane, k), rows_of(s[u], sb, ld16, plane, k);
@@ -720,7 +720,7 @@ template <int Q> __global__ __launch_bounds__(NT, 2) void muon_sym_split_kernel(
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u) {
             if (step_k(wave, u0 + u) >= K) break;
-            mfma_tile<2>(acc[0], f[u], s[u]);
+            mfma_tile(acc[0], f[u], s[u]);
             if (const int k = step_k(wave, u0 + u + AHEAD); k < K) rows_of(f[u], fb, ld16, plane, k), rows_of(s[u], sb, ld16, plane, k);
         }
     }
@@ -751,7 +751,7 @@ template <bool LAST> __global__ __launch_bounds__(NT, 2) void muon_update_split_
     const int xrow = lane >> 2, xc = lane & 3;
     const _Float16* x = p.planes + (p.flip ? r.x1 : r.x0) + xrow * np + j0 + xc * 8;
     const _Float16* sb = p.planes + r.bm + (i0 + m16) * dp + kc * 8;
-    Frags<2> s[2];
+    Frags s[2];
     u32x4_t xr[2][2][2];                                                      // step, plane, rows k + 16 h + lane / 4
 #pragma unroll
     for (int u = 0; u < 2; ++u)
@@ -778,7 +778,7 @@ template <bool LAST> __global__ __launch_bounds__(NT, 2) void muon_update_split_
             *reinterpret_cast<u32x4_t*>(mine + 32 * ROWB + at) = xr[u][1][h];
         }
         wave_sync();
-        Frags<2> f;
+        Frags f;
 #pragma unroll
         for (int q = 0; q < 2; ++q) {                                         // (bit 3 of rows 8 kc .. 8 kc + 7: kc & 1)
             const char* a = mine + (8 * kc + (m16 >> 2)) * ROWB + ((q ^ (kc & 1)) * 32) + (m16 & 3) * 8;
@@ -790,7 +790,7 @@ template <bool LAST> __global__ __launch_bounds__(NT, 2) void muon_update_split_
             w.hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s_t*)(a + 36 * ROWB));
             f.l[q] = __builtin_bit_cast(f16x8_t, w);
         }
-        mfma_tile<2>(acc[0], f, s[u]);
+        mfma_tile(acc[0], f, s[u]);
     }
     wave_sync();
     f32x4_t v[M::U];
@@ -798,7 +798,7 @@ template <bool LAST> __global__ __launch_bounds__(NT, 2) void muon_update_split_
     leave_update<T, LAST>(p, r, b, i0, j0, part, v);
 }
 
-// ---- narrow matrices: d <= 160 ------------------------------------------------------------------------------------------------
+// ---- narrow matrices: d <= 128 ------------------------------------------------------------------------------------------------
 // The chain above costs 3 dependent launches a step whatever the size, ~6 us each with next to no work in them.  With few rows a
 // workgroup can hold everything that the step needs in LDS: q (dp x dp planes) and a SLAB of X's columns.  X' = q X stays inside a slab; only
 // A = X X^T couples the slabs, through dp x dp partial sums.
@@ -809,7 +809,7 @@ template <bool LAST> __global__ __launch_bounds__(NT, 2) void muon_update_split_
 // diagonal (each fragment read serves two tiles; a diagonal one reads its fragments once), the update in PAIRS of 16-column strips (each
 // fragment of q serves both), rewritten in place by the wave that owns them.  Rows of the LDS images are padded by 16 bytes: an odd number
 // of 16-byte pieces, so that the 16 rows of a fragment read start in different banks.
-constexpr int NW_T = 512, NWAVES = NW_T / 64, MAX_SLABS = 8, MAX_D = 5, MAX_SLAB_D = 2;
+constexpr int NW_T = 512, NWAVES = NW_T / 64, MAX_SLABS = 8, MAX_D = 4, MAX_SLAB_D = 2;
 template <int D> struct Narrow {
     static constexpr int DP = 32 * D, NM = D * (D + 1) / 2;
     static constexpr int PARTS = D == 1 ? 8 : D == 2 ? 2 : 1;             // few macro tiles: the columns in PARTS ranges, so that all waves have some
@@ -818,7 +818,7 @@ template <int D> struct Narrow {
     static constexpr int SCRATCH = PARTS > 1 ? ITEMS * 4096 : 0;
     static constexpr int REGION = 2 * APLANE > SCRATCH ? 2 * APLANE : SCRATCH;      // A / q planes, or partial tiles
 };
-constexpr int W_MAX[MAX_D + 1] = {0, 896, 512, 288, 160, 64};       // columns that leave room for REGION in 160 KB
+constexpr int W_MAX[MAX_D + 1] = {0, 896, 512, 288, 160};       // columns that leave room for REGION in 160 KB
 struct NarrowP {
     StageP s;
     int mode, k, steps;                              // N_*; this launch's step
@@ -1375,6 +1375,7 @@ bool ranges(const double* coeffs, int steps, Steps& S) {
     double xb = 1.0001;
     for (int k = 0; k < steps; ++k) {
         const double a = coeffs[3 * k], b = coeffs[3 * k + 1], c = coeffs[3 * k + 2];
+        if (!isfinite(a + b + c)) return false;
         double qb = fabs(a), nx = 0.0;                       // (the padding and A = 0 count: q(0) = a)
         for (int i = 0; i <= 2000; ++i) {
             const double x = xb * i / 2000.0, q = a + b * x * x + c * x * x * x * x;
@@ -1577,8 +1578,7 @@ int run_job(const char* what, const Job& j, void* ws, int64_t ws_bytes, void* st
             else if (group == 1) narrow_single<1>(narrow, recs, C.count, C.maxW, st);
             else if (group == 2) narrow_single<2>(narrow, recs, C.count, C.maxW, st);
             else if (group == 3) narrow_single<3>(narrow, recs, C.count, C.maxW, st);
-            else if (group == 4) narrow_single<4>(narrow, recs, C.count, C.maxW, st);
-            else narrow_single<5>(narrow, recs, C.count, C.maxW, st);
+            else narrow_single<4>(narrow, recs, C.count, C.maxW, st);
             planes += C.plane_elems;
             parts += C.parts;
             for (int k = 0; k < GRIDS; ++k) tiles[k] += C.tiles[k];

@@ -574,6 +574,23 @@ def _rows3(t: torch.Tensor, name: str, N: int, HW: int, C: int, out: bool = Fals
     return n, r
 
 
+def _apart(a, an, ar, b, bn, br, N, HW, C, name):
+    """Refuses a (N, HW, C) output `b` that shares memory with the input `a` in any way but being the same tensor."""
+    ea, eb, a0, b0 = a.element_size(), b.element_size(), a.data_ptr(), b.data_ptr()
+    la, lb = (HW - 1) * ar + C, (HW - 1) * br + C                 # an image's extent
+    if b0 >= a0 + ((N - 1) * an + la) * ea or a0 >= b0 + ((N - 1) * bn + lb) * eb:
+        return
+    if a.dtype == b.dtype and a0 == b0 and (N == 1 or an == bn) and (HW == 1 or ar == br):
+        return
+    if ea == eb:
+        d = (b0 - a0) // ea
+        if N > 1 and an == bn and an > 0 and d % an >= la and d % an + lb <= an:          # other rows of the same images
+            return
+        if HW > 1 and ar == br and ar > 0 and (N == 1 or an == bn and an % ar == 0) and d % ar >= C and d % ar + C <= ar:      # other columns
+            return
+    raise ValueError(f"poet_amd: {name} overlaps an input that it is not")
+
+
 def _gna_args(x, params, G, act):
     """Checks what both directions share: (device, N, HW, C, activation code)."""
     if not x.is_cuda:
@@ -613,6 +630,7 @@ def groupnorm_act_fwd(x, gamma, beta, y, G, act="none", stats=None, eps=1e-5):
         raise ValueError("poet_amd: y and stats must live on x's device, stats as a contiguous fp32 (N, G, 2) tensor")
     if N == 0 or HW == 0:
         return y
+    _apart(x, xn, xr, y, yn, yr, N, HW, C, "y")
     with _on_device(dev) as stream:
         n = _gna_ws(N, HW, C, G)
         ws = torch.empty(n, dtype=torch.uint8, device=dev)
@@ -625,7 +643,7 @@ def groupnorm_act_fwd(x, gamma, beta, y, G, act="none", stats=None, eps=1e-5):
 
 def groupnorm_act_bwd(dy, x, stats, gamma, beta, G, act="none", dx=None, dgamma=None, dbeta=None, accumulate=False):
     """Gradients of groupnorm_act_fwd from its input and stats (z is recomputed): dx in x's type, dgamma / dbeta fp32, overwritten or
-    (accumulate) added to.  Any of them may be left out (dgamma and dbeta together)."""
+    (accumulate) added to.  Any of them may be left out (dgamma and dbeta together); dx may be x or dy."""
     dev, N, HW, C, a = _gna_args(x, (gamma, beta, dgamma, dbeta), G, act)
     (xn, xr), (dn, dr) = _rows3(x, "x", N, HW, C), _rows3(dy, "dy", N, HW, C)
     on, orow = (0, 0) if dx is None else _rows3(dx, "dx", N, HW, C, out=True)
@@ -633,13 +651,16 @@ def groupnorm_act_bwd(dy, x, stats, gamma, beta, G, act="none", dx=None, dgamma=
         raise ValueError("poet_amd: dx has x's type, and dy, dx live on x's device")
     if not (stats.dtype is torch.float32 and stats.device == dev and stats.is_contiguous() and stats.numel() == 2 * N * G):
         raise ValueError("poet_amd: stats must be the contiguous fp32 (N, G, 2) tensor of the forward pass")
-    if (dgamma is None) != (dbeta is None):
-        raise ValueError("poet_amd: dgamma and dbeta go together")
+    if (dgamma is None) != (dbeta is None) or dgamma is not None and C > 0 and dgamma.data_ptr() == dbeta.data_ptr():
+        raise ValueError("poet_amd: dgamma and dbeta go together, and are two tensors")
     xd, yd = dcode(x), dcode(dy)
     if N == 0 or HW == 0 or dx is None and dgamma is None:
         if dgamma is not None and not accumulate:
             dgamma.zero_(), dbeta.zero_()
         return dx, dgamma, dbeta
+    if dx is not None:
+        _apart(x, xn, xr, dx, on, orow, N, HW, C, "dx")
+        _apart(dy, dn, dr, dx, on, orow, N, HW, C, "dx")
     with _on_device(dev) as stream:
         n = _gna_ws(N, HW, C, G)
         ws = torch.empty(n, dtype=torch.uint8, device=dev)
@@ -956,6 +977,19 @@ def _muon_dims(shapes):
     return rows, cols
 
 
+def _clash(items):
+    """Whether a written matrix shares bytes with another one: items (start, rows, row stride, row width, written, index), in bytes; items of one
+    index may overlap.  Matrices of one row stride that lie side by side in it do not."""
+    active = []
+    for s, rows, ld, w, wr, i in sorted(items):
+        active = [a for a in active if a[1] > s]
+        for s2, _, ld2, w2, wr2, i2 in active:
+            if (wr or wr2) and i != i2 and not (ld == ld2 and (s - s2) % ld >= w2 and (s - s2) % ld + w <= ld):
+                return True
+        active.append((s, s + (rows - 1) * ld + w, ld, w, wr, i))
+    return False
+
+
 def _muon_ws(lib, rows, cols, n, device):
     need = lib.poet_muon_workspace(rows, cols, n)
     if need < 0:
@@ -967,7 +1001,8 @@ def orthogonalize(g, out=None, steps=5, coeffs=NS_COEFFS, eps=1e-7):
     """Newton-Schulz orthogonalisation: X = g / (|g|_F + eps), then `steps` times X <- (a I + b X X^T + c (X X^T)^2) X (from the shorter
     side).  g: a tensor (..., m, n), or a list of 2-D tensors of any shapes, one type (fp32, bf16, fp16) and device; the result has g's
     form and type (or goes to `out`, which may be g).  coeffs: (a, b, c), or one such triple per step.  Products carry 22-bit operands
-    and fp32 sums.  All matrices of a call run in one chain of 2 + 3 steps launches, so a list costs little more than its longest chain."""
+    and fp32 sums.  The matrices of a call are worked on together (the narrow ones, those with up to 256 rows or columns and the others
+    each in one chain of launches), so a list costs little more than its longest chains; a matrix's result does not depend on the list."""
     single = torch.is_tensor(g)
     if single and g.dim() < 2:
         raise ValueError(f"poet_amd: g must be (..., m, n), got {tuple(g.shape)}")
@@ -975,16 +1010,18 @@ def orthogonalize(g, out=None, steps=5, coeffs=NS_COEFFS, eps=1e-7):
         g = list(g)
         if any(t.dim() != 2 for t in g):
             raise ValueError("poet_amd: the tensors of a list are 2-D")
-    if out is None:
+    given = out is not None
+    if not given:
         out = torch.empty(g.shape, dtype=g.dtype, device=g.device) if single else [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in g]
     gs = [g] if single else g
     os_ = [out] if single else list(out)
     if len(gs) != len(os_) or any(a.shape != b.shape for a, b in zip(gs, os_)):
         raise ValueError("poet_amd: out must have g's shapes")
-    for t in (*gs, *os_):
-        _req(t, "g")
-        if t.device != gs[0].device or t.dtype != (gs[0] if any(t is v for v in gs) else os_[0]).dtype:
-            raise ValueError("poet_amd: the matrices of a call share one device and one type")
+    for ts in (gs, os_):
+        for t in ts:
+            _req(t, "g")
+            if t.device != gs[0].device or t.dtype != ts[0].dtype:
+                raise ValueError("poet_amd: the matrices of a call share one device, inputs one type and outputs one")
     if not 1 <= steps <= 16:
         raise ValueError(f"poet_amd: 1 .. 16 steps, got {steps}")
     cf = _ns_coeffs(coeffs, steps)
@@ -1003,8 +1040,6 @@ def orthogonalize(g, out=None, steps=5, coeffs=NS_COEFFS, eps=1e-7):
         if b.dim() > 3:
             b = b.view(-1, m, n)
         k = a.shape[0] if a.dim() == 3 else 1
-        if k > 1 and b.stride(0) < (m - 1) * max(b.stride(-2), n) + n:
-            raise ValueError("poet_amd: the matrices of the output overlap")
         a0, b0, sa, sb = a.data_ptr(), b.data_ptr(), (a.stride(0) * a.element_size() if k > 1 else 0), (b.stride(0) * b.element_size() if k > 1 else 0)
         keep.append(a)
         gp += [a0 + i * sa for i in range(k)]
@@ -1015,8 +1050,10 @@ def orthogonalize(g, out=None, steps=5, coeffs=NS_COEFFS, eps=1e-7):
     n = len(gp)
     if n == 0:
         return out
-    if len(set(op)) != n:
-        raise ValueError("poet_amd: the same output twice in one call")
+    if given:
+        sizes = ((gp, gl, gs[0].element_size(), False), (op, ol, os_[0].element_size(), True))
+        if _clash([(p[i], shapes[i][0], ld[i] * e, shapes[i][1] * e, wr, i) for p, ld, e, wr in sizes for i in range(n)]):
+            raise ValueError("poet_amd: an output overlaps another output, or another matrix's input")
     lib = _lib.load()
     dev = gs[0].device
     rows, cols = _muon_dims(shapes)
@@ -1060,8 +1097,10 @@ class MuonPlan:
                         raise ValueError("poet_amd: bf16 images are contiguous bf16 tensors of the parameter's size, lr_scale fp32 words, on its device")
         self.rows, self.cols = _muon_dims([p.shape for p in params])
         pp, mp = [p.data_ptr() for p in params], [m.data_ptr() for m in moments]
-        if len(set(pp + mp)) != 2 * n:
-            raise ValueError("poet_amd: the same parameter or moment twice in one call")
+        held = [(t, wr) for l, wr in ((params, True), (moments, True), (p_bf16, True), (p_bf16_lo, True), (grads, False), (lr_scale, False)) for t in l or ()]
+        size = [t.numel() * t.element_size() for t, _ in held]
+        if _clash([(t.data_ptr(), 1, b, b, wr, i) for i, ((t, wr), b) in enumerate(zip(held, size))]):
+            raise ValueError("poet_amd: a parameter, moment or bf16 image overlaps another tensor of the call")
         ptrs = C.c_void_p * n
         lst = lambda l: None if l is None else ptrs(*[t.data_ptr() for t in l])        # noqa: E731
         fn = MUON_SCALES[scale]

@@ -289,3 +289,37 @@ def test_refusals(ops):
             call()
     assert torch.equal(p, g) and (m == 0).all()
     ops.muon_step([], [], [], lr=0.1)
+
+
+def test_outputs_side_by_side_and_outputs_that_overlap(ops):
+    """Views of one buffer as outputs: columns of the same rows, interleaved batches, and what would write an element twice or into another
+    matrix's input, refused before anything runs."""
+    buf = torch.zeros(40, 96, device="cuda")
+    gs = [matrix(40, 32, i).cuda() for i in range(3)]
+    ops.orthogonalize(gs, out=[buf[:, 32 * i:32 * (i + 1)] for i in range(3)])
+    for i, g in enumerate(gs):
+        assert torch.equal(buf[:, 32 * i:32 * (i + 1)], ops.orthogonalize(g))
+    src = buf.clone()
+    cols = [src[:, :32], src[:, 32:64], src[:, 64:]]
+    want = [ops.orthogonalize(c) for c in cols]
+    ops.orthogonalize(cols, out=cols)                                            # in place, on column views
+    assert all(torch.equal(c, w) for c, w in zip(cols, want))
+    g3 = torch.stack(gs)
+    out3 = torch.zeros(40, 3, 32, device="cuda").transpose(0, 1)                 # the batch between rows and columns
+    ops.orthogonalize(g3, out=out3)
+    assert torch.equal(out3, ops.orthogonalize(g3))
+    flat = torch.randn(5 * 40 * 32, device="cuda")
+    a, b, c = flat[:1280].view(40, 32), flat[1280:2560].view(40, 32), flat[2000:3280].view(40, 32)
+    keep = flat.clone()
+    wide, half = torch.zeros(40, 32, device="cuda"), [g.bfloat16() for g in gs[:2]]
+    for call in (lambda: ops.orthogonalize([a, gs[0]], out=[b, c]), lambda: ops.orthogonalize([a, b], out=[b, torch.empty_like(a)]),
+                 lambda: ops.orthogonalize([a, b], out=[torch.empty_like(a), a]), lambda: ops.orthogonalize(torch.stack([a, b]), out=b.expand(2, 40, 32)),
+                 lambda: ops.orthogonalize(half, out=[wide, half[1]]), lambda: ops.orthogonalize(half, out=[half[0], wide]),
+                 lambda: ops.muon_step([a], [a], [torch.zeros_like(a)], lr=0.1), lambda: ops.muon_step([a], [b], [b], lr=0.1),
+                 lambda: ops.muon_step([a, b], [gs[0], gs[1]], [torch.zeros_like(a), c], lr=0.1),
+                 lambda: ops.muon_step([a], [b], [gs[0]], lr=0.1, p_bf16=[flat.view(torch.bfloat16)[100:1380]])):
+        with pytest.raises(ValueError):
+            call()
+    assert torch.equal(flat, keep) and (wide == 0).all()
+    ops.muon_step([a, b], [gs[0], gs[0]], [torch.zeros_like(a), torch.zeros_like(a)], lr=0.1)      # (one gradient for two matrices is fine)
+    assert not torch.equal(flat, keep)
