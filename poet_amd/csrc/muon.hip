@@ -21,6 +21,9 @@
 
 #include <math.h>
 
+#include <algorithm>
+#include <new>
+
 namespace poet {
 
 namespace {
@@ -313,24 +316,28 @@ template <int ROWB> __device__ __forceinline__ int swz_col(int krow) {
     else return ((krow >> 1) & 1) | (((krow >> 3) & 1) << 1);
 }
 
+// Threads of a workgroup with a T x T tile, and its waves' shares of it: 64: 4 waves of 32 x 32; 128: 8 waves of 32 x 64 (first x second), so that
+// two waves of a SIMD alternate between LDS reads and matrix instructions (2048 x 2048: 850 -> 835 us).
+constexpr int threads_of(int T) { return T == 128 ? 512 : 256; }
 // SETS > 1: stage k of BK goes to accumulator set k % SETS, so that the sum has the order of the split kernels below.
-// acc[set][f][s][r] += sum_k first[f 16 + 4 (lane / 16) + r][k] second[s 16 + lane % 16][k] over a T x T tile, 4 waves of T/2 x T/2.
+// acc[set][f][s][r] += sum_k first[f 16 + 4 (lane / 16) + r][k] second[s 16 + lane % 16][k] over a T x T tile.
 // second: rows of K contiguous elements.  first: the same, or (KM) stored [k][column].  K % BK == 0; every row / column read exists
 // (planes are padded to whole tiles).
 template <int T, int BK, bool KM, int SETS> struct Core {
-    static constexpr int ROWB = BK * 2, CPR = BK / 8, F = T / 32, PLANE = T * BK * 2, STAGE = 4 * PLANE;
-    static constexpr int NL = PLANE / 16 / NT;                                            // 16-byte loads per thread and plane
+    static constexpr int N = threads_of(T), F = 2, S = T / 32, WF = T / 32;                // a wave's 16 x 16 tiles; waves along the first operand
+    static constexpr int ROWB = BK * 2, CPR = BK / 8, PLANE = T * BK * 2, STAGE = 4 * PLANE;
+    static constexpr int NL = PLANE / 16 / N;                                            // 16-byte loads per thread and plane
     static constexpr int COLB = T * 2, CPC = T / 8;
     static constexpr int AHEAD = T == 64 && SETS == 1 ? 4 : 2, UNROLL = SETS > AHEAD ? SETS : AHEAD;      // stages in registers on their way to LDS
     static __device__ __forceinline__ void run(const _Float16* fh, const _Float16* fl, int64_t ldf, const _Float16* sh, const _Float16* sl, int64_t lds_,
-                                               int K, char* smem, f32x4_t (&acc)[SETS][F][F]) {
-        const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wf = (wave >> 1) * (T / 2), ws = (wave & 1) * (T / 2);
+                                               int K, char* smem, f32x4_t (&acc)[SETS][F][S]) {
+        const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wf = wave % WF * 32, ws = wave / WF * (T / 2);
         const int m16 = lane & 15, kc = lane >> 4;
         int64_t go[NL], so[NL];
         int lo_f[NL], lo_s[NL];
 #pragma unroll
         for (int q = 0; q < NL; ++q) {
-            const int idx = q * NT + tid, row = idx / CPR, c = idx % CPR;
+            const int idx = q * N + tid, row = idx / CPR, c = idx % CPR;
             so[q] = row * lds_ + c * 8;
             lo_s[q] = row * ROWB + ((c ^ swz_row<ROWB>(row)) & (CPR - 1)) * 16;
             if constexpr (KM) {
@@ -378,7 +385,7 @@ template <int T, int BK, bool KM, int SETS> struct Core {
             }
         }
     }
-    static __device__ __forceinline__ void stage(const char* st, f32x4_t (&acc)[F][F], int wf, int ws, int m16, int kc) {
+    static __device__ __forceinline__ void stage(const char* st, f32x4_t (&acc)[F][S], int wf, int ws, int m16, int kc) {
 #pragma unroll
         for (int h = 0; h < BK / 32; ++h) {
             f16x8_t fhv[F], flv[F];
@@ -402,7 +409,7 @@ template <int T, int BK, bool KM, int SETS> struct Core {
                 }
             }
 #pragma unroll
-            for (int s = 0; s < F; ++s) {
+            for (int s = 0; s < S; ++s) {
                 const int row = ws + s * 16 + m16, a = row * ROWB + (((h * 4 + kc) ^ swz_row<ROWB>(row)) & (CPR - 1)) * 16;
                 const f16x8_t shv = *reinterpret_cast<const f16x8_t*>(st + 2 * PLANE + a), slv = *reinterpret_cast<const f16x8_t*>(st + 3 * PLANE + a);
 #pragma unroll
@@ -431,18 +438,19 @@ __device__ __forceinline__ void store_some(_Float16* o, _Float16* ol, const uint
             reinterpret_cast<uint16_t*>(ol)[e] = (uint16_t)((e & 2 ? lo.y : lo.x) >> (e & 1) * 16);
         }
 }
-// A T x T fp32 tile in LDS, 16-byte pieces XORed so that rows and columns of 4 read without conflicts.  A workgroup's threads hold it as
-// pieces: piece u of a thread is row u (NT / P) + threadIdx / P, columns 4 (threadIdx % P) .. + 3, P = T / 4.
+// A T x T fp32 tile in LDS, 16-byte pieces XORed so that rows and columns of 4 read without conflicts.  A workgroup's N threads hold it as
+// pieces: piece u of a thread is row u (N / P) + threadIdx / P, columns 4 (threadIdx % P) .. + 3, P = T / 4.
 template <int T> struct Meet {
-    static constexpr int P = T / 4, U = T * P / NT, F = T / 16;
+    static constexpr int N = threads_of(T), P = T / 4, U = T * P / N, F = T / 16;
     static __device__ __forceinline__ int at(int i, int piece) { return i * T + ((piece ^ (i >> 2)) & (P - 1)) * 4; }
-    static __device__ __forceinline__ int row(int u) { return u * (NT / P) + threadIdx.x / P; }
+    static __device__ __forceinline__ int row(int u) { return u * (N / P) + threadIdx.x / P; }
     static __device__ __forceinline__ int col() { return (threadIdx.x % P) * 4; }
-    // the tile in the accumulators of four waves of T / 2 x T / 2 -> this thread's pieces
-    static __device__ __forceinline__ void share(float* part, const f32x4_t (&acc)[T / 32][T / 32], int wf, int ws, int m16, int kc, f32x4_t (&v)[U]) {
+    // the tile in the accumulators of the waves (Core's shares) -> this thread's pieces
+    static __device__ __forceinline__ void share(float* part, const f32x4_t (&acc)[2][T / 32], f32x4_t (&v)[U]) {
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m16 = lane & 15, kc = lane >> 4, wf = wave % (T / 32) * 32, ws = wave / (T / 32) * (T / 2);
         __syncthreads();                                                      // (the last stage's operands have been read)
 #pragma unroll
-        for (int f = 0; f < T / 32; ++f)
+        for (int f = 0; f < 2; ++f)
 #pragma unroll
             for (int s = 0; s < T / 32; ++s) *reinterpret_cast<f32x4_t*>(part + at(ws + s * 16 + m16, ((wf + f * 16) >> 2) + kc)) = acc[f][s];
         __syncthreads();
@@ -605,19 +613,19 @@ __device__ __forceinline__ void rectangle(int t, int tn, int& bi, int& bj) {  //
     bi = __builtin_amdgcn_readfirstlane(divide(t, tn, j));
     bj = __builtin_amdgcn_readfirstlane(j);
 }
-template <int SETS, int F> __device__ __forceinline__ void zero(f32x4_t (&acc)[SETS][F][F]) {
+template <int SETS, int S> __device__ __forceinline__ void zero(f32x4_t (&acc)[SETS][2][S]) {
 #pragma unroll
-    for (int q = 0; q < SETS * F * F; ++q) acc[q / (F * F)][q / F % F][q % F] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    for (int q = 0; q < SETS * 2 * S; ++q) acc[q / (2 * S)][q / S % 2][q % S] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 }
-template <int SETS, int F> __device__ __forceinline__ void fold_sets(f32x4_t (&acc)[SETS][F][F]) {
+template <int SETS, int S> __device__ __forceinline__ void fold_sets(f32x4_t (&acc)[SETS][2][S]) {
     if constexpr (SETS == 4) {
 #pragma unroll
-        for (int q = 0; q < F * F; ++q) acc[0][q / F][q % F] = (acc[0][q / F][q % F] + acc[1][q / F][q % F]) + (acc[2][q / F][q % F] + acc[3][q / F][q % F]);
+        for (int q = 0; q < 2 * S; ++q) acc[0][q / S][q % S] = (acc[0][q / S][q % S] + acc[1][q / S][q % S]) + (acc[2][q / S][q % S] + acc[3][q / S][q % S]);
     }
 }
 
 // A = X X^T (Q = 0), or q = a I + b A + c A A (Q = 1): tiles on and below the diagonal
-template <int T, int BK, int SETS, int Q> __global__ __launch_bounds__(NT, 2) void muon_sym_kernel(const StageP p) {
+template <int T, int BK, int SETS, int Q> __global__ __launch_bounds__(threads_of(T), threads_of(T) / 128) void muon_sym_kernel(const StageP p) {
     typedef Core<T, BK, false, SETS> C;
     typedef Meet<T> M;
     static_assert(2 * C::STAGE >= T * T * 4, "the tile fits the stages' LDS");
@@ -629,21 +637,20 @@ template <int T, int BK, int SETS, int Q> __global__ __launch_bounds__(NT, 2) vo
     const int64_t ld = Q ? dp : r.np, plane = (int64_t)dp * ld;
     const _Float16* in = p.planes + (Q ? r.am : p.flip ? r.x1 : r.x0);
     const int K = Q ? (r.d + BK - 1) / BK * BK : (r.n + BK - 1) / BK * BK;
-    f32x4_t acc[SETS][C::F][C::F];
+    f32x4_t acc[SETS][C::F][C::S];
     zero(acc);
     uint2 ah[M::U], al[M::U];
     if constexpr (Q && T == 64) a_pieces<T>(p, r, i0, j0, ah, al);            // (ahead of the product: 16 registers)
     C::run(in + j0 * ld, in + plane + j0 * ld, ld, in + i0 * ld, in + plane + i0 * ld, ld, K, smem, acc);
     if constexpr (Q && T != 64) a_pieces<T>(p, r, i0, j0, ah, al);
     fold_sets(acc);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     f32x4_t v[M::U];
-    M::share(reinterpret_cast<float*>(smem), acc[0], (wave >> 1) * (T / 2), (wave & 1) * (T / 2), lane & 15, lane >> 4, v);
+    M::share(reinterpret_cast<float*>(smem), acc[0], v);
     leave_sym<T, Q>(p, r, i0, j0, reinterpret_cast<float*>(smem), v, ah, al);
 }
 
 // X' = q X; the last step leaves the planes: the output matrix, or the weight update
-template <int T, int BK, int SETS, bool LAST> __global__ __launch_bounds__(NT, 2) void muon_update_kernel(const StageP p) {
+template <int T, int BK, int SETS, bool LAST> __global__ __launch_bounds__(threads_of(T), threads_of(T) / 128) void muon_update_kernel(const StageP p) {
     typedef Core<T, BK, true, SETS> C;
     typedef Meet<T> M;
     __shared__ __attribute__((aligned(16))) char smem[2 * C::STAGE];
@@ -656,13 +663,12 @@ template <int T, int BK, int SETS, bool LAST> __global__ __launch_bounds__(NT, 2
     const int64_t np = r.np, plane = (int64_t)dp * np, sq = (int64_t)dp * dp;
     const _Float16* x = p.planes + (p.flip ? r.x1 : r.x0);
     const _Float16* qm = p.planes + r.bm;
-    f32x4_t acc[SETS][C::F][C::F];
+    f32x4_t acc[SETS][C::F][C::S];
     zero(acc);
     C::run(x + j0, x + plane + j0, np, qm + (int64_t)i0 * dp, qm + sq + (int64_t)i0 * dp, dp, (r.d + BK - 1) / BK * BK, smem, acc);
     fold_sets(acc);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     f32x4_t v[M::U];
-    M::share(reinterpret_cast<float*>(smem), acc[0], (wave >> 1) * (T / 2), (wave & 1) * (T / 2), lane & 15, lane >> 4, v);
+    M::share(reinterpret_cast<float*>(smem), acc[0], v);
     leave_update<T, LAST>(p, r, b, i0, j0, reinterpret_cast<float*>(smem), v);
 }
 
@@ -1302,9 +1308,9 @@ Choice tiles_of(const int* rows, const int* cols, int n) {
     return {{sym >= 512 ? 128 : 64, upd >= 256 ? 128 : 64}, {ssym > 256 ? 64 : 32, supd > 512 ? 64 : 32}};
 }
 
-// the records of one group among matrices [first, n) (at most `most` of them): shape-dependent members into rec (when given), sizes into L;
-// returns the index behind the last one taken, or -1: too large
-int layout(const int* rows, const int* cols, int first, int n, int group, const Choice& choice, int most, Layout& L, Rec* rec) {
+// the records of one group among matrices [first, n) -- or among order[first .. n) -- (at most `most` of them): shape-dependent members into rec
+// (when given), sizes into L; returns the index behind the last one taken, or -1: too large
+int layout(const int* rows, const int* cols, const int* order, int first, int n, int group, const Choice& choice, int most, Layout& L, Rec* rec) {
     const Tiles T = group == SMALL ? choice.small : choice.large;
     const int P = T.sym == 128 || T.upd == 128 ? 128 : 64;   // planes hold whole tiles of every kind
     int64_t planes = 0, parts = 0, tiles[GRIDS] = {0, 0, 0};
@@ -1312,12 +1318,13 @@ int layout(const int* rows, const int* cols, int first, int n, int group, const 
     L.maxW = 0;
     for (; i < n && count < most; ++i) {
         Rec r = {};
-        if (group_of(rows[i], cols[i], r.W) != group) continue;
-        r.rows = rows[i];
-        r.cols = cols[i];
-        r.turned = rows[i] > cols[i];
-        r.d = r.turned ? cols[i] : rows[i];
-        r.n = r.turned ? rows[i] : cols[i];
+        const int m = order ? order[i] : i;
+        if (group_of(rows[m], cols[m], r.W) != group) continue;
+        r.rows = rows[m];
+        r.cols = cols[m];
+        r.turned = r.rows > r.cols;
+        r.d = r.turned ? r.cols : r.rows;
+        r.n = r.turned ? r.rows : r.cols;
         const int64_t e = (int64_t)r.rows * r.cols;
         r.nb = (int)(e > 256ll * NORM_ELEMS ? 256 : cdiv(e, NORM_ELEMS));
         int64_t mine[GRIDS] = {0, 0, 0};
@@ -1368,6 +1375,35 @@ int layout(const int* rows, const int* cols, int first, int n, int group, const 
     return i;
 }
 
+// The order of a group's matrices in the grids: as listed when they are of one length; else the long ones first, dealt to the 8 XCDs (each takes a
+// contiguous eighth of a grid's tiles), so that no XCD is left with all the long sums of X X^T (15 matrices of 256 x 256, 5 of 512 x 256 and 10
+// of 1024 x 256: 280 -> 249 us).  order: room for 3 n entries; returns their number.
+int arrange(const int* rows, const int* cols, int n, int group, int* order) {
+    int count = 0, W;
+    bool same = true;
+    auto length = [&](int i) { return rows[i] > cols[i] ? rows[i] : cols[i]; };
+    for (int i = 0; i < n; ++i)
+        if (group_of(rows[i], cols[i], W) == group) {
+            order[count++] = i;
+            same = same && length(i) == length(order[0]);
+        }
+    if (same) return count;
+    int *sorted = order + n, *bin = sorted + n;
+    int64_t load[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    for (int k = 0; k < count; ++k) sorted[k] = order[k];
+    std::sort(sorted, sorted + count, [&](int a, int b) { return length(a) != length(b) ? length(a) > length(b) : a < b; });
+    for (int k = 0; k < count; ++k) {
+        const int64_t t = cdiv(rows[sorted[k]] < cols[sorted[k]] ? rows[sorted[k]] : cols[sorted[k]], 32);
+        bin[k] = (int)(std::min_element(load, load + 8) - load);
+        load[bin[k]] += t * (t + 1) / 2;
+    }
+    int at = 0;
+    for (int b = 0; b < 8; ++b)
+        for (int k = 0; k < count; ++k)
+            if (bin[k] == b) order[at++] = sorted[k];
+    return count;
+}
+
 // exponents that keep X_k, A and q of every step within a quarter of fp16's range; false: the iteration leaves any useful range
 struct Steps { int ex[MAX_STEPS + 1], ea[MAX_STEPS], eq[MAX_STEPS]; };
 bool ranges(const double* coeffs, int steps, Steps& S) {
@@ -1416,13 +1452,13 @@ struct Job {
 template <int Q> void sym_product(int T, bool split, const StageP& p, hipStream_t st) {
     if (T == 32) hipLaunchKernelGGL((muon_sym_split_kernel<Q>), dim3(p.total), dim3(NT), 0, st, p);
     else if (split) hipLaunchKernelGGL((muon_sym_kernel<64, 64, 4, Q>), dim3(p.total), dim3(NT), 0, st, p);
-    else if (T == 128) hipLaunchKernelGGL((muon_sym_kernel<128, 32, 1, Q>), dim3(p.total), dim3(NT), 0, st, p);
+    else if (T == 128) hipLaunchKernelGGL((muon_sym_kernel<128, 32, 1, Q>), dim3(p.total), dim3(threads_of(128)), 0, st, p);
     else hipLaunchKernelGGL((muon_sym_kernel<64, 64, 1, Q>), dim3(p.total), dim3(NT), 0, st, p);
 }
 template <bool LAST> void update_product(int T, bool split, const StageP& p, hipStream_t st) {
     if (T == 32) hipLaunchKernelGGL((muon_update_split_kernel<LAST>), dim3(p.total), dim3(NT), 0, st, p);
     else if (split) hipLaunchKernelGGL((muon_update_kernel<64, 64, 4, LAST>), dim3(p.total), dim3(NT), 0, st, p);
-    else if (T == 128) hipLaunchKernelGGL((muon_update_kernel<128, 32, 1, LAST>), dim3(p.total), dim3(NT), 0, st, p);
+    else if (T == 128) hipLaunchKernelGGL((muon_update_kernel<128, 32, 1, LAST>), dim3(p.total), dim3(threads_of(128)), 0, st, p);
     else hipLaunchKernelGGL((muon_update_kernel<64, 64, 1, LAST>), dim3(p.total), dim3(NT), 0, st, p);
 }
 StageP stage_params(const Layout& L, const Job& j, const Steps& S, char* ws) {
@@ -1502,7 +1538,7 @@ int64_t workspace_of(const int* rows, const int* cols, int n, const Choice& T) {
     int64_t need = 0;
     for (int group = 0; group < GROUPS; ++group) {
         Layout L;
-        if (layout(rows, cols, 0, n, group, T, n, L, nullptr) < 0) return -1;
+        if (layout(rows, cols, nullptr, 0, n, group, T, n, L, nullptr) < 0) return -1;
         need += L.total;
     }
     return need > 256 ? need : 256;
@@ -1524,12 +1560,18 @@ int run_job(const char* what, const Job& j, void* ws, int64_t ws_bytes, void* st
     POET_CHECK(need >= 0, POET_ERR_UNSUPPORTED, "%s: too many tiles", what);
     POET_CHECK(ws && ((uintptr_t)ws % 256) == 0 && ws_bytes >= need, POET_ERR_ARG, "%s: workspace of %lld bytes needed (256-byte aligned), %lld given", what,
                (long long)need, (long long)ws_bytes);
+    struct Ints {
+        int* p;
+        ~Ints() { delete[] p; }
+    } order = {new (std::nothrow) int[3 * (size_t)j.n]};
+    POET_CHECK(order.p, POET_ERR_ARG, "%s: no host memory for a list of %d", what, j.n);
     hipStream_t st = (hipStream_t)stream;
     char* base = (char*)ws;
     for (int group = 0; group < GROUPS; ++group) {
         Layout L;
-        layout(j.rows, j.cols, 0, j.n, group, T, j.n, L, nullptr);
-        if (!L.count) continue;
+        const int members = arrange(j.rows, j.cols, j.n, group, order.p);
+        if (!members) continue;
+        layout(j.rows, j.cols, order.p, 0, members, group, T, members, L, nullptr);
         const bool single = group > 0 && group <= MAX_D;
         NormP np = {};
         np.table = (Rec*)(base + L.table);
@@ -1547,13 +1589,12 @@ int run_job(const char* what, const Job& j, void* ws, int64_t ws_bytes, void* st
             Recs recs = {};
             Layout C;
             const int from = at;
-            at = layout(j.rows, j.cols, from, j.n, group, T, CHUNK, C, recs.r);
+            at = layout(j.rows, j.cols, order.p, from, members, group, T, CHUNK, C, recs.r);
             int blocks = 0;
-            for (int i = from, c = 0; c < C.count; ++i) {
-                int W;
-                if (group_of(j.rows[i], j.cols[i], W) != group) continue;
-                Rec& r = recs.r[c++];
-                if (np.first + c == 1) shape = r;
+            for (int c = 0; c < C.count; ++c) {
+                const int i = order.p[from + c];
+                Rec& r = recs.r[c];
+                if (np.first + c == 0) shape = r;
                 one_shape = one_shape && r.d == shape.d && r.n == shape.n;
                 r.x0 += planes; r.x1 += planes; r.am += planes; r.bm += planes;
                 r.part0 += parts;
