@@ -317,9 +317,10 @@ template <int ROWB> __device__ __forceinline__ int swz_col(int krow) {
 }
 
 // Threads of a workgroup with a T x T tile, and its waves' shares of it: 64: 4 waves of 32 x 32; 128: 8 waves of 32 x 64 (first x second), so that
-// two waves of a SIMD alternate between LDS reads and matrix instructions (2048 x 2048: 850 -> 835 us; of 4 waves of 64 x 64, fragments read a stage
-// ahead, two workgroups on a CU, 858, where these take 816).  Of the 55 us of a 2048^3 product's launch 44 are left without the loads and 39 without
-// the rest.
+// two waves of a SIMD alternate between LDS reads and matrix instructions (4 waves of 64 x 64 that read their fragments a stage ahead: 858 us at
+// 2048 x 2048 where these took 816).  A 2048^3 update takes 56 us (0.92 PFLOP/s of fp16 products, a large library product reaches 1.03); 44 are
+// left without its loads, 39 without everything else.  A symmetric 2048 x 2048 x 2048 product, 528 tiles of
+// 64 x 64 on 256 CUs, takes 50 us: three tiles after one another on some CUs, and 1 MB of operands through a CU's port per tile.
 constexpr int threads_of(int T) { return T == 128 ? 512 : 256; }
 // SETS > 1: stage k of BK goes to accumulator set k % SETS, so that the sum has the order of the split kernels below.
 // acc[set][f][s][r] += sum_k first[f 16 + 4 (lane / 16) + r][k] second[s 16 + lane % 16][k] over a T x T tile.
@@ -330,107 +331,57 @@ template <int T, int BK, bool KM, int SETS, int SLOTS> struct Core {
     static constexpr int ROWB = BK * 2, CPR = BK / 8, PLANE = T * BK * 2, STAGE = 4 * PLANE;
     static constexpr int NL = PLANE / 16 / N;                                            // 16-byte loads per thread and plane
     static constexpr int COLB = T * 2, CPC = T / 8;
-    static constexpr int AHEAD = T == 64 && SETS == 1 ? 4 : 2, UNROLL = SETS > AHEAD ? SETS : AHEAD;      // stages in registers on their way to LDS
-    static __device__ __forceinline__ void run(const _Float16* fh, const _Float16* fl, int64_t ldf, const _Float16* sh, const _Float16* sl, int64_t lds_,
-                                               int K, char* smem, f32x4_t (&acc)[SETS][F][S]) {
-        const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wf = wave % WF * 32, ws = wave / WF * (T / 2);
-        const int m16 = lane & 15, kc = lane >> 4;
-        int64_t go[NL], so[NL];
-        int lo_f[NL], lo_s[NL];
-#pragma unroll
-        for (int q = 0; q < NL; ++q) {
-            const int idx = q * N + tid, row = idx / CPR, c = idx % CPR;
-            so[q] = row * lds_ + c * 8;
-            lo_s[q] = row * ROWB + ((c ^ swz_row<ROWB>(row)) & (CPR - 1)) * 16;
-            if constexpr (KM) {
-                const int kr = idx / CPC, cc = idx % CPC;
-                go[q] = kr * ldf + cc * 8;
-                lo_f[q] = kr * COLB + (((cc >> 1) ^ swz_col<COLB>(kr)) * 32) + (cc & 1) * 16;
-            } else {
-                go[q] = row * ldf + c * 8;
-                lo_f[q] = lo_s[q];
-            }
-        }
-        u32x4_t rf[AHEAD][2][NL], rs[AHEAD][2][NL];
-        auto fetch = [&](int k, u32x4_t (&f)[2][NL], u32x4_t (&s)[2][NL]) {
-            const int64_t kf = KM ? (int64_t)k * ldf : k;
-#pragma unroll
-            for (int q = 0; q < NL; ++q) {
-                f[0][q] = *reinterpret_cast<const u32x4_t*>(fh + go[q] + kf);
-                f[1][q] = *reinterpret_cast<const u32x4_t*>(fl + go[q] + kf);
-                s[0][q] = *reinterpret_cast<const u32x4_t*>(sh + so[q] + k);
-                s[1][q] = *reinterpret_cast<const u32x4_t*>(sl + so[q] + k);
-            }
-        };
-        auto store = [&](char* st, const u32x4_t (&f)[2][NL], const u32x4_t (&s)[2][NL]) {
-#pragma unroll
-            for (int q = 0; q < NL; ++q) {
-                *reinterpret_cast<u32x4_t*>(st + lo_f[q]) = f[0][q];
-                *reinterpret_cast<u32x4_t*>(st + PLANE + lo_f[q]) = f[1][q];
-                *reinterpret_cast<u32x4_t*>(st + 2 * PLANE + lo_s[q]) = s[0][q];
-                *reinterpret_cast<u32x4_t*>(st + 3 * PLANE + lo_s[q]) = s[1][q];
-            }
-        };
-#pragma unroll
-        for (int a = 0; a < AHEAD; ++a)
-            if (a * BK < K) fetch(a * BK, rf[a], rs[a]);
-        for (int k0 = 0; k0 < K; k0 += UNROLL * BK) {
-#pragma unroll
-            for (int a = 0; a < UNROLL; ++a) {
-                const int k = k0 + a * BK;
-                if (k >= K) break;
-                char* st = smem + (a & 1) * STAGE;
-                store(st, rf[a % AHEAD], rs[a % AHEAD]);          // (this slot's readers, two stages back, passed the barrier of the stage between)
-                __syncthreads();
-                if (k + AHEAD * BK < K) fetch(k + AHEAD * BK, rf[a % AHEAD], rs[a % AHEAD]);
-                stage(st, acc[a % SETS], wf, ws, m16, kc);
-            }
-        }
-    }
-    // T = 128: the stages reach LDS by DMA, a ring of SLOTS of them (two, and two workgroups on a CU; four where no CU gets a second workgroup: 2048 x
-    // 2048, 256 and 136 tiles: 816 -> 780 us; 4 x 4096 x 1024 the other way round, 1347 -> 1246 with two).  A wave moves 1 KB of each of the four planes;
-    // counted waits and a raw barrier, one a stage: every wave's pieces of stage k have arrived and every wave has read stage k - 1, into whose slot stage k + SLOTS - 1 goes.  (Inline
-    // assembly because the compiler would drain the queue in front of every LDS read.  M0 is written behind its back -- it takes no such clobber --
-    // and nothing else in these kernels uses it.)
     static constexpr int LDS = SLOTS * STAGE;
+    // Stages reach LDS by DMA, a ring of SLOTS of them: a wave moves NL KB of each of the four planes.  Counted waits and a raw barrier, one a stage:
+    // every wave's pieces of stage k have arrived and every wave has read stage k - 1, into whose slot stage k + SLOTS - 1 goes.  Two slots, and two
+    // workgroups on a CU; four where no CU gets a second workgroup (1024 x 1024: 234 -> 210 us, ten 1024 x 256: 175 -> 169, 2048 x 2048: 816 -> 780;
+    // 4 x 4096 x 1024 with four throughout: 1347 against 1246).  (Inline assembly because the compiler would drain the queue in front of every LDS
+    // read.  M0 is written behind its back -- it takes no such clobber -- and nothing else in this file uses it.)
     static __device__ __forceinline__ void dma(uint32_t voff, const void* base, uint32_t lds) {
         asm volatile("s_nop 4\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(base), "s"(lds) : "memory");
     }
-    static __device__ __forceinline__ void ring(const _Float16* fh, const _Float16* fl, int64_t ldf, const _Float16* sh, const _Float16* sl, int64_t lds_,
+    static __device__ __forceinline__ void run(const _Float16* fh, const _Float16* fl, int64_t ldf, const _Float16* sh, const _Float16* sl, int64_t lds_,
                                                 int K, char* smem, f32x4_t (&acc)[SETS][F][S]) {
-        static_assert(SETS == 1 && NL == 1 && LDS >= T * T * 4, "one 16-byte piece per thread and plane");
+        static_assert(LDS >= T * T * 4, "the tile fits the stages' LDS");
         const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wf = wave % WF * 32, ws = wave / WF * (T / 2);
         const int m16 = lane & 15, kc = lane >> 4;
-        // which piece of a stage belongs at this thread's place of a plane
-        const int row = tid / CPR, c = ((tid % CPR) ^ swz_row<ROWB>(row)) & (CPR - 1);
-        const uint32_t so = (uint32_t)(row * lds_ + c * 8) * 2u;
-        uint32_t go;
-        if constexpr (KM) {
-            const int kr = tid / CPC, pc = tid % CPC;
-            go = (uint32_t)(kr * ldf + (((((pc >> 1) ^ swz_col<COLB>(kr)) << 1) | (pc & 1)) * 8)) * 2u;
-        } else go = (uint32_t)(row * ldf + c * 8) * 2u;
+        // which pieces of a stage belong at this thread's places of a plane
+        uint32_t go[NL], so[NL];
+#pragma unroll
+        for (int q = 0; q < NL; ++q) {
+            const int idx = q * N + tid, row = idx / CPR, c = ((idx % CPR) ^ swz_row<ROWB>(row)) & (CPR - 1);
+            so[q] = (uint32_t)(row * lds_ + c * 8) * 2u;
+            if constexpr (KM) {
+                const int kr = idx / CPC, pc = idx % CPC;
+                go[q] = (uint32_t)(kr * ldf + (((((pc >> 1) ^ swz_col<COLB>(kr)) << 1) | (pc & 1)) * 8)) * 2u;
+            } else go[q] = (uint32_t)(row * ldf + c * 8) * 2u;
+        }
         const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)smem + wave * 1024;
         auto issue = [&](int k, int slot) {
             const int64_t kf = (KM ? k * ldf : k) * BK, ks = (int64_t)k * BK;
-            const uint32_t to = base + slot * STAGE;
-            dma(go, fh + kf, to);
-            dma(go, fl + kf, to + PLANE);
-            dma(so, sh + ks, to + 2 * PLANE);
-            dma(so, sl + ks, to + 3 * PLANE);
+#pragma unroll
+            for (int q = 0; q < NL; ++q) {
+                const uint32_t to = base + slot * STAGE + q * N * 16;
+                dma(go[q], fh + kf, to);
+                dma(go[q], fl + kf, to + PLANE);
+                dma(so[q], sh + ks, to + 2 * PLANE);
+                dma(so[q], sl + ks, to + 3 * PLANE);
+            }
         };
+        constexpr int UNROLL = SETS > SLOTS ? SETS : SLOTS;
         const int nk = K / BK;
 #pragma unroll
         for (int a = 0; a < SLOTS - 1; ++a)
             if (a < nk) issue(a, a);
-        for (int k0 = 0; k0 < nk; k0 += SLOTS) {
+        for (int k0 = 0; k0 < nk; k0 += UNROLL) {
 #pragma unroll
-            for (int a = 0; a < SLOTS; ++a) {
+            for (int a = 0; a < UNROLL; ++a) {
                 const int k = k0 + a;
                 if (k >= nk) break;
-                if (nk - 1 - k >= SLOTS - 2) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(4 * (SLOTS - 2)) : "memory");
+                if (nk - 1 - k >= SLOTS - 2) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(4 * NL * (SLOTS - 2)) : "memory");
                 else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
                 if (k + SLOTS - 1 < nk) issue(k + SLOTS - 1, (a + SLOTS - 1) % SLOTS);
-                stage(smem + a * STAGE, acc[0], wf, ws, m16, kc);
+                stage(smem + a % SLOTS * STAGE, acc[a % SETS], wf, ws, m16, kc);
             }
         }
     }
@@ -674,7 +625,7 @@ template <int SETS, int S> __device__ __forceinline__ void fold_sets(f32x4_t (&a
 }
 
 // A = X X^T (Q = 0), or q = a I + b A + c A A (Q = 1): tiles on and below the diagonal
-template <int T, int BK, int SETS, int SLOTS, int Q> __global__ __launch_bounds__(threads_of(T), SLOTS == 2 ? threads_of(T) / 128 : 2) void muon_sym_kernel(const StageP p) {
+template <int T, int BK, int SETS, int SLOTS, int Q> __global__ __launch_bounds__(threads_of(T), T == 128 && SLOTS == 2 ? 4 : 2) void muon_sym_kernel(const StageP p) {
     typedef Core<T, BK, false, SETS, SLOTS> C;
     typedef Meet<T> M;
     static_assert(C::LDS >= T * T * 4, "the tile fits the stages' LDS");
@@ -690,8 +641,7 @@ template <int T, int BK, int SETS, int SLOTS, int Q> __global__ __launch_bounds_
     zero(acc);
     uint2 ah[M::U], al[M::U];
     if constexpr (Q && T == 64) a_pieces<T>(p, r, i0, j0, ah, al);            // (ahead of the product: 16 registers)
-    if constexpr (T == 128) C::ring(in + j0 * ld, in + plane + j0 * ld, ld, in + i0 * ld, in + plane + i0 * ld, ld, K, smem, acc);
-    else C::run(in + j0 * ld, in + plane + j0 * ld, ld, in + i0 * ld, in + plane + i0 * ld, ld, K, smem, acc);
+    C::run(in + j0 * ld, in + plane + j0 * ld, ld, in + i0 * ld, in + plane + i0 * ld, ld, K, smem, acc);
     if constexpr (Q && T != 64) a_pieces<T>(p, r, i0, j0, ah, al);
     fold_sets(acc);
     f32x4_t v[M::U];
@@ -700,7 +650,7 @@ template <int T, int BK, int SETS, int SLOTS, int Q> __global__ __launch_bounds_
 }
 
 // X' = q X; the last step leaves the planes: the output matrix, or the weight update
-template <int T, int BK, int SETS, int SLOTS, bool LAST> __global__ __launch_bounds__(threads_of(T), SLOTS == 2 ? threads_of(T) / 128 : 2) void muon_update_kernel(const StageP p) {
+template <int T, int BK, int SETS, int SLOTS, bool LAST> __global__ __launch_bounds__(threads_of(T), T == 128 && SLOTS == 2 ? 4 : 2) void muon_update_kernel(const StageP p) {
     typedef Core<T, BK, true, SETS, SLOTS> C;
     typedef Meet<T> M;
     extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -716,8 +666,7 @@ template <int T, int BK, int SETS, int SLOTS, bool LAST> __global__ __launch_bou
     f32x4_t acc[SETS][C::F][C::S];
     zero(acc);
     const int K = (r.d + BK - 1) / BK * BK;
-    if constexpr (T == 128) C::ring(x + j0, x + plane + j0, np, qm + (int64_t)i0 * dp, qm + sq + (int64_t)i0 * dp, dp, K, smem, acc);
-    else C::run(x + j0, x + plane + j0, np, qm + (int64_t)i0 * dp, qm + sq + (int64_t)i0 * dp, dp, K, smem, acc);
+    C::run(x + j0, x + plane + j0, np, qm + (int64_t)i0 * dp, qm + sq + (int64_t)i0 * dp, dp, K, smem, acc);
     fold_sets(acc);
     f32x4_t v[M::U];
     M::share(reinterpret_cast<float*>(smem), acc[0], v);
@@ -1340,11 +1289,12 @@ int group_of(int rows, int cols, int& W) {
 }
 
 Choice tiles_of(const int* rows, const int* cols, int n) {
-    // d > 256: 128 x 128 tiles halve the operand traffic per product, 64 x 64 tiles make (up to) four times as many workgroups: the large ones once
-    // they keep half of the CUs busy (update of 1024 x 1024, 64 tiles: 302 us against 230, 1536 x 1536, 144 tiles: 506 against 516, 2048 x 2048, 256
-    // tiles: 842 against 996; symmetric products of 1536 x 1536, 78 tiles: 689 against 516, 2048 x 2048, 136 tiles: 780 against 832, 16 x 512 x
-    // 512, 160 tiles of only 16 stages: 333 against 322, 6 x 1024 x 1024, 216 tiles: 572 against 633).  d <= 256: 32 x 32 tiles while they fit the
-    // chip once (twice in the update): four 256 x 256 87 us against 116; sixteen 144 against 120, ten 1024 x 256 231 against 189.
+    // d > 256: 128 x 128 tiles halve the operand traffic per product, 64 x 64 tiles make (up to) four times as many workgroups.  The update takes the
+    // large ones once they keep half of the CUs busy (1024 x 1024, 64 tiles: 302 us against 230, 1536 x 1536, 144 tiles: 402 against 419, 2048 x
+    // 2048, 256 tiles: 763 against 822, 4 x 4096 x 1024: 1119 against 1476), the symmetric products
+    // once they fill it (2048 x 2048, 136 tiles: 783 against 763, 6 x 1024 x 1024, 216 tiles: 549 against 531, 3000 x 3000, 300 tiles:
+    // 2019 against 2066).  d <= 256: 32 x 32 tiles while they fit the chip once (twice in the update): four 256 x 256 87 us against 116; sixteen 144
+    // against 111, ten 1024 x 256 231 against 169.
     int64_t sym = 0, upd = 0, ssym = 0, supd = 0;
     for (int i = 0; i < n; ++i) {
         int W;
@@ -1359,7 +1309,7 @@ Choice tiles_of(const int* rows, const int* cols, int n) {
             supd += (int64_t)cdiv(rows[i], 32) * cdiv(cols[i], 32);
         }
     }
-    return {{sym >= CUS / 2 ? 128 : 64, upd >= CUS / 2 ? 128 : 64}, {ssym > 256 ? 64 : 32, supd > 512 ? 64 : 32}};
+    return {{sym >= CUS ? 128 : 64, upd >= CUS / 2 ? 128 : 64}, {ssym > 256 ? 64 : 32, supd > 512 ? 64 : 32}};
 }
 
 // the records of one group among matrices [first, n) -- or among order[first .. n) -- (at most `most` of them): shape-dependent members into rec
@@ -1517,15 +1467,19 @@ template <int T, int BK, int SETS, int SLOTS, bool LAST> void update_staged(cons
 }
 template <int Q> void sym_product(int T, bool split, const StageP& p, hipStream_t st) {
     if (T == 32) hipLaunchKernelGGL((muon_sym_split_kernel<Q>), dim3(p.total), dim3(NT), 0, st, p);
-    else if (split) sym_staged<64, 64, 4, 2, Q>(p, st);
-    else if (T == 64) sym_staged<64, 64, 1, 2, Q>(p, st);
+    else if (split && p.total > CUS) sym_staged<64, 64, 4, 2, Q>(p, st);
+    else if (split) sym_staged<64, 64, 4, 4, Q>(p, st);
+    else if (T == 64 && p.total > CUS) sym_staged<64, 64, 1, 2, Q>(p, st);
+    else if (T == 64) sym_staged<64, 64, 1, 4, Q>(p, st);
     else if (p.total > CUS) sym_staged<128, 32, 1, 2, Q>(p, st);
     else sym_staged<128, 32, 1, 4, Q>(p, st);
 }
 template <bool LAST> void update_product(int T, bool split, const StageP& p, hipStream_t st) {
     if (T == 32) hipLaunchKernelGGL((muon_update_split_kernel<LAST>), dim3(p.total), dim3(NT), 0, st, p);
-    else if (split) update_staged<64, 64, 4, 2, LAST>(p, st);
-    else if (T == 64) update_staged<64, 64, 1, 2, LAST>(p, st);
+    else if (split && p.total > CUS) update_staged<64, 64, 4, 2, LAST>(p, st);
+    else if (split) update_staged<64, 64, 4, 4, LAST>(p, st);
+    else if (T == 64 && p.total > CUS) update_staged<64, 64, 1, 2, LAST>(p, st);
+    else if (T == 64) update_staged<64, 64, 1, 4, LAST>(p, st);
     else if (p.total > CUS) update_staged<128, 32, 1, 2, LAST>(p, st);
     else update_staged<128, 32, 1, 4, LAST>(p, st);
 }
