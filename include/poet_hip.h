@@ -58,8 +58,8 @@ extern "C" {
 
 #define POET_F32 0
 #define POET_BF16 1
-#define POET_F16 2   /* IEEE half STORAGE (11 significant bits in the same 2 bytes as bf16's 8): accepted by poet_groupnorm_act_* and as
-                        the q_dtype of poet_msda_fused_fwd / _bwd -- the sampling offsets and attention logits, values of a few units that no GEMM
+#define POET_F16 2   /* IEEE half STORAGE (11 significant bits in the same 2 bytes as bf16's 8): accepted by poet_groupnorm_act_* and
+                        poet_orthogonalize, and as the q_dtype of poet_msda_fused_fwd / _bwd -- the sampling offsets and attention logits, values of a few units that no GEMM
                         ever reads as an operand -- produced by poet_gemm with c_dtype = POET_BF16 and c_f16 = 1.  Gradients of
                         such a buffer are bf16. */
 
@@ -388,7 +388,8 @@ int poet_groupnorm_bwd(const void* dy, const void* x, const float* stats, const 
  * y likewise.  y = act(gamma h + beta), h = (x - mean) rstd over the HW x (C / G) values of (image, group); any C / G.
  * act: POET_ACT_*.  Types of (x, y): (fp32, fp32), (bf16, bf16), (fp16, fp16), (bf16, fp32), (fp32, bf16); gamma / beta fp32 (C).
  * stats (N, G, 2) fp32 = (mean, rstd): written by forward (optional there), read by backward, 8-byte aligned.
- * y may be x itself.  Backward recomputes z = gamma h + beta: dx (optional; x's type) and dgamma / dbeta (optional, together; fp32 (C)),
+ * y may be x itself, dx may be x or dy (no other overlap).  Backward recomputes z = gamma h + beta: dx (optional; x's type) and dgamma / dbeta
+ * (optional, together; fp32 (C)),
  * overwritten, or added to when `accumulate` != 0.  No atomics: results are bit-reproducible.
  * workspace: caller-owned, poet_groupnorm_act_workspace(N, HW, C, G) bytes (negative: an error code), 8-byte aligned; contents
  * undefined afterwards, not shared with a launch that may run at the same time. */
@@ -458,7 +459,7 @@ int poet_adamw(float* p, const float* g, float* m, float* v, uint16_t* p_bf16, u
                                         belongs to another optimiser (poet_muon_step) and is left alone: p, m, v, images */,
                void* stream);
 /* ------------------------------------------------------------------------------------------------
- * Orthogonalised updates of weight matrices (the Muon optimiser), a LIST of n matrices of any shapes in one chain of launches.
+ * Orthogonalised updates of weight matrices (the Muon optimiser), a LIST of n matrices of any shapes in a few chains of launches.
  * Matrix i is rows[i] x cols[i] (1 .. 2^20 each).  With u the input (orthogonalize) or the update direction (muon_step):
  *     X = u / (||u||_F + eps), turned so that rows <= cols;  steps times: A = X X^T, X <- (a I + b A + c A^2) X;  result X, turned back.
  * coeffs_host: steps x (a, b, c), 1 <= steps <= 16; coefficients under which the scalar iteration leaves |x| < 1e3 on [0, 1] are refused.

@@ -13,9 +13,9 @@
 //    the same simulation, to within 10 %) at a third of the fp16 rate, five times the rate of the fp32 matrix instructions.  The exponents s
 //    come from bounds of the scalar iteration on [0, 1] (host), so that nothing overflows and lo parts stay normal numbers.
 //  * Iterating on A alone (d x d, cheaper for n >> d) was rejected: it squares the condition number, 2e-4 off at fp32.
-//  * A LIST of matrices of any shapes runs in ONE chain of launches (2 + 3 steps): a device table of records, each workgroup finds
-//    its (matrix, tile) from the first tiles.  A stage's tiles of all matrices overlap; PoET's encoder alone has 30 matrices of which none
-//    fills the chip.
+//  * A LIST of matrices of any shapes is worked on together: its matrices fall into groups by their own shape (group_of below), and the matrices
+//    of a group share launches -- one for the narrowest, 2 + steps for narrow ones in slabs, a chain of 2 + 3 steps for the rest: a device table
+//    of records, each workgroup finds its (matrix, tile) from the first tiles.  PoET's encoder alone has 30 matrices of which none fills the chip.
 //  * No atomics anywhere: results do not depend on workgroup order, nor on the other matrices of the list.
 #include "common.cuh"
 
@@ -675,11 +675,11 @@ template <int T, int BK, int SETS, int SLOTS, bool LAST> __global__ __launch_bou
 
 // ---- 3b: the same products for short lists of matrices with d <= 256: 32 x 32 tiles, K split over the waves -------------------------
 // With K = d <= 256 a launch is a few microseconds of latency: of the 64 x 64 tiles above, staged through LDS, a K = 256 product is
-// store - barrier - read - multiply in turn with one wave per SIMD, and 128 KB of operands pass one CU's port.  Here the tile is a quarter, so that
+// four stages in turn with one wave per SIMD, and 128 KB of operands pass one CU's port.  Here the tile is a quarter, so that
 // four times as many CUs pull operands, and every wave multiplies the whole tile over its own steps of 32 k, its fragments loaded straight
 // into registers (a lane's 16 bytes of a row are the fragment), all in flight at once, no barrier; the partial tiles meet once in LDS.  Four
-// 256 x 256 matrices: 116 -> 89 us.  Half as much reuse of every operand byte, and 64-byte pieces of rows instead of 128: ten 1024 x 256
-// take 231 us this way against 189 with the staged tiles (and as much with 64 x 64 tiles that load like these).
+// 256 x 256 matrices: 110 -> 83 us.  Half as much reuse of every operand byte, and 64-byte pieces of rows instead of 128: ten 1024 x 256
+// take 231 us this way against 169 with the staged tiles (and as much as 231 with 64 x 64 tiles that load like these).
 struct Frags { f16x8_t h[2], l[2]; };
 __device__ __forceinline__ void mfma_tile(f32x4_t (&acc)[2][2], const Frags& f, const Frags& s) {
 #pragma unroll
@@ -1293,8 +1293,8 @@ Choice tiles_of(const int* rows, const int* cols, int n) {
     // large ones once they keep half of the CUs busy (1024 x 1024, 64 tiles: 302 us against 230, 1536 x 1536, 144 tiles: 402 against 419, 2048 x
     // 2048, 256 tiles: 763 against 822, 4 x 4096 x 1024: 1119 against 1476), the symmetric products
     // once they fill it (2048 x 2048, 136 tiles: 783 against 763, 6 x 1024 x 1024, 216 tiles: 549 against 531, 3000 x 3000, 300 tiles:
-    // 2019 against 2066).  d <= 256: 32 x 32 tiles while they fit the chip once (twice in the update): four 256 x 256 87 us against 116; sixteen 144
-    // against 111, ten 1024 x 256 231 against 169.
+    // 2019 against 2066).  d <= 256: 32 x 32 tiles while they fit the chip once (twice in the update): four 256 x 256 83 us against
+    // 110, seven 95 against 115; sixteen 144 against 111, ten 1024 x 256 231 against 169.
     int64_t sym = 0, upd = 0, ssym = 0, supd = 0;
     for (int i = 0; i < n; ++i) {
         int W;

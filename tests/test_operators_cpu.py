@@ -2,6 +2,9 @@
 error codes before anything is launched, the tensor-level wrappers raise."""
 import ctypes
 import os
+import re
+import shutil
+import subprocess
 
 import pytest
 import torch
@@ -155,3 +158,16 @@ def test_sizes_beyond_a_launch_are_refused(lib):
     assert need > 0 and gn_fwd(lib, N=1 << 24, HW=1, C=64, G=64, nws=need) in REFUSED and b"threads" in lib.poet_hip_last_error()
     for cf in ((3.0, float("nan"), 0.0), (3.0, 0.0, float("nan")), (3.0, float("-inf"), 0.0)):
         assert orth(lib, coeffs=cf) in REFUSED and b"range" in lib.poet_hip_last_error()
+
+
+def test_m0_is_only_written_by_the_dma(tmp_path):
+    """The tiles' LDS-DMA sets M0 by hand in inline assembly (hipcc takes no "m0" clobber): safe only while nothing else in that source uses it."""
+    from poet_amd.build import CSRC, FLAGS, _hipcc
+    if not (os.path.exists(_hipcc()) or shutil.which(_hipcc())):
+        pytest.skip("no hipcc")
+    out = str(tmp_path / "muon.s")
+    subprocess.check_call([_hipcc(), *FLAGS, "-S", "--cuda-device-only", os.path.join(CSRC, "muon.hip"), "-o", out], stderr=subprocess.DEVNULL)
+    text = open(out).read()
+    lines = [l.strip() for l in text.splitlines() if re.search(r"\bm0\b", l) and not l.lstrip().startswith((";", "//"))]
+    assert lines and all(re.fullmatch(r"s_mov_b32 m0, s\d+", l) for l in lines), [l for l in lines if not re.fullmatch(r"s_mov_b32 m0, s\d+", l)][:5]
+    assert not re.search(r"v_movrel|s_set_gpr_idx", text)
