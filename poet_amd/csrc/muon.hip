@@ -481,27 +481,33 @@ template <int T> struct Meet {
             for (int e = 0; e < 4; ++e) v[u][e] = part[at(col() + e, row(u) >> 2) + (row(u) & 3)];
     }
 };
+// four neighbouring elements of the output matrix, or of the weight update from the old weights o, where these are aligned (ovec)
+__device__ __forceinline__ void put4(const Rec& m, const StageP& p, float lr, int64_t at, const f32x4_t& v, f32x4_t o) {
+    if (p.muon) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = fmaf(-lr * m.out_scale, v[e], o[e] - lr * p.wd * o[e]);
+        *reinterpret_cast<f32x4_t*>((float*)m.o + at) = o;
+        if (m.p16) {
+            const uint2 hi = make_uint2(pack_bf2(o[0], o[1]), pack_bf2(o[2], o[3]));
+            *reinterpret_cast<uint2*>(m.p16 + at) = hi;
+            if (m.p16lo)
+                *reinterpret_cast<uint2*>(m.p16lo + at) = make_uint2(pack_bf2(o[0] - __uint_as_float(hi.x << 16), o[1] - __uint_as_float(hi.x & 0xffff0000u)),
+                                                                     pack_bf2(o[2] - __uint_as_float(hi.y << 16), o[3] - __uint_as_float(hi.y & 0xffff0000u)));
+        }
+    } else if (p.o_dtype == POET_F32) *reinterpret_cast<f32x4_t*>((float*)m.o + at) = v;
+    else {
+        const float w[4] = {v[0], v[1], v[2], v[3]};
+        if (p.o_dtype == POET_BF16) vec<bf16_t, 4>::st((bf16_t*)m.o + at, w);
+        else vec<f16_t, 4>::st((f16_t*)m.o + at, w);
+    }
+}
 // columns col .. col + 3 of a row of the output matrix, or of the weight update
 __device__ __forceinline__ void write4(const Rec& m, const StageP& p, float lr, int row, int col, const f32x4_t& v) {
     if (row >= m.rows || col >= m.cols) return;
     const int64_t at = row * m.ldo + col;
-    if (p.muon) {
+    if (m.ovec) put4(m, p, lr, at, v, p.muon ? *reinterpret_cast<const f32x4_t*>((const float*)m.o + at) : v);       // (cols % 4 == 0)
+    else if (p.muon) {
         float* w = (float*)m.o + at;
-        if (m.ovec) {                                                         // (cols % 4 == 0)
-            f32x4_t o = *reinterpret_cast<f32x4_t*>(w);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] = fmaf(-lr * m.out_scale, v[e], o[e] - lr * p.wd * o[e]);
-            *reinterpret_cast<f32x4_t*>(w) = o;
-            if (m.p16) {
-                const uint2 hi = make_uint2(pack_bf2(o[0], o[1]), pack_bf2(o[2], o[3]));
-                *reinterpret_cast<uint2*>(m.p16 + at) = hi;
-                if (m.p16lo)
-                    *reinterpret_cast<uint2*>(m.p16lo + at) =
-                        make_uint2(pack_bf2(o[0] - __uint_as_float(hi.x << 16), o[1] - __uint_as_float(hi.x & 0xffff0000u)),
-                                   pack_bf2(o[2] - __uint_as_float(hi.y << 16), o[3] - __uint_as_float(hi.y & 0xffff0000u)));
-            }
-            return;
-        }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             if (col + e >= m.cols) break;
@@ -513,11 +519,6 @@ __device__ __forceinline__ void write4(const Rec& m, const StageP& p, float lr, 
                 if (m.p16lo) m.p16lo[at + e] = f2bf(nw - bf2f(hi));
             }
         }
-    } else if (m.ovec && p.o_dtype == POET_F32) *reinterpret_cast<f32x4_t*>((float*)m.o + at) = v;
-    else if (m.ovec) {
-        const float o[4] = {v[0], v[1], v[2], v[3]};
-        if (p.o_dtype == POET_BF16) vec<bf16_t, 4>::st((bf16_t*)m.o + at, o);
-        else vec<f16_t, 4>::st((f16_t*)m.o + at, o);
     } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
@@ -863,6 +864,79 @@ template <int D> struct Slab {
         const int da = NW_T / cols, dc = NW_T % cols;
         double sum = 0.0;
         constexpr int U = 8;                                                  // loads in flight
+        if (r.rows_vec) {                                                     // (cols, j0 and the strides are multiples of 4; 32 x 896: 52 -> 40 us with finish())
+            const int cols4 = cols / 4, total4 = total / 4, da4 = NW_T / cols4, dc4 = NW_T % cols4;
+            int a4 = threadIdx.x / cols4, c4 = threadIdx.x % cols4;
+            auto vectors = [&](auto&& fetch, auto&& value) {                  // fetch(u, offset), then value(u, offset) -> four values
+                for (int e = threadIdx.x; e < total4; e += U * NW_T) {
+                    int64_t at[U];
+                    int ra[U], rc[U];
+#pragma unroll
+                    for (int u = 0; u < U; ++u) {
+                        const bool in = e + u * NW_T < total4;                // (behind the end: the first vector again)
+                        ra[u] = in ? a4 : 0;
+                        rc[u] = in ? c4 * 4 : 0;
+                        at[u] = (row0 + ra[u]) * r.ldg + col0 + rc[u];
+                        fetch(u, at[u]);
+                        a4 += da4;
+                        c4 += dc4;
+                        if (c4 >= cols4) c4 -= cols4, ++a4;
+                    }
+#pragma unroll
+                    for (int u = 0; u < U; ++u) {
+                        if (e + u * NW_T >= total4) break;
+                        const f32x4_t v = value(u, at[u]);
+                        uint32_t b[4];
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            sum = fma((double)v[q], (double)v[q], sum);
+                            b[q] = __float_as_uint(v[q]);
+                        }
+                        if (!r.turned) {
+                            char* o = x + ra[u] * xs + rc[u] * 2;
+                            *reinterpret_cast<uint2*>(o) = make_uint2((b[0] >> 16) | (b[1] & 0xffff0000u), (b[2] >> 16) | (b[3] & 0xffff0000u));
+                            *reinterpret_cast<uint2*>(o + xplane) = make_uint2((b[0] & 0xffffu) | (b[1] << 16), (b[2] & 0xffffu) | (b[3] << 16));
+                        } else {
+#pragma unroll
+                            for (int q = 0; q < 4; ++q) {
+                                char* o = x + (rc[u] + q) * xs + ra[u] * 2;
+                                *reinterpret_cast<uint16_t*>(o) = (uint16_t)(b[q] >> 16);
+                                *reinterpret_cast<uint16_t*>(o + xplane) = (uint16_t)b[q];
+                            }
+                        }
+                    }
+                }
+            };
+            f32x4_t g4[U], m4[U];
+            if (p.muon)
+                vectors([&](int u, int64_t at) { g4[u] = *reinterpret_cast<const f32x4_t*>((const float*)r.g + at), m4[u] = *reinterpret_cast<const f32x4_t*>(r.mom + at); },
+                        [&](int u, int64_t at) {
+                            f32x4_t v;
+#pragma unroll
+                            for (int q = 0; q < 4; ++q) {
+                                if constexpr (FIRST) {
+                                    float m = m4[u][q];
+                                    v[q] = direction(g4[u][q] * gs, m, p.mu, p.omu, p.nesterov);
+                                    m4[u][q] = m;
+                                } else v[q] = p.nesterov ? fmaf(p.mu, m4[u][q], p.omu * (g4[u][q] * gs)) : m4[u][q];
+                            }
+                            if constexpr (FIRST) *reinterpret_cast<f32x4_t*>(r.mom + at) = m4[u];
+                            return v;
+                        });
+            else if (p.g_dtype == POET_F32)
+                vectors([&](int u, int64_t at) { g4[u] = *reinterpret_cast<const f32x4_t*>((const float*)r.g + at); }, [&](int u, int64_t) { return g4[u]; });
+            else {
+                const bool bf = p.g_dtype == POET_BF16;
+                uint2 h4[U];
+                vectors([&](int u, int64_t at) { h4[u] = *reinterpret_cast<const uint2*>((const uint16_t*)r.g + at); },
+                        [&](int u, int64_t) {
+                            const uint2 w = h4[u];
+                            return bf ? f32x4_t{__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u)}
+                                      : f32x4_t{h_lo(w.x), h_hi(w.x), h_lo(w.y), h_hi(w.y)};
+                        });
+            }
+            return sum;
+        }
         auto batches = [&](auto&& fetch, auto&& value) {                      // fetch(u, offset of the element), then value(u, offset)
             for (int e = threadIdx.x; e < total; e += U * NW_T) {
                 int64_t at[U];
@@ -913,17 +987,18 @@ template <int D> struct Slab {
         int ex = 0;
         const float inv = (float)frexp(by, &ex);
         __syncthreads();
-#pragma unroll 4
-        for (int o = threadIdx.x * 4; o < xplane; o += NW_T * 4) {
-            const uint32_t h = *reinterpret_cast<const uint32_t*>(x + o), l = *reinterpret_cast<const uint32_t*>(x + xplane + o);
-            union { _Float16 f[2]; uint32_t u; } nh, nl;
+#pragma unroll 2
+        for (int o = threadIdx.x * 16; o < xplane; o += NW_T * 16) {          // (rows are whole 16-byte pieces)
+            const u32x4_t h = *reinterpret_cast<const u32x4_t*>(x + o), l = *reinterpret_cast<const u32x4_t*>(x + xplane + o);
+            u32x4_t nh, nl;
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const uint32_t bits = e ? (h & 0xffff0000u) | (l >> 16) : (h << 16) | (l & 0xffffu);
-                split16(ldexpf(__uint_as_float(bits) * inv, ex), nh.f[e], nl.f[e]);
+            for (int q = 0; q < 4; ++q) {
+                const float v0 = ldexpf(__uint_as_float((h[q] << 16) | (l[q] & 0xffffu)) * inv, ex), v1 = ldexpf(__uint_as_float((h[q] & 0xffff0000u) | (l[q] >> 16)) * inv, ex);
+                nh[q] = pack_h2(v0, v1);
+                nl[q] = pack_h2(v0 - h_lo(nh[q]), v1 - h_hi(nh[q]));
             }
-            *reinterpret_cast<uint32_t*>(x + o) = nh.u;
-            *reinterpret_cast<uint32_t*>(x + xplane + o) = nl.u;
+            *reinterpret_cast<u32x4_t*>(x + o) = nh;
+            *reinterpret_cast<u32x4_t*>(x + xplane + o) = nl;
         }
         __syncthreads();
     }
@@ -1019,9 +1094,22 @@ template <int D> struct Slab {
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
             const int i = bi * 32 + (q & 1) * 16 + m16, j = bj * 32 + (q >> 1) * 16 + 4 * kc;
+            if (bi == bj && (q & 1) < (q >> 1)) continue;                     // (above the diagonal)
+            if (bi == bj && (q & 1) == (q >> 1)) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (i >= j + e) put_a(i, j + e, acc[q >> 1][q & 1][e] * scale);
+                for (int e = 0; e < 4; ++e)
+                    if (i >= j + e) put_a(i, j + e, acc[q >> 1][q & 1][e] * scale);
+                continue;
+            }
+            H4 h, l;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                split16(acc[q >> 1][q & 1][e] * scale, h.h[e], l.h[e]);
+                *reinterpret_cast<_Float16*>(reg + (j + e) * N::AROW + i * 2) = h.h[e];
+                *reinterpret_cast<_Float16*>(reg + N::APLANE + (j + e) * N::AROW + i * 2) = l.h[e];
+            }
+            *reinterpret_cast<uint2*>(reg + i * N::AROW + j * 2) = h.u;
+            *reinterpret_cast<uint2*>(reg + N::APLANE + i * N::AROW + j * 2) = l.u;
         }
     }
     // A of the whole slab, for a matrix of one slab
@@ -1148,6 +1236,41 @@ template <int D> struct Slab {
         const int jn = min(W, r.n - j0), cols = r.turned ? r.d : jn, total = r.d * jn;
         int a = threadIdx.x / cols, c = threadIdx.x % cols;                    // output row (of this slab) and column
         const int da = NW_T / cols, dc = NW_T % cols, row0 = r.turned ? j0 : 0, col0 = r.turned ? 0 : j0;
+        if (r.ovec) {
+            constexpr int U = 4;
+            const int cols4 = cols / 4, total4 = total / 4, da4 = NW_T / cols4, dc4 = NW_T % cols4;
+            int a4 = threadIdx.x / cols4, c4 = threadIdx.x % cols4;
+            for (int e = threadIdx.x; e < total4; e += U * NW_T) {
+                f32x4_t v[U], w[U];
+                int64_t at[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const bool in = e + u * NW_T < total4;
+                    const int ra = in ? a4 : 0, rc = in ? c4 * 4 : 0;
+                    at[u] = (row0 + ra) * r.ldo + col0 + rc;
+                    if (p.muon) w[u] = *reinterpret_cast<const f32x4_t*>((const float*)r.o + at[u]);
+                    if (!r.turned) {
+                        const char* o = x + ra * xs + rc * 2;
+                        const uint2 h = *reinterpret_cast<const uint2*>(o), l = *reinterpret_cast<const uint2*>(o + xplane);
+                        v[u] = f32x4_t{__uint_as_float((h.x << 16) | (l.x & 0xffffu)), __uint_as_float((h.x & 0xffff0000u) | (l.x >> 16)),
+                                       __uint_as_float((h.y << 16) | (l.y & 0xffffu)), __uint_as_float((h.y & 0xffff0000u) | (l.y >> 16))};
+                    } else {
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            const char* o = x + (rc + q) * xs + ra * 2;
+                            v[u][q] = __uint_as_float(((uint32_t)*reinterpret_cast<const uint16_t*>(o) << 16) | *reinterpret_cast<const uint16_t*>(o + xplane));
+                        }
+                    }
+                    a4 += da4;
+                    c4 += dc4;
+                    if (c4 >= cols4) c4 -= cols4, ++a4;
+                }
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    if (e + u * NW_T < total4) put4(r, p, lr, at[u], v[u], w[u]);
+            }
+            return;
+        }
         constexpr int U = 8;
         for (int e = threadIdx.x; e < total; e += U * NW_T) {
             float v[U], w[U];
@@ -1276,7 +1399,7 @@ int group_of(int rows, int cols, int& W) {
     const int d = rows < cols ? rows : cols, n = rows < cols ? cols : rows, D = cdiv(d, 32);
     W = 0;
     if (d > 256) return 0;
-    if (D <= MAX_D && n <= W_MAX[D]) {                       // (66 x 256: 61 us against 85 with the chain; 60 x 300: 50 against 89)
+    if (D <= MAX_D && n <= W_MAX[D]) {                       // (66 x 256: 55 us against 85 with the chain; 60 x 300: 44 against 89)
         W = up(n, 32);
         return D;
     }
