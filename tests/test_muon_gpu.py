@@ -323,3 +323,38 @@ def test_outputs_side_by_side_and_outputs_that_overlap(ops):
     assert torch.equal(flat, keep) and (wide == 0).all()
     ops.muon_step([a, b], [gs[0], gs[0]], [torch.zeros_like(a), torch.zeros_like(a)], lr=0.1)      # (one gradient for two matrices is fine)
     assert not torch.equal(flat, keep)
+
+
+@pytest.mark.parametrize("shapes", [[(1100, 1030)] * 6, [(256, 256)] * 9 + [(900, 256)] * 4 + [(200, 410)] * 3 + [(700, 300), (260, 1500), (300, 300)], [(400, 2600), (2500, 500), (600, 600), (520, 300)]])
+def test_mixed_lists_on_a_dirty_workspace(ops, shapes):
+    """Large tiles in both products; lists of several lengths, which are not worked on in their order: still the bits of calls of their own."""
+    gs = [matrix(m, n, seed=i).cuda() for i, (m, n) in enumerate(shapes)]
+    torch.full((1 << 27,), float("nan"), device="cuda")
+    outs = ops.orthogonalize(gs)
+    again = ops.orthogonalize(gs[::-1])[::-1]
+    for i, g in enumerate(gs):
+        torch.full((1 << 27,), float("nan"), device="cuda")
+        assert torch.equal(outs[i], ops.orthogonalize(g)) and torch.equal(outs[i], again[i]), shapes[i]
+    small = min(range(len(shapes)), key=lambda i: shapes[i][0] * shapes[i][1])
+    check(outs[small], gs[small], f"{shapes[small]}")
+    check(outs[-1], gs[-1], f"{shapes[-1]}")
+
+
+def test_muon_step_takes_images_and_odd_alignment_of_narrow_matrices(ops):
+    """Whole vectors, single elements and bf16 images of narrow and ordinary matrices: the bits of the aligned update, and images = its rounding."""
+    for shape in ((24, 132), (132, 24), (66, 256), (31, 57), (260, 280)):
+        p, g, m = (matrix(*shape, seed=s).cuda() for s in range(3))
+        n = p.numel()
+        res = []
+        for off in (0, 1):                                                       # (1: nothing is 16-byte aligned)
+            bufs = [torch.zeros(n + 4, device="cuda")[off:off + n].view(shape) for _ in range(3)]
+            imgs = [torch.zeros(n + 4, dtype=torch.bfloat16, device="cuda")[off:off + n].view(shape) for _ in range(2)]
+            for b, t in zip(bufs, (p, g, m)):
+                b.copy_(t)
+            ops.muon_step([bufs[0]], [bufs[1]], [bufs[2]], lr=0.02, weight_decay=0.1, p_bf16=[imgs[0]], p_bf16_lo=[imgs[1]])
+            hi = bufs[0].bfloat16()
+            assert torch.equal(imgs[0], hi) and torch.equal(imgs[1], (bufs[0] - hi.float()).bfloat16())
+            res.append(bufs)
+        assert torch.equal(res[0][2], res[1][2])                                 # the momenta
+        d = (res[0][0].double() - res[1][0].double()).norm() / res[0][0].double().norm()
+        assert d <= 2.0 ** -22                                                   # (|u|_F summed in another order of 64-bit terms: one step of X_0's scale at most)
