@@ -20,7 +20,7 @@
 // A few groups of an image whose rows fit a workgroup's registers need ONE launch and one read (gna_fit_kernel below).
 // Nothing is accumulated with atomics: results do not depend on the order of workgroups.
 //
-// Measured: 8 x 19200 x 256 fp16 + GELU forward 52 us (1 17.9, 2 4.5, 3 32.6: 4.8 TB/s in 3, the rate of a large copy); the same in fp32,
+// Measured: 8 x 19200 x 256 fp16 + GELU forward 61 us, 51 with x still in the cache (1 17.9, 2 4.9, 3 32.7: 4.8 TB/s in 3); the same in fp32,
 // forward and backward, 250 us (31.7 + 5 + 54.9, 70.2 + 5.1 + 78.9: 5.7 and 6.0 TB/s in 3, what the cache kept included); 16 x 4800 x 256
 // bf16 + SiLU 23 us forward in one launch (3.4 TB/s: one workgroup of 1024 a CU, the load, the sums and the store one after the other).
 #include "common.cuh"
