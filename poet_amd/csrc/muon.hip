@@ -806,7 +806,7 @@ template <bool LAST> __global__ __launch_bounds__(NT, 2) void muon_update_split_
     leave_update<T, LAST>(p, r, b, i0, j0, part, v);
 }
 
-// ---- narrow matrices: d <= 128 ------------------------------------------------------------------------------------------------
+// ---- narrow matrices: d <= 96 ------------------------------------------------------------------------------------------------
 // The chain above costs 3 dependent launches a step whatever the size, ~6 us each with next to no work in them.  With few rows a
 // workgroup can hold everything that the step needs in LDS: q (dp x dp planes) and a SLAB of X's columns.  X' = q X stays inside a slab; only
 // A = X X^T couples the slabs, through dp x dp partial sums.
@@ -817,7 +817,7 @@ template <bool LAST> __global__ __launch_bounds__(NT, 2) void muon_update_split_
 // diagonal (each fragment read serves two tiles; a diagonal one reads its fragments once), the update in PAIRS of 16-column strips (each
 // fragment of q serves both), rewritten in place by the wave that owns them.  Rows of the LDS images are padded by 16 bytes: an odd number
 // of 16-byte pieces, so that the 16 rows of a fragment read start in different banks.
-constexpr int NW_T = 512, NWAVES = NW_T / 64, MAX_SLABS = 8, MAX_D = 4, MAX_SLAB_D = 2;
+constexpr int NW_T = 512, NWAVES = NW_T / 64, MAX_SLABS = 8, MAX_D = 3, MAX_SLAB_D = 2;
 template <int D> struct Narrow {
     static constexpr int DP = 32 * D, NM = D * (D + 1) / 2;
     static constexpr int PARTS = D == 1 ? 8 : D == 2 ? 2 : 1;             // few macro tiles: the columns in PARTS ranges, so that all waves have some
@@ -826,7 +826,7 @@ template <int D> struct Narrow {
     static constexpr int SCRATCH = PARTS > 1 ? ITEMS * 4096 : 0;
     static constexpr int REGION = 2 * APLANE > SCRATCH ? 2 * APLANE : SCRATCH;      // A / q planes, or partial tiles
 };
-constexpr int W_MAX[MAX_D + 1] = {0, 896, 512, 288, 160};       // columns that leave room for REGION in 160 KB
+constexpr int W_MAX[MAX_D + 1] = {0, 896, 512, 288};       // columns that leave room for REGION in 160 KB
 struct NarrowP {
     StageP s;
     int mode, k, steps;                              // N_*; this launch's step
@@ -1304,11 +1304,15 @@ template <int D> struct Slab {
     }
 };
 
+// the records of a long list of them
+__global__ __launch_bounds__(NT) void muon_table_kernel(Rec* table, int count, const Recs recs) {
+    for (int i = threadIdx.x; i < count * (int)(sizeof(Rec) / 4); i += NT) ((uint32_t*)table)[i] = ((const uint32_t*)recs.r)[i];
+}
 // one matrix per workgroup, start to end
 template <int D> __global__ __launch_bounds__(NW_T, 2) void muon_narrow_kernel(const NarrowP p, const Recs recs) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     __shared__ double red[NWAVES];
-    const Rec& r = recs.r[blockIdx.x];
+    const Rec r = p.s.table ? p.s.table[blockIdx.x] : recs.r[blockIdx.x];
     const StageP& sp = p.s;
     const Slab<D> L(smem, r.W);
     double s = L.template load<true>(r, sp, grad_scale_of(sp.gscale, sp.sqnorm, sp.max_norm), 0);
@@ -1399,12 +1403,12 @@ int group_of(int rows, int cols, int& W) {
     const int d = rows < cols ? rows : cols, n = rows < cols ? cols : rows, D = cdiv(d, 32);
     W = 0;
     if (d > 256) return 0;
-    if (D <= MAX_D && n <= W_MAX[D]) {                       // (66 x 256: 55 us against 85 with the chain; 60 x 300: 44 against 89)
+    if (D <= MAX_D && n <= W_MAX[D]) {                       // (66 x 256: 55 us against 70 with the chain; 60 x 300: 44 against 72; 120 x 150 would take 80 against 72)
         W = up(n, 32);
         return D;
     }
-    // slabs of 256 columns (at most 8, wider then): 20 x 2000: 73 us against 143 with the chain, 60 x 1500: 106 against 120; with three tiles of
-    // rows and more the chain wins (90 x 400: 96 against 81, 131 x 257: 115 against 81)
+    // slabs of 256 columns (at most 8, wider then): 20 x 2000: 47 us against 123 with the chain, four 60 x 1500: 73 against 119; with three tiles
+    // of rows and more the chain wins (90 x 400: 96 against 78, 131 x 257: 115 against 79)
     if (D > MAX_SLAB_D || n > MAX_SLABS * W_MAX[D]) return SMALL;
     const int slabs = cdiv(n, 256) < MAX_SLABS ? cdiv(n, 256) : MAX_SLABS;
     W = up(cdiv(n, slabs), 32);
@@ -1498,7 +1502,8 @@ int layout(const int* rows, const int* cols, const int* order, int first, int n,
     L.part = (L.firsts + (int64_t)count * GRIDS * 4 + 15) / 16 * 16;
     L.planes = (L.part + parts * 8 + 255) / 256 * 256;
     L.total = (L.planes + planes * 2 + 255) / 256 * 256;
-    if (group > 0 && group <= MAX_D) L.total = 0;            // (all in LDS)
+    if (group > 0 && group <= MAX_D) L.total = count > CHUNK ? L.firsts : 0;      // (all in LDS; the table of a long list)
+    L.total = (L.total + 255) / 256 * 256;
     return i;
 }
 
@@ -1662,7 +1667,7 @@ NarrowP narrow_params(const Layout& L, const Job& j, const Steps& S, char* ws) {
     return p;
 }
 template <int D> int narrow_lds(int W) { return Narrow<D>::REGION + 2 * Narrow<D>::DP * (W * 2 + 16); }
-template <int D> void narrow_single(const NarrowP& p, const Recs& recs, int count, int W, hipStream_t st) {
+template <int D> void narrow_single(const NarrowP& p, const Recs& recs, int count, int W, hipStream_t st) {       // records: recs, or p.s.table
     static unsigned long long done = 0;
     static_assert(Narrow<D>::REGION + 2 * Narrow<D>::DP * (W_MAX[D] * 2 + 16) + 256 <= 160 * 1024, "LDS");
     lds_attr_once((const void*)muon_narrow_kernel<D>, narrow_lds<D>(W_MAX[D]), done);
@@ -1725,7 +1730,8 @@ int run_job(const char* what, const Job& j, void* ws, int64_t ws_bytes, void* st
         np.n = L.count;
         np.g_dtype = j.g_dtype; np.muon = j.muon; np.nesterov = j.nesterov;
         np.mu = (float)j.mu; np.omu = (float)(1.0 - j.mu); np.gscale = j.gscale; np.max_norm = j.max_norm; np.sqnorm = j.sqnorm;
-        const NarrowP narrow = narrow_params(L, j, S, base);
+        NarrowP narrow = narrow_params(L, j, S, base);
+        Recs short_list = {};
         int64_t planes = 0;                                   // of the chunks before this one
         int parts = 0, tiles[GRIDS] = {0, 0, 0};
         Rec shape = {};
@@ -1761,16 +1767,19 @@ int run_job(const char* what, const Job& j, void* ws, int64_t ws_bytes, void* st
             }
             np.count = C.count;
             if (!single) hipLaunchKernelGGL(muon_norm_kernel, dim3(blocks), dim3(NT), 0, st, np, recs);
-            else if (group == 1) narrow_single<1>(narrow, recs, C.count, C.maxW, st);
-            else if (group == 2) narrow_single<2>(narrow, recs, C.count, C.maxW, st);
-            else if (group == 3) narrow_single<3>(narrow, recs, C.count, C.maxW, st);
-            else narrow_single<4>(narrow, recs, C.count, C.maxW, st);
+            else if (L.count > CHUNK) hipLaunchKernelGGL(muon_table_kernel, dim3(1), dim3(NT), 0, st, np.table + np.first, C.count, recs);
+            else short_list = recs;
             planes += C.plane_elems;
             parts += C.parts;
             for (int k = 0; k < GRIDS; ++k) tiles[k] += C.tiles[k];
             np.first += C.count;
         }
-        if (group == 0) chain(T.large, false, shape, one_shape, L, j, S, base, st);
+        if (single) {                                         // (a hundred 66 x 256: 5 launches of 24 one after the other 258 us, 68 with the table)
+            if (L.count <= CHUNK) narrow.s.table = nullptr;
+            if (group == 1) narrow_single<1>(narrow, short_list, L.count, L.maxW, st);
+            else if (group == 2) narrow_single<2>(narrow, short_list, L.count, L.maxW, st);
+            else narrow_single<3>(narrow, short_list, L.count, L.maxW, st);
+        } else if (group == 0) chain(T.large, false, shape, one_shape, L, j, S, base, st);
         else if (group == SMALL) chain(T.small, true, shape, one_shape, L, j, S, base, st);
         else if (group == MAX_D + 1) narrow_slabs<1>(narrow, L, st);
         else if (group == MAX_D + 2) narrow_slabs<2>(narrow, L, st);

@@ -358,3 +358,25 @@ def test_muon_step_takes_images_and_odd_alignment_of_narrow_matrices(ops):
         assert torch.equal(res[0][2], res[1][2])                                 # the momenta
         d = (res[0][0].double() - res[1][0].double()).norm() / res[0][0].double().norm()
         assert d <= 2.0 ** -22                                                   # (|u|_F summed in another order of 64-bit terms: one step of X_0's scale at most)
+
+
+def test_long_lists_of_narrow_matrices(ops):
+    """More narrow matrices than a launch takes by value: the bits of calls of their own, also in place and for the update."""
+    shapes = [(20, 100), (7, 33), (90, 64), (50, 60), (1, 1)] * 30
+    gs = [matrix(m, n, seed=i).cuda() for i, (m, n) in enumerate(shapes)]
+    outs = ops.orthogonalize(gs)
+    for i, (g, o) in enumerate(zip(gs, outs)):
+        if i < 5 or i >= 145:
+            check(o, g, f"{shapes[i]}")
+        assert torch.equal(o, ops.orthogonalize(g)), shapes[i]
+    ps, ms = [matrix(m, n, seed=500 + i).cuda() for i, (m, n) in enumerate(shapes)], [torch.zeros_like(g) for g in gs]
+    p1, m1 = [p.clone() for p in ps], [m.clone() for m in ms]
+    ops.muon_step(ps, gs, ms, lr=0.1)
+    for i in range(0, 150, 7):
+        ops.muon_step([p1[i]], [gs[i]], [m1[i]], lr=0.1)
+        assert torch.equal(ps[i], p1[i]) and torch.equal(ms[i], m1[i]), shapes[i]
+    same = torch.stack([matrix(24, 40, seed=i) for i in range(70)]).cuda()
+    want = ops.orthogonalize(same)
+    assert torch.equal(want[69], ops.orthogonalize(same[69]))
+    ops.orthogonalize(same, out=same)
+    assert torch.equal(same, want)
