@@ -260,21 +260,28 @@ __global__ __launch_bounds__(NT) void muon_pack_kernel(const StageP p) {
                 else vec<f16_t, 4>::ld((const f16_t*)r.g + i, v[k]);
             }
         }
-    } else {
+    } else {                                                          // (behind an edge: the last element again, so that all loads are in flight)
+        auto at = [&](int k, int e) { return min(sr + q0 + 16 * k, r.rows - 1) * r.ldg + min(sc + c4 + e, r.cols - 1); };
+        auto all = [&](auto&& fetch) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
+            for (int k = 0; k < 4; ++k)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int row = sr + q0 + 16 * k, col = sc + c4 + e;
-                v[k][e] = 0.f;
-                if (row < r.rows && col < r.cols) {
-                    if (p.muon) {
-                        const int64_t i = (int64_t)row * r.cols + col;
-                        const float m = r.mom[i];
-                        v[k][e] = p.nesterov ? fmaf(p.mu, m, p.omu * (((const float*)r.g)[i] * gs)) : m;
-                    } else v[k][e] = ld_any(r.g, row * r.ldg + col, p.g_dtype);
-                }
-            }
+                for (int e = 0; e < 4; ++e) v[k][e] = fetch(at(k, e));
+        };
+        if (p.muon) {
+            float m[4][4];
+            all([&](int64_t i) { return ((const float*)r.g)[i]; });
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) m[k][e] = r.mom[at(k, e)];
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[k][e] = p.nesterov ? fmaf(p.mu, m[k][e], p.omu * (v[k][e] * gs)) : m[k][e];
+        } else if (p.g_dtype == POET_F32) all([&](int64_t i) { return ld1<float>(r.g, i); });
+        else if (p.g_dtype == POET_BF16) all([&](int64_t i) { return ld1<bf16_t>(r.g, i); });
+        else all([&](int64_t i) { return ld1<f16_t>(r.g, i); });
     }
 #pragma unroll
     for (int k = 0; k < 4; ++k)
