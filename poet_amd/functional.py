@@ -670,7 +670,7 @@ class GroupNormActFn(torch.autograd.Function):
     def forward(ctx, x, w, b, groups, act, eps):
         y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
         stats = torch.empty((x.shape[0], groups, 2), dtype=torch.float32, device=x.device)
-        ops.groupnorm_act_fwd(x, w, b, y, groups, act, stats, eps)
+        ops.groupnorm_act_fwd(x, w, b, y, groups, act, stats, eps, fresh=True)
         ctx.save_for_backward(x, stats, w, b)
         ctx.params, ctx.cfg = (w, b), (groups, act)
         return y
@@ -685,16 +685,16 @@ class GroupNormActFn(torch.autograd.Function):
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
         if not (need_w or need_b):
-            ops.groupnorm_act_bwd(dy, x, stats, w, b, groups, act, dx)
+            ops.groupnorm_act_bwd(dy, x, stats, w, b, groups, act, dx, fresh=True)
             return dx, None, None, None, None, None
         pw, pb = ctx.params
         dw, db = getattr(pw, "_grad_view", None), getattr(pb, "_grad_view", None)
         if dw is not None and db is not None:
-            ops.groupnorm_act_bwd(dy, x, stats, w, b, groups, act, dx, dw, db, True)
+            ops.groupnorm_act_bwd(dy, x, stats, w, b, groups, act, dx, dw, db, True, fresh=True)
             return dx, None, None, None, None, None
-        dw, db = torch.empty((2, w.numel()), dtype=torch.float32, device=x.device).unbind(0)
-        ops.groupnorm_act_bwd(dy, x, stats, w, b, groups, act, dx, dw, db)
-        return dx, dw.view(w.shape) if need_w else None, db.view(b.shape) if need_b else None, None, None, None
+        dw, db = torch.empty(w.shape, dtype=torch.float32, device=x.device), torch.empty(b.shape, dtype=torch.float32, device=x.device)
+        ops.groupnorm_act_bwd(dy, x, stats, w, b, groups, act, dx, dw, db, fresh=True)
+        return dx, dw if need_w else None, db if need_b else None, None, None, None
 
 
 def group_norm_act(x, weight, bias, groups, act="none", eps=1e-5):
@@ -711,7 +711,7 @@ def group_norm_act(x, weight, bias, groups, act="none", eps=1e-5):
         y = GroupNormActFn.apply(x3, weight, bias, int(groups), act, float(eps))
     else:
         y = torch.empty(x3.shape, dtype=x.dtype, device=x.device)
-        ops.groupnorm_act_fwd(x3, weight, bias, y, int(groups), act, None, float(eps))
+        ops.groupnorm_act_fwd(x3, weight, bias, y, int(groups), act, None, float(eps), fresh=True)
     return y if nd == 3 else y.view(x.shape)
 
 

@@ -619,18 +619,21 @@ def _gna_ws(N, HW, C, G):
     return n
 
 
-def groupnorm_act_fwd(x, gamma, beta, y, G, act="none", stats=None, eps=1e-5):
+def groupnorm_act_fwd(x, gamma, beta, y, G, act="none", stats=None, eps=1e-5, fresh=False):
     """y = act(gamma (x - mean) rstd + beta), statistics over the rows and the C / G channels of each (image, group).  x, y (N, HW, C) with
     contiguous channels, any image / row strides (a level's rows of a token buffer); types: equal (fp32, bf16, fp16), or fp32 with bf16.
-    stats: optional (N, G, 2) fp32 output (mean, rstd), what groupnorm_act_bwd reads.  y may be x."""
+    stats: optional (N, G, 2) fp32 output (mean, rstd), what groupnorm_act_bwd reads.  y may be x.  fresh: y (and stats) were allocated for this
+    call, contiguous on x's device, and need no checks."""
     dev, N, HW, C, a = _gna_args(x, (gamma, beta), G, act)
-    (xn, xr), (yn, yr) = _rows3(x, "x", N, HW, C), _rows3(y, "y", N, HW, C, out=True)
+    xn, xr = _rows3(x, "x", N, HW, C)
+    yn, yr = (HW * C, C) if fresh else _rows3(y, "y", N, HW, C, out=True)
     xd, yd = dcode(x), dcode(y)
-    if y.device != dev or stats is not None and not (stats.device == dev and stats.dtype is torch.float32 and stats.is_contiguous() and stats.numel() == 2 * N * G):
+    if not fresh and (y.device != dev or stats is not None and not (stats.device == dev and stats.dtype is torch.float32 and stats.is_contiguous() and stats.numel() == 2 * N * G)):
         raise ValueError("poet_amd: y and stats must live on x's device, stats as a contiguous fp32 (N, G, 2) tensor")
     if N == 0 or HW == 0:
         return y
-    _apart(x, xn, xr, y, yn, yr, N, HW, C, "y")
+    if not fresh:
+        _apart(x, xn, xr, y, yn, yr, N, HW, C, "y")
     with _on_device(dev) as stream:
         n = _gna_ws(N, HW, C, G)
         ws = torch.empty(n, dtype=torch.uint8, device=dev)
@@ -641,13 +644,14 @@ def groupnorm_act_fwd(x, gamma, beta, y, G, act="none", stats=None, eps=1e-5):
     return y
 
 
-def groupnorm_act_bwd(dy, x, stats, gamma, beta, G, act="none", dx=None, dgamma=None, dbeta=None, accumulate=False):
+def groupnorm_act_bwd(dy, x, stats, gamma, beta, G, act="none", dx=None, dgamma=None, dbeta=None, accumulate=False, fresh=False):
     """Gradients of groupnorm_act_fwd from its input and stats (z is recomputed): dx in x's type, dgamma / dbeta fp32, overwritten or
-    (accumulate) added to.  Any of them may be left out (dgamma and dbeta together); dx may be x or dy."""
+    (accumulate) added to.  Any of them may be left out (dgamma and dbeta together); dx may be x or dy.
+    fresh: dx was allocated for this call, contiguous, of x's type and on its device, and needs no checks."""
     dev, N, HW, C, a = _gna_args(x, (gamma, beta, dgamma, dbeta), G, act)
     (xn, xr), (dn, dr) = _rows3(x, "x", N, HW, C), _rows3(dy, "dy", N, HW, C)
-    on, orow = (0, 0) if dx is None else _rows3(dx, "dx", N, HW, C, out=True)
-    if dx is not None and (dx.dtype != x.dtype or dx.device != dev) or dy.device != dev:
+    on, orow = (0, 0) if dx is None else (HW * C, C) if fresh else _rows3(dx, "dx", N, HW, C, out=True)
+    if dx is not None and not fresh and (dx.dtype != x.dtype or dx.device != dev) or dy.device != dev:
         raise ValueError("poet_amd: dx has x's type, and dy, dx live on x's device")
     if not (stats.dtype is torch.float32 and stats.device == dev and stats.is_contiguous() and stats.numel() == 2 * N * G):
         raise ValueError("poet_amd: stats must be the contiguous fp32 (N, G, 2) tensor of the forward pass")
@@ -658,7 +662,7 @@ def groupnorm_act_bwd(dy, x, stats, gamma, beta, G, act="none", dx=None, dgamma=
         if dgamma is not None and not accumulate:
             dgamma.zero_(), dbeta.zero_()
         return dx, dgamma, dbeta
-    if dx is not None:
+    if dx is not None and not fresh:
         _apart(x, xn, xr, dx, on, orow, N, HW, C, "dx")
         _apart(dy, dn, dr, dx, on, orow, N, HW, C, "dx")
     with _on_device(dev) as stream:
