@@ -12,7 +12,9 @@
 // finds its chunk where the first left it: in the L2 of its XCD or in the memory-side cache):
 //   1. partial sums of the chunk.  Forward: (mean, M2) per group -- a lane accumulates x - p and (x - p)^2 against its OWN first
 //      sample p of the channel (with n <= 64 samples per lane sum (x-p)^2 <= (n + 1) M2, so a lane loses at most n ulp whatever the
-//      mean / spread ratio or outliers are) and lanes / channels / chunks combine by the parallel-variance formula.
+//      mean / spread ratio or outliers are) and lanes / channels / chunks combine by the parallel-variance formula.  A sum at the magnitude of
+//      n mean is rounded by ulps of the mean, which 1 / sqrt(eps) shows where a group is constant: the mean is that sum / n, and then the
+//      mean of the deviations from it (a constant group comes out exactly beta).
 //      Backward: sum dz and sum dz h per channel, and their gamma-weighted sums per group.
 //   2. a wave per (image, group) folds the chunks' partials (4 .. 5 us; every workgroup of 3 folding for itself took longer: a few KB of
 //      dependent loads at the head of each of ~1000 workgroups).
@@ -220,21 +222,30 @@ template <typename TX, int V> __global__ __launch_bounds__(NT) void gna_stats_ke
         }
     }
     const float fc = (float)cnt, rc = cnt ? 1.f / fc : 0.f;
-    float w[V];
+    float w[V], d[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) w[i] = fmaf(fc, pv[i], S[i]);
     to_channels<V>(k, w, red, chan);
     to_groups(k, chan, grp);
-    const float inv = 1.f / ((float)(k.row1 - k.row0) * (float)k.cps);
+    const float n = (float)(k.row1 - k.row0) * (float)k.cps, inv = 1.f / n;
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-        const float d = k.active ? fmaf(S[i], rc, pv[i]) - grp[(k.l * V + i) / k.cps] * inv : 0.f;
-        w[i] = fmaf(-S[i] * rc, S[i], Q[i]) + fc * d * d;
+    for (int i = 0; i < V; ++i) {                          // about grp inv, some ulps off the mean
+        d[i] = k.active ? pv[i] - grp[(k.l * V + i) / k.cps] * inv : 0.f;
+        w[i] = fmaf(fc, d[i], S[i]);
     }
     to_channels<V>(k, w, red, chan);
     to_groups(k, chan, grp2);
-    for (int g = threadIdx.x; g < k.ng; g += NT)
-        p.part[(((int64_t)k.n * p.G + k.g0 + g) * p.T + k.t) * p.P + k.piece] = make_float2(grp[g] * inv, fmaxf(grp2[g], 0.f));
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        d[i] = fmaf(S[i], rc, d[i]);
+        w[i] = fmaf(-S[i] * rc, S[i], Q[i]) + fc * d[i] * d[i];
+    }
+    to_channels<V>(k, w, red, chan);
+    to_groups(k, chan, red);
+    for (int g = threadIdx.x; g < k.ng; g += NT) {
+        const float c = grp2[g] / n;
+        p.part[(((int64_t)k.n * p.G + k.g0 + g) * p.T + k.t) * p.P + k.piece] = make_float2(fmaf(grp[g], inv, c), fmaxf(fmaf(-grp2[g], c, red[g]), 0.f));
+    }
 }
 
 // ---- forward, 2: fold the chunks, normalise, activate ----------------------------------------------------
@@ -454,20 +465,26 @@ template <typename T> struct Raw<T, 1> {
     __device__ __forceinline__ void ld(const T* p) { w = io<T>::ld(p); }
     __device__ __forceinline__ void get(float* o) const { o[0] = w; }
 };
-// sum of v over the workgroup's threads that share this thread's group (lanes lg * g .. of every LPR): lg and LPR powers of two up to 64, or
-// one group for the whole workgroup
-template <int BT> __device__ __forceinline__ float group_sum(float v, float* sh, int lg, int LPR, bool one, int grp) {
+// sums of v over the workgroup's threads that share this thread's group (lanes lg * g .. of every LPR): lg and LPR powers of two up to 64, or
+// one group for the whole workgroup.  sh: K BT floats.
+template <int BT, int K> __device__ __forceinline__ void group_sums(float (&v)[K], float* sh, int lg, int LPR, bool one, int grp) {
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1)
-        if (one || o < lg || o >= LPR) v += __shfl_xor(v, o, 64);
+        if (one || o < lg || o >= LPR)
+#pragma unroll
+            for (int q = 0; q < K; ++q) v[q] += __shfl_xor(v[q], o, 64);
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     __syncthreads();
-    if (one ? lane == 0 : lane < LPR && (lane & (lg - 1)) == 0) sh[wave * 64 + (one ? 0 : lane / lg)] = v;
-    __syncthreads();
-    float s = 0.f;
+    if (one ? lane == 0 : lane < LPR && (lane & (lg - 1)) == 0)
 #pragma unroll
-    for (int w = 0; w < BT / 64; ++w) s += sh[w * 64 + grp];
-    return s;
+        for (int q = 0; q < K; ++q) sh[q * BT + wave * 64 + (one ? 0 : lane / lg)] = v[q];
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < K; ++q) {
+        v[q] = 0.f;
+#pragma unroll
+        for (int w = 0; w < BT / 64; ++w) v[q] += sh[q * BT + w * 64 + grp];
+    }
 }
 struct Fit {                            // where this thread works
     int n, g0, c, grp, l, r, LPR, RP, lg;
@@ -493,11 +510,11 @@ template <int BT, int V> __device__ __forceinline__ Fit fit_of(const GnaP& p) {
 }
 
 template <typename TX, int V, int BT, int NR> __global__ __launch_bounds__(BT) void gna_fit_kernel(const GnaP p) {
-    __shared__ float sh[BT / 64 * 64];
+    __shared__ float sh[2 * BT];
     const Fit f = fit_of<BT, V>(p);
     const TX* x = (const TX*)p.x + f.n * p.xn + f.c;
     Raw<TX, V> raw[NR];
-    float s = 0.f, first = 0.f;                            // (sums against the thread's first value: a mean far from 0 costs no digits)
+    float s[2] = {0.f, 0.f}, first = 0.f;                  // (sums against the thread's first value)
     const int rows = f.active ? p.HW : 0;
 #pragma unroll
     for (int u = 0; u < NR; ++u)
@@ -511,21 +528,27 @@ template <typename TX, int V, int BT, int NR> __global__ __launch_bounds__(BT) v
             if (u == 0) first = v[0];
             cnt += V;
 #pragma unroll
-            for (int i = 0; i < V; ++i) s += v[i] - first;
+            for (int i = 0; i < V; ++i) s[0] += v[i] - first;
         }
-    s = fmaf((float)cnt, first, s);
-    const float inv = 1.f / ((float)p.HW * (float)p.cpg);
-    const float mean = group_sum<BT>(s, sh, f.lg, f.LPR, f.one, f.grp) * inv;
-    s = 0.f;
+    const float n = (float)p.HW * (float)p.cpg;
+    float about[1] = {fmaf((float)cnt, first, s[0])};
+    group_sums<BT>(about, sh, f.lg, f.LPR, f.one, f.grp);
+    about[0] /= n;                                         // some ulps off the mean: the deviations from it say how many
+    s[0] = 0.f;
 #pragma unroll
     for (int u = 0; u < NR; ++u)
         if (f.r + u * f.RP < rows) {
             float v[V];
             raw[u].get(v);
 #pragma unroll
-            for (int i = 0; i < V; ++i) s = fmaf(v[i] - mean, v[i] - mean, s);
+            for (int i = 0; i < V; ++i) {
+                const float d = v[i] - about[0];
+                s[0] += d;
+                s[1] = fmaf(d, d, s[1]);
+            }
         }
-    const float rstd = 1.f / sqrtf(group_sum<BT>(s, sh, f.lg, f.LPR, f.one, f.grp) * inv + p.eps);
+    group_sums<BT>(s, sh, f.lg, f.LPR, f.one, f.grp);
+    const float c = s[0] / n, mean = about[0] + c, rstd = 1.f / sqrtf(fmaxf(fmaf(-s[0], c, s[1]), 0.f) / n + p.eps);
     if (p.stats && f.r == 0 && f.l % f.lg == 0) *reinterpret_cast<float2*>(p.stats + 2 * ((int64_t)f.n * p.G + f.g0 + f.grp)) = make_float2(mean, rstd);
     if (!f.active) return;
     float sc[V], b[V];
