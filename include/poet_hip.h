@@ -386,6 +386,7 @@ int poet_groupnorm_bwd(const void* dy, const void* x, const float* stats, const 
 
 /* GroupNorm with an activation on channels-last rows: x (N, HW, C) at image / row strides x_n / x_r (elements, channels contiguous),
  * y likewise.  y = act(gamma h + beta), h = (x - mean) rstd over the HW x (C / G) values of (image, group); any C / G.
+ * A group with a NaN, an infinity, or squared deviations whose sum leaves fp32 comes out NaN, the others are untouched by it.
  * act: POET_ACT_*.  Types of (x, y): (fp32, fp32), (bf16, bf16), (fp16, fp16), (bf16, fp32), (fp32, bf16); gamma / beta fp32 (C).
  * stats (N, G, 2) fp32 = (mean, rstd): written by forward (optional there), read by backward, 8-byte aligned.
  * y may be x itself, dx may be x or dy (no other overlap).  Backward recomputes z = gamma h + beta: dx (optional; x's type) and dgamma / dbeta

@@ -103,6 +103,12 @@ template <int ACT> __device__ __forceinline__ float act_df(float z, float dy) { 
     return dy;
 }
 
+// ---- statistics -----------------------------------------------------------------------------------------
+__device__ __forceinline__ float not_below_zero(float v) { return v < 0.f ? 0.f : v; }                 // (a NaN stays one)
+// Sums of squares beyond fp32 (deviations from 1.8e19 / sqrt(n) on) are infinite, or infinity - infinity: such a group comes out NaN, like one that
+// holds an infinity, not finite and wrong.
+__device__ __forceinline__ float rstd_of(float var, float eps) { return var < INFINITY ? 1.f / sqrtf(var + eps) : NAN; }
+
 // ---- this workgroup's chunk and slab ------------------------------------------------------------------
 struct Blk {
     int n, t, s, row0, row1;          // image, chunk, slab; rows [row0, row1)
@@ -244,7 +250,7 @@ template <typename TX, int V> __global__ __launch_bounds__(NT) void gna_stats_ke
     to_groups(k, chan, red);
     for (int g = threadIdx.x; g < k.ng; g += NT) {
         const float c = grp2[g] / n;
-        p.part[(((int64_t)k.n * p.G + k.g0 + g) * p.T + k.t) * p.P + k.piece] = make_float2(fmaf(grp[g], inv, c), fmaxf(fmaf(-grp2[g], c, red[g]), 0.f));
+        p.part[(((int64_t)k.n * p.G + k.g0 + g) * p.T + k.t) * p.P + k.piece] = make_float2(fmaf(grp[g], inv, c), not_below_zero(fmaf(-grp2[g], c, red[g])));
     }
 }
 
@@ -300,7 +306,7 @@ template <bool BWD> __global__ __launch_bounds__(NT) void gna_fold_kernel(const 
             q += fmaf(weight(i) * d, d, e[i].y);
         }
         q = team_sum(q, 64);
-        if (lane == 0) p.folded[ng] = make_float2(mean, 1.f / sqrtf(q / total + p.eps));
+        if (lane == 0) p.folded[ng] = make_float2(mean, rstd_of(q / total, p.eps));
     }
 }
 
@@ -548,7 +554,7 @@ template <typename TX, int V, int BT, int NR> __global__ __launch_bounds__(BT) v
             }
         }
     group_sums<BT>(s, sh, f.lg, f.LPR, f.one, f.grp);
-    const float c = s[0] / n, mean = about[0] + c, rstd = 1.f / sqrtf(fmaxf(fmaf(-s[0], c, s[1]), 0.f) / n + p.eps);
+    const float c = s[0] / n, mean = about[0] + c, rstd = rstd_of(not_below_zero(fmaf(-s[0], c, s[1])) / n, p.eps);
     if (p.stats && f.r == 0 && f.l % f.lg == 0) *reinterpret_cast<float2*>(p.stats + 2 * ((int64_t)f.n * p.G + f.g0 + f.grp)) = make_float2(mean, rstd);
     if (!f.active) return;
     float sc[V], b[V];

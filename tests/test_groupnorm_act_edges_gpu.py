@@ -47,3 +47,24 @@ def test_a_far_mean_with_a_small_spread(ops):
         want = 2.0 ** -9 / (2.0 ** -18 + 1e-5) ** 0.5
         # (rstd: the variance's sums of n equal squares, eps and the root, a few roundings of 2^-24; the deviation itself is exact)
         assert (y.double().abs() - want).abs().max() <= 16 * 2.0 ** -24 * want
+
+
+@pytest.mark.parametrize("HW", [40, 900, 20000])
+@pytest.mark.parametrize("size", [1e20, 1e25, 1e37])
+def test_squares_beyond_fp32_are_not_finite(ops, HW, size):
+    """Deviations whose squares leave fp32: the variance is not representable, so the group comes out NaN, never finite and wrong; the other groups
+    and images are untouched.  Deviations of 1e15 (sums of squares to 1e36) stay in range."""
+    x, w, b, _ = make(2, HW, 64, torch.float32, seed=HW)
+    clean, big = torch.empty_like(x), x.clone()
+    ops.groupnorm_act_fwd(x, w, b, clean, 8, "silu")
+    big[1, :, 8:16] *= size
+    y, stats = torch.empty_like(x), torch.empty(2, 8, 2, device="cuda")
+    ops.groupnorm_act_fwd(big, w, b, y, 8, "silu", stats=stats)
+    assert torch.isnan(y[1, :, 8:16]).all() and torch.isnan(stats[1, 1, 1])
+    keep = torch.ones(2, 1, 64, dtype=torch.bool, device="cuda").expand(2, HW, 64).clone()
+    keep[1, :, 8:16] = False
+    assert torch.equal(y[keep], clean[keep])
+    big[1, :, 8:16] = x[1, :, 8:16] * 1e15
+    ops.groupnorm_act_fwd(big, w, b, y, 8, "silu")
+    r = ref(big, w, b, 8, "silu", 1e-5)
+    check(y, r["y"], r["tol_y"], "deviations of 1e15")
