@@ -699,8 +699,9 @@ class GroupNormActFn(torch.autograd.Function):
 
 def group_norm_act(x, weight, bias, groups, act="none", eps=1e-5):
     """act(group_norm(x)) for channels-last x (N, ..., C) in fp32, bf16 or fp16; fp32 weight / bias (C).  act: "none", "relu", "gelu" (erf),
-    "silu".  Differentiable once in x, weight and bias; the result has x's type.  Rows may be strided (a slice of a token buffer); x is
-    copied only when its channels are not contiguous or its middle dimensions do not merge."""
+    "silu".  Differentiable once in x, weight and bias, in backward mode (forward-mode tangents are refused); the result has x's type.  Rows
+    may be strided (a slice of a token buffer); x is copied only when its channels are not contiguous or its middle dimensions do not merge."""
+    ops._no_tangent("group_norm_act", x, weight, bias)
     nd = x.dim()
     if nd < 2:
         raise ValueError(f"poet_amd: x must be (N, ..., C), got {tuple(x.shape)}")

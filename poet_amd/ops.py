@@ -8,6 +8,7 @@ import os
 from typing import Optional, Sequence
 
 import torch
+from torch.autograd import forward_ad as _forward_ad
 
 from . import _lib
 from ._lib import BF16, F32, GemmDesc
@@ -532,6 +533,12 @@ ACT = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}          # POET_ACT_*
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+
+
+def _no_tangent(what, *tensors):
+    """Refuses forward-mode differentiation: a result computed here would lose the tangent without a word."""
+    if _forward_ad._current_level >= 0 and any(_forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"poet_amd: {what} has no forward-mode derivative (pass tensors without tangents)")
 
 
 class _on_device:

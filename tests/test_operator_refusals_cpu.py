@@ -1,0 +1,23 @@
+"""What the GroupNorm + activation and orthogonalisation operators refuse before they look at a device."""
+import pytest
+import torch
+import torch.autograd.forward_ad as fwd
+
+
+@pytest.mark.parametrize("which", [0, 1, 2])
+@pytest.mark.parametrize("grad", [True, False])
+def test_group_norm_act_refuses_forward_mode_tangents(which, grad):
+    """A tangent on x, weight or bias is refused (with gradients on and off: no_grad does not switch forward mode off); inside a dual level, tensors
+    without one go on to the ordinary checks."""
+    from poet_amd import GroupNormAct, PoetHipError, functional
+    args = [torch.randn(2, 5, 8), torch.ones(8), torch.zeros(8)]
+    with fwd.dual_level(), torch.set_grad_enabled(grad):
+        dual = list(args)
+        dual[which] = fwd.make_dual(args[which], torch.ones_like(args[which]))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            functional.group_norm_act(*dual, 2, act="silu")
+        with pytest.raises(PoetHipError):                   # (no GPU path for CPU tensors)
+            functional.group_norm_act(*args, 2, act="silu")
+    if which == 0:
+        with fwd.dual_level(), pytest.raises(NotImplementedError, match="forward-mode"):
+            GroupNormAct(2, 8)(fwd.make_dual(args[0], args[0]))
