@@ -1013,7 +1013,8 @@ def orthogonalize(g, out=None, steps=5, coeffs=NS_COEFFS, eps=1e-7):
     side).  g: a tensor (..., m, n), or a list of 2-D tensors of any shapes, one type (fp32, bf16, fp16) and device; the result has g's
     form and type (or goes to `out`, which may be g).  coeffs: (a, b, c), or one such triple per step.  Products carry 22-bit operands
     and fp32 sums.  The matrices of a call are worked on together (the narrow ones, those with up to 256 rows or columns and the others
-    each in one chain of launches), so a list costs little more than its longest chains; a matrix's result does not depend on the list."""
+    each in one chain of launches), so a list costs little more than its longest chains; a matrix's result does not depend on the list.
+    Not differentiable: input that asks for a gradient (requires_grad while gradients are on, a forward-mode tangent) is refused -- detach it."""
     single = torch.is_tensor(g)
     if single and g.dim() < 2:
         raise ValueError(f"poet_amd: g must be (..., m, n), got {tuple(g.shape)}")
@@ -1021,6 +1022,9 @@ def orthogonalize(g, out=None, steps=5, coeffs=NS_COEFFS, eps=1e-7):
         g = list(g)
         if any(t.dim() != 2 for t in g):
             raise ValueError("poet_amd: the tensors of a list are 2-D")
+    _no_tangent("orthogonalize", *([g] if single else g))
+    if torch.is_grad_enabled() and (g.requires_grad if single else any(t.requires_grad for t in g)):
+        raise NotImplementedError("poet_amd: orthogonalize has no gradient (pass g.detach())")
     given = out is not None
     if not given:
         out = torch.empty(g.shape, dtype=g.dtype, device=g.device) if single else [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in g]

@@ -21,3 +21,24 @@ def test_group_norm_act_refuses_forward_mode_tangents(which, grad):
     if which == 0:
         with fwd.dual_level(), pytest.raises(NotImplementedError, match="forward-mode"):
             GroupNormAct(2, 8)(fwd.make_dual(args[0], args[0]))
+
+
+def test_orthogonalize_refuses_what_asks_for_a_gradient():
+    """requires_grad under enabled gradients, or a tangent, alone and in a list; detached, or under no_grad, the ordinary checks are next."""
+    from poet_amd import PoetHipError, ops
+    g, p = torch.randn(4, 6), torch.nn.Parameter(torch.randn(4, 6))
+    for arg in (p, [g, p], p * 2, torch.stack([p, p])):
+        with pytest.raises(NotImplementedError, match="no gradient"):
+            ops.orthogonalize(arg)
+    with fwd.dual_level():
+        d = fwd.make_dual(g, g)
+        for arg in (d, [g, d]):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                ops.orthogonalize(arg)
+            with torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
+                ops.orthogonalize(arg)
+    for arg in (g, p.detach(), [g, p.detach()]):
+        with pytest.raises(PoetHipError):                   # (no GPU path for CPU tensors)
+            ops.orthogonalize(arg)
+    with torch.no_grad(), pytest.raises(PoetHipError):
+        ops.orthogonalize(p)
