@@ -456,9 +456,13 @@ int poet_adamw(float* p, const float* g, float* m, float* v, uint16_t* p_bf16, u
                const float* sqnorm, float max_norm, float grad_scale,
                const uint32_t* step_dev /* optional: the step count is read from this device word instead of `step` */,
                const float* lr_scale /* optional: lr multiplier per block of 64 elements, ceil(n/64) floats (the 0.1x group of
-                                        main.py:41,253-271 inside one contiguous range); where its sign bit is set (-0 too) the block
-                                        belongs to another optimiser (poet_muon_step) and is left alone: p, m, v, images */,
+                                        main.py:41,253-271 inside one contiguous range) */,
                void* stream);
+/* ... on the blocks of 64 elements whose byte of `skip` (optional, ceil(n/64) bytes) is 0; the others belong to another optimiser (poet_muon_step) and are
+ * left alone: p, m, v, images. */
+int poet_adamw_blocks(float* p, const float* g, float* m, float* v, uint16_t* p_bf16, uint16_t* p_bf16_lo, int64_t n, float lr, float beta1,
+                      float beta2, float eps, float weight_decay, int step, const float* sqnorm, float max_norm, float grad_scale,
+                      const uint32_t* step_dev, const float* lr_scale, const uint8_t* skip, void* stream);
 /* ------------------------------------------------------------------------------------------------
  * Orthogonalised updates of weight matrices (the Muon optimiser), a LIST of n matrices of any shapes in a few chains of launches.
  * Matrix i is rows[i] x cols[i] (1 .. 2^20 each).  With u the input (orthogonalize) or the update direction (muon_step):
@@ -473,7 +477,7 @@ int poet_adamw(float* p, const float* g, float* m, float* v, uint16_t* p_bf16, u
  * poet_orthogonalize: o[i] = orthogonalised g[i]; row strides ldg / ldo in elements; types POET_F32 / BF16 / F16.
  * poet_muon_step (fp32, contiguous): g' = g grad_scale [x min(1, max_norm / (sqrt(*sqnorm) grad_scale + 1e-6)) with sqnorm];
  *     m <- momentum m + (1 - momentum) g';   u = nesterov ? momentum m + (1 - momentum) g' : m;
- *     p <- p - lr_i wd p - lr_i shape_scale[i] X,   lr_i = lr |*lr_scale[i]|  (optional device words; the sign is the caller's mark);
+ *     p <- p - lr_i wd p - lr_i shape_scale[i] X,   lr_i = lr |*lr_scale[i]|  (optional device words, whose magnitude counts);
  *     p_bf16 / p_bf16_lo (optional lists, as of poet_adamw): bf16 image of p and the bf16 residual.
  * ---------------------------------------------------------------------------------------------- */
 int64_t poet_muon_workspace(const int* rows_host, const int* cols_host, int n);

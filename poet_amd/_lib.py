@@ -86,6 +86,7 @@ _PROTOS = {
     "poet_match_gather": ([vp, vp, vp, vp, i32, i32, vp, vp, vp, vp, vp], i32),
     "poet_sqnorm": ([vp, i64, vp, vp], i32),
     "poet_adamw": ([vp, vp, vp, vp, vp, vp, i64, f32, f32, f32, f32, f32, i32, vp, f32, f32, vp, vp, vp], i32),
+    "poet_adamw_blocks": ([vp, vp, vp, vp, vp, vp, i64, f32, f32, f32, f32, f32, i32, vp, f32, f32, vp, vp, vp, vp], i32),
     "poet_muon_workspace": ([vp, vp, i32], i64),
     "poet_orthogonalize": ([vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, vp, f32, vp, i64, vp], i32),
     "poet_muon_step": ([vp, vp, vp, vp, vp, vp, vp, vp, vp, i32, f32, C.c_double, i32, f32, i32, vp, f32, vp, f32, f32, vp, i64, vp], i32),

@@ -622,14 +622,12 @@ __global__ __launch_bounds__(256) void adamw_kernel(float* __restrict__ p, const
                                                     float* __restrict__ v, uint16_t* __restrict__ pb, uint16_t* __restrict__ pb_lo, int64_t n, float lr,
                                                     float b1, float b2, float eps, float wd, float bc1, float bc2s,
                                                     const float* __restrict__ sqnorm, float max_norm, float gscale,
-                                                    const uint32_t* __restrict__ step_dev, const float* __restrict__ lr_scale, int vec4) {
+                                                    const uint32_t* __restrict__ step_dev, const float* __restrict__ lr_scale,
+                                                    const uint8_t* __restrict__ skip, int vec4) {
     const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
     if (i >= n) return;
-    if (lr_scale) {                                          // per-64-element learning-rate multiplier (LR groups inside one range)
-        const float s = lr_scale[i >> 6];
-        if (__float_as_uint(s) >> 31) return;                // (the sign marks a block of another optimiser's, also at a rate of -0)
-        lr *= s;
-    }
+    if (skip && skip[i >> 6]) return;                        // a block of 64 elements that another optimiser steps
+    if (lr_scale) lr *= lr_scale[i >> 6];                    // per-64-element learning-rate multiplier (LR groups inside one range)
     if (step_dev) {                                          // graph replay: bias corrections from the device-side step
         const float t = (float)(*step_dev);
         bc1 = 1.f - powf(b1, t);
@@ -1117,6 +1115,13 @@ extern "C" int poet_sqnorm(const float* g, int64_t n, float* out, void* stream) 
 extern "C" int poet_adamw(float* p, const float* g, float* m, float* v, uint16_t* p_bf16, uint16_t* p_bf16_lo, int64_t n, float lr, float beta1,
                           float beta2, float eps, float weight_decay, int step, const float* sqnorm, float max_norm,
                           float grad_scale, const uint32_t* step_dev, const float* lr_scale, void* stream) {
+    return poet_adamw_blocks(p, g, m, v, p_bf16, p_bf16_lo, n, lr, beta1, beta2, eps, weight_decay, step, sqnorm, max_norm, grad_scale, step_dev, lr_scale,
+                             nullptr, stream);
+}
+
+extern "C" int poet_adamw_blocks(float* p, const float* g, float* m, float* v, uint16_t* p_bf16, uint16_t* p_bf16_lo, int64_t n, float lr, float beta1,
+                                 float beta2, float eps, float weight_decay, int step, const float* sqnorm, float max_norm,
+                                 float grad_scale, const uint32_t* step_dev, const float* lr_scale, const uint8_t* skip, void* stream) {
     POET_CHECK(p && g && m && v && n > 0 && (step >= 1 || step_dev), POET_ERR_ARG, "adamw: bad args");
     const float bc1 = 1.f - powf(beta1, (float)step);
     const float bc2s = sqrtf(1.f - powf(beta2, (float)step));
@@ -1125,7 +1130,7 @@ extern "C" int poet_adamw(float* p, const float* g, float* m, float* v, uint16_t
     const uintptr_t al16 = (reinterpret_cast<uintptr_t>(p_bf16) | reinterpret_cast<uintptr_t>(p_bf16_lo));
     const int vec4 = ((al & 15) == 0 && (al16 & 7) == 0) ? 1 : 0;
     hipLaunchKernelGGL(adamw_kernel, dim3(cdiv(cdiv(n, 4), 256)), dim3(256), 0, ST, p, g, m, v, p_bf16, p_bf16_lo, n, lr, beta1, beta2, eps,
-                       weight_decay, bc1, bc2s, sqnorm, max_norm, grad_scale, step_dev, lr_scale, vec4);
+                       weight_decay, bc1, bc2s, sqnorm, max_norm, grad_scale, step_dev, lr_scale, skip, vec4);
     POET_LAUNCH_CHECK();
     return POET_OK;
 }

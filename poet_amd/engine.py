@@ -57,7 +57,7 @@ class ParamArena:
     muon: options of ops.MuonPlan.step / its `scale` (or True) -- the weight matrices (MUON_SKIP: not the embeddings and tables, not the
     heads' output layers) step by orthogonalised updates instead of AdamW, their first Adam moment being the momentum; learning rate,
     schedule, clip and weight decay are AdamW's (scale "rms" by default: steps of AdamW's size).  Self-attention's stacked in-projection
-    counts as three matrices.  lr_scale is negative over their blocks (poet_adamw leaves those alone).
+    counts as three matrices.  muon_blocks marks their blocks of 64 elements (poet_adamw_blocks leaves those alone).
     """
     MUON_SKIP = re.compile(r"level_embed|query_embed|^backbone\.|_head\w*\.\d+\.layers\.2\.")
 
@@ -154,10 +154,14 @@ class ParamArena:
         # carries the 0.1x group of sampling_offsets AND the schedule (set_lr rescales it in place, so a replayed graph
         # follows a StepLR exactly like the eager path does; main.py:278 lr_scheduler.step()).
         self.muon_names = [n for n, p, _ in self.entries if p.dim() >= 2 and not self.MUON_SKIP.search(n)] if muon else []
-        for n, p, o in self.entries if muon else ():
-            if n in set(self.muon_names):
-                for i in range(o // ALIGN, (o + p.numel() + ALIGN - 1) // ALIGN):
-                    scale[i] = -scale[i]
+        self.muon_blocks = None
+        if muon:
+            marks = [0] * len(scale)
+            for n, p, o in self.entries:
+                if n in set(self.muon_names):
+                    for i in range(o // ALIGN, (o + p.numel() + ALIGN - 1) // ALIGN):
+                        marks[i] = 1
+            self.muon_blocks = torch.tensor(marks, dtype=torch.uint8, device=dev)
         self.lr_scale_base = torch.tensor(scale, dtype=torch.float32, device=dev)
         self.lr_scale = self.lr_scale_base.clone()
         self.base_lr = self.lr = float(lr)
@@ -191,6 +195,8 @@ class ParamArena:
     def set_lr(self, lr: float):
         """Scheduler entry (the reference's StepLR, main.py:277-278): effective from the next optimiser launch, eager or
         replayed.  The sampling_offsets group keeps its 0.1x ratio."""
+        if self.muon is not None and not lr >= 0:             # (the matrices' learning-rate words count by their magnitude)
+            raise ValueError(f"ParamArena.set_lr: with Muon updates the learning rate must not be negative, got {lr}")
         self.lr = float(lr)
         self.lr_scale.copy_(self.lr_scale_base * (self.lr / self.groups[0][2]))
 
@@ -287,7 +293,7 @@ class ParamArena:
                 ops.adamw(self.flat[a:b], self.grad[a:b], self.m[a:b], self.v[a:b], b - a, lr, self.betas[0], self.betas[1],
                           self.eps, self.weight_decay, self.step_count, sqnorm_buf=sq, max_norm=max_norm, grad_scale=gs,
                           p_bf16=self.flat_bf16[a:b], step_dev=step_dev, lr_scale=self.lr_scale[a // ALIGN:],
-                          p_bf16_lo=self.flat_bf16_lo[a:b])
+                          p_bf16_lo=self.flat_bf16_lo[a:b], skip=None if self.muon_blocks is None else self.muon_blocks[a // ALIGN:])
         if self.muon is not None:
             plan, opts = self.muon
             plan.step(**{"lr": self.groups[0][2], "weight_decay": self.weight_decay, "sqnorm_buf": sq, "max_norm": max_norm, "grad_scale": gs, **opts})

@@ -956,10 +956,11 @@ def sqnorm(g, out):
 
 
 def adamw(p, g, m, v, n, lr, beta1, beta2, eps, wd, step, sqnorm_buf=None, max_norm=0.0, grad_scale=1.0, p_bf16=None, step_dev=None,
-          lr_scale=None, p_bf16_lo=None):
+          lr_scale=None, p_bf16_lo=None, skip=None):
+    """skip: a byte (uint8) per 64 elements, non-zero where the block belongs to another optimiser and is left alone."""
     lib = _lib.load()
-    _lib.check(lib.poet_adamw(_req(p, "p").data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), _ptr(p_bf16), _ptr(p_bf16_lo), n, lr, beta1, beta2,
-                              eps, wd, step, _ptr(sqnorm_buf), max_norm, grad_scale, _ptr(step_dev), _ptr(lr_scale), _stream()), "poet_adamw")
+    _lib.check(lib.poet_adamw_blocks(_req(p, "p").data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), _ptr(p_bf16), _ptr(p_bf16_lo), n, lr, beta1, beta2,
+                                     eps, wd, step, _ptr(sqnorm_buf), max_norm, grad_scale, _ptr(step_dev), _ptr(lr_scale), _ptr(skip), _stream()), "poet_adamw")
 
 
 NS_COEFFS = (3.4445, -4.7750, 2.0315)           # the quintic step of the Muon optimiser: steep at 0, |x| stays within 0.7 .. 1.2 afterwards
