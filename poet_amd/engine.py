@@ -54,7 +54,7 @@ class ParamArena:
     Parameters that never receive a gradient in this configuration (transformer.reference_points.*
     in bbox mode; the reason the reference needs find_unused_parameters=True) stay outside, exactly as
     torch.optim.AdamW skips parameters whose .grad is None.
-    muon: options of ops.MuonPlan.step / its `scale` (or True) -- the weight matrices (MUON_SKIP: not the embeddings and tables, not the
+    muon: options of ops.MuonPlan.step / its `scale` as a dict (True or an empty one: the defaults; None or False: off) -- the weight matrices (MUON_SKIP: not the embeddings and tables, not the
     heads' output layers) step by orthogonalised updates instead of AdamW, their first Adam moment being the momentum; learning rate,
     schedule, clip and weight decay are AdamW's (scale "rms" by default: steps of AdamW's size).  Self-attention's stacked in-projection
     counts as three matrices.  muon_blocks marks their blocks of 64 elements (poet_adamw_blocks leaves those alone).
@@ -63,6 +63,7 @@ class ParamArena:
 
     def __init__(self, model: nn.Module, lr=2e-4, lr_proj_mult=0.1, proj_names=("reference_points", "sampling_offsets"),
                  weight_decay=1e-4, betas=(0.9, 0.999), eps=1e-8, exclude=("transformer.reference_points",), lr_backbone_mult=0.1, muon=None):
+        muon = {} if muon is True else dict(muon) if muon or isinstance(muon, dict) else None
         named = [(n, p) for n, p in model.named_parameters() if p.requires_grad and not any(e in n for e in exclude)]
         # Only the hot path's own parameters live here (their gradients are written by the HIP backward programs).  Anything
         # else that is trainable -- e.g. a real backbone, which the reference trains at lr_backbone (main.py:253-271) -- would
@@ -153,9 +154,9 @@ class ParamArena:
         # Learning rate = base_lr (a host scalar baked into captured graphs) x this per-64-element DEVICE table: the table
         # carries the 0.1x group of sampling_offsets AND the schedule (set_lr rescales it in place, so a replayed graph
         # follows a StepLR exactly like the eager path does; main.py:278 lr_scheduler.step()).
-        self.muon_names = [n for n, p, _ in self.entries if p.dim() >= 2 and not self.MUON_SKIP.search(n)] if muon else []
+        self.muon_names = [n for n, p, _ in self.entries if p.dim() >= 2 and not self.MUON_SKIP.search(n)] if muon is not None else []
         self.muon_blocks = None
-        if muon:
+        if muon is not None:
             marks = [0] * len(scale)
             for n, p, o in self.entries:
                 if n in set(self.muon_names):
@@ -173,9 +174,8 @@ class ParamArena:
         self.step_word = torch.zeros(1, dtype=torch.int32, device=dev)       # device copy of step_count (graph replays bump it)
         self.world = 1
         self.muon = None
-        if muon:
-            opts = {} if muon is True else dict(muon)
-            self.muon = (self._muon_plan(opts.pop("scale", "rms")), opts)
+        if muon is not None:
+            self.muon = (self._muon_plan(muon.pop("scale", "rms")), muon)
         # model.load_state_dict copies into the fp32 arena views in place; the bf16 operand shadow must follow
         model.register_load_state_dict_post_hook(lambda module, incompatible: self.refresh_shadow())
 

@@ -42,3 +42,21 @@ def test_orthogonalize_refuses_what_asks_for_a_gradient():
             ops.orthogonalize(arg)
     with torch.no_grad(), pytest.raises(PoetHipError):
         ops.orthogonalize(p)
+
+
+def arena(**kw):
+    """A parameter arena over one encoder-like Linear, on the CPU (where Muon is refused, after its options have been looked at)."""
+    from poet_amd import ParamArena
+    m = torch.nn.Module()
+    m.transformer = torch.nn.Module()
+    m.transformer.encoder = torch.nn.Linear(8, 4)
+    return ParamArena(m, **kw)
+
+
+def test_an_empty_dict_of_muon_options_means_the_defaults():
+    for off in (None, False):
+        a = arena(muon=off)
+        assert a.muon is None and a.muon_names == [] and a.muon_blocks is None
+    for on in (True, {}, dict(momentum=0.9)):
+        with pytest.raises(ValueError, match="GPU"):
+            arena(muon=on)
