@@ -4,6 +4,7 @@ and an op-for-op PyTorch counterpart of the reference's matcher/loss (kept uncha
 """
 from __future__ import annotations
 
+import inspect
 import math
 import os
 import re
@@ -64,6 +65,7 @@ class ParamArena:
     def __init__(self, model: nn.Module, lr=2e-4, lr_proj_mult=0.1, proj_names=("reference_points", "sampling_offsets"),
                  weight_decay=1e-4, betas=(0.9, 0.999), eps=1e-8, exclude=("transformer.reference_points",), lr_backbone_mult=0.1, muon=None):
         muon = {} if muon is True else dict(muon) if muon or isinstance(muon, dict) else None
+        self._check_muon(muon)
         named = [(n, p) for n, p in model.named_parameters() if p.requires_grad and not any(e in n for e in exclude)]
         # Only the hot path's own parameters live here (their gradients are written by the HIP backward programs).  Anything
         # else that is trainable -- e.g. a real backbone, which the reference trains at lr_backbone (main.py:253-271) -- would
@@ -179,6 +181,19 @@ class ParamArena:
         # model.load_state_dict copies into the fp32 arena views in place; the bf16 operand shadow must follow
         model.register_load_state_dict_post_hook(lambda module, incompatible: self.refresh_shadow())
 
+    @staticmethod
+    def _check_muon(opts):
+        """Refuses options of the Muon step that its first call would refuse."""
+        if opts is None:
+            return
+        known = ["scale"] + [k for k in inspect.signature(ops.MuonPlan.step).parameters if k != "self"]
+        unknown = [k for k in opts if k not in known]
+        if unknown:
+            raise ValueError(f"ParamArena: unknown Muon options {unknown}, known are {known}")
+        if opts.get("scale", "rms") not in ops.MUON_SCALES:
+            raise ValueError(f"ParamArena: Muon's scale must be one of {sorted(ops.MUON_SCALES)}, got {opts['scale']!r}")
+        ops._muon_options(**{k: v for k, v in opts.items() if k in ("momentum", "steps", "coeffs", "eps")})
+
     def _muon_plan(self, scale):
         if not self.flat.is_cuda:
             raise ValueError("ParamArena: Muon updates need the model on the GPU")
@@ -281,22 +296,22 @@ class ParamArena:
     def step(self, max_norm: float = 0.1, step_dev=None):
         """clip_grad_norm_(max_norm) + AdamW (engine.py:77-81) on the flat arenas.  With `step_dev` (a device word) the
         step count / bias corrections are read on the device, so the launch sequence can be replayed from a hipGraph."""
-        self.step_count += 1
         gs = 1.0 / self.world
         sq = None
         if max_norm > 0:
             ops.zero_(self.sq) if self.sq.is_cuda else self.sq.zero_()
             ops.sqnorm(self.grad, self.sq)
             sq = self.sq
+        if self.muon is not None:                             # (first: what it refuses, it refuses before anything has changed)
+            plan, opts = self.muon
+            plan.step(**{"lr": self.groups[0][2], "weight_decay": self.weight_decay, "sqnorm_buf": sq, "max_norm": max_norm, "grad_scale": gs, **opts})
+        self.step_count += 1
         for a, b, lr in self.groups:
             if b > a:
                 ops.adamw(self.flat[a:b], self.grad[a:b], self.m[a:b], self.v[a:b], b - a, lr, self.betas[0], self.betas[1],
                           self.eps, self.weight_decay, self.step_count, sqnorm_buf=sq, max_norm=max_norm, grad_scale=gs,
                           p_bf16=self.flat_bf16[a:b], step_dev=step_dev, lr_scale=self.lr_scale[a // ALIGN:],
                           p_bf16_lo=self.flat_bf16_lo[a:b], skip=None if self.muon_blocks is None else self.muon_blocks[a // ALIGN:])
-        if self.muon is not None:
-            plan, opts = self.muon
-            plan.step(**{"lr": self.groups[0][2], "weight_decay": self.weight_decay, "sqnorm_buf": sq, "max_norm": max_norm, "grad_scale": gs, **opts})
 
     def grad_norm(self) -> torch.Tensor:
         return torch.sqrt(self.sq[0]) / self.world

@@ -1084,6 +1084,17 @@ def orthogonalize(g, out=None, steps=5, coeffs=NS_COEFFS, eps=1e-7):
 MUON_SCALES = {"spectral": lambda r, c: max(1.0, r / c) ** 0.5, "rms": lambda r, c: 0.2 * max(r, c) ** 0.5}
 
 
+def _muon_options(momentum=0.95, steps=5, coeffs=NS_COEFFS, eps=1e-7):
+    """Checks the options of a Muon step (the C entry point refuses coefficients that leave the iteration's range); the coefficients as it takes them."""
+    if not 0.0 <= momentum < 1.0:
+        raise ValueError(f"poet_amd: momentum must be in [0, 1), got {momentum}")
+    if not 1 <= steps <= 16:
+        raise ValueError(f"poet_amd: 1 .. 16 steps, got {steps}")
+    if not eps >= 0.0:
+        raise ValueError(f"poet_amd: eps must not be negative, got {eps}")
+    return _ns_coeffs(coeffs, steps)
+
+
 class MuonPlan:
     """A list of fp32 weight matrices with their gradients and moments (more than two dimensions: rows x the rest), checked once, for the
     updates of a training run: `plan.step(lr, ...)` = muon_step on them.  The tensors are held, and have to stay where they are.
@@ -1125,16 +1136,12 @@ class MuonPlan:
         self.device, self.held = dev, (params, grads, moments, p_bf16, p_bf16_lo, lr_scale)
 
     def step(self, lr, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5, coeffs=NS_COEFFS, eps=1e-7, sqnorm_buf=None, max_norm=0.0, grad_scale=1.0):
-        if not 0.0 <= momentum < 1.0:
-            raise ValueError(f"poet_amd: momentum must be in [0, 1), got {momentum}")
-        if not 1 <= steps <= 16:
-            raise ValueError(f"poet_amd: 1 .. 16 steps, got {steps}")
+        cf = _muon_options(momentum, steps, coeffs, eps)
         if self.n == 0:
             return
         if sqnorm_buf is not None and (sqnorm_buf.dtype != torch.float32 or sqnorm_buf.device != self.device):
             raise ValueError("poet_amd: sqnorm_buf is an fp32 tensor on the parameters' device")
         lib = _lib.load()
-        cf = _ns_coeffs(coeffs, steps)
         with _on_device(self.device) as stream:
             ws = _muon_ws(lib, self.rows, self.cols, self.n, self.device)
             _lib.check(lib.poet_muon_step(*self.arrays, lr, momentum, int(nesterov), weight_decay, steps, cf, eps, _ptr(sqnorm_buf), max_norm, grad_scale,

@@ -60,3 +60,15 @@ def test_an_empty_dict_of_muon_options_means_the_defaults():
     for on in (True, {}, dict(momentum=0.9)):
         with pytest.raises(ValueError, match="GPU"):
             arena(muon=on)
+
+
+def test_muon_options_are_checked_when_the_arena_is_built():
+    """Unknown names and values that the first step would refuse, before a parameter is moved; a refusal further on is of the device only."""
+    for bad in (dict(beta=0.9), dict(momentun=0.9), dict(momentum=1.0), dict(momentum=-0.1), dict(momentum=float("nan")), dict(steps=0), dict(steps=17),
+                dict(eps=-1.0), dict(coeffs=(1.0, 2.0)), dict(steps=3, coeffs=[(3.0, -3.2, 1.2)] * 2), dict(scale="max"), dict(self=1)):
+        with pytest.raises(ValueError) as e:
+            arena(muon=bad)
+        assert "GPU" not in str(e.value), bad
+    for good in (dict(momentum=0.0, nesterov=False, steps=3, coeffs=[(3.0, -3.2, 1.2)] * 3, eps=0.0, scale="spectral"), dict(lr=0.02, weight_decay=0.0)):
+        with pytest.raises(ValueError, match="GPU"):
+            arena(muon=good)
