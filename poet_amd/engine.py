@@ -56,11 +56,11 @@ class ParamArena:
     in bbox mode; the reason the reference needs find_unused_parameters=True) stay outside, exactly as
     torch.optim.AdamW skips parameters whose .grad is None.
     muon: options of ops.MuonPlan.step / its `scale` as a dict (True or an empty one: the defaults; None or False: off) -- the weight matrices (MUON_SKIP: not the embeddings and tables, not the
-    heads' output layers) step by orthogonalised updates instead of AdamW, their first Adam moment being the momentum; learning rate,
+    output layers: the heads' last ones and, in learned mode, the 2-row reference points) step by orthogonalised updates instead of AdamW, their first Adam moment being the momentum; learning rate,
     schedule, clip and weight decay are AdamW's (scale "rms" by default: steps of AdamW's size).  Self-attention's stacked in-projection
     counts as three matrices.  muon_blocks marks their blocks of 64 elements (poet_adamw_blocks leaves those alone).
     """
-    MUON_SKIP = re.compile(r"level_embed|query_embed|^backbone\.|_head\w*\.\d+\.layers\.2\.")
+    MUON_SKIP = re.compile(r"level_embed|query_embed|^backbone\.|_head\w*\.\d+\.layers\.2\.|^transformer\.reference_points\.")
 
     def __init__(self, model: nn.Module, lr=2e-4, lr_proj_mult=0.1, proj_names=("reference_points", "sampling_offsets"),
                  weight_decay=1e-4, betas=(0.9, 0.999), eps=1e-8, exclude=("transformer.reference_points",), lr_backbone_mult=0.1, muon=None):
