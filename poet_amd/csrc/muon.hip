@@ -1500,6 +1500,7 @@ int layout(const int* rows, const int* cols, const int* order, int first, int n,
         if (rec) rec[count] = r;
         ++count;
     }
+    if (group > 0 && group <= MAX_D && (int64_t)count * NW_T >= 1ll << 32) return -1;      // (a workgroup each: more threads than a launch can have)
     L.count = count;
     L.parts = (int)parts;
     L.plane_elems = planes;
@@ -1714,7 +1715,7 @@ int run_job(const char* what, const Job& j, void* ws, int64_t ws_bytes, void* st
     POET_CHECK(ranges(j.coeffs, j.steps, S), POET_ERR_ARG, "%s: these coefficients leave the range the iteration can hold", what);
     const Choice T = tiles_of(j.rows, j.cols, j.n);
     const int64_t need = workspace_of(j.rows, j.cols, j.n, T);
-    POET_CHECK(need >= 0, POET_ERR_UNSUPPORTED, "%s: too many tiles", what);
+    POET_CHECK(need >= 0, POET_ERR_UNSUPPORTED, "%s: too many matrices or tiles", what);
     POET_CHECK(ws && ((uintptr_t)ws % 256) == 0 && ws_bytes >= need, POET_ERR_ARG, "%s: workspace of %lld bytes needed (256-byte aligned), %lld given", what,
                (long long)need, (long long)ws_bytes);
     struct Ints {
@@ -1807,7 +1808,7 @@ extern "C" int64_t poet_muon_workspace(const int* rows_host, const int* cols_hos
     for (int i = 0; i < n; ++i)
         POET_CHECK(rows_host[i] > 0 && cols_host[i] > 0 && rows_host[i] <= (1 << 20) && cols_host[i] <= (1 << 20), POET_ERR_ARG, "muon_workspace: matrix %d is %d x %d", i, rows_host[i], cols_host[i]);
     const int64_t need = workspace_of(rows_host, cols_host, n, tiles_of(rows_host, cols_host, n));
-    POET_CHECK(need >= 0, POET_ERR_UNSUPPORTED, "muon_workspace: too many tiles");
+    POET_CHECK(need >= 0, POET_ERR_UNSUPPORTED, "muon_workspace: too many matrices or tiles");
     return need;
 }
 

@@ -1,4 +1,6 @@
 """What the GroupNorm + activation and orthogonalisation operators refuse before they look at a device."""
+import ctypes
+
 import pytest
 import torch
 import torch.autograd.forward_ad as fwd
@@ -72,3 +74,14 @@ def test_muon_options_are_checked_when_the_arena_is_built():
     for good in (dict(momentum=0.0, nesterov=False, steps=3, coeffs=[(3.0, -3.2, 1.2)] * 3, eps=0.0, scale="spectral"), dict(lr=0.02, weight_decay=0.0)):
         with pytest.raises(ValueError, match="GPU"):
             arena(muon=good)
+
+
+def test_more_narrow_matrices_than_a_launch_has_workgroups_are_refused():
+    """2^23 workgroups of 512 threads are 2^32: refused with the workspace, before another group of the list has been updated."""
+    from poet_amd import _lib
+    lib, n = _lib.load(), 1 << 23
+    dims = (ctypes.c_int * (n + 1))(*[2] * (n + 1))
+    assert lib.poet_muon_workspace(dims, dims, n - 1) > 0
+    assert lib.poet_muon_workspace(dims, dims, n) < 0 and b"too many matrices" in lib.poet_hip_last_error()
+    dims[n] = 300
+    assert lib.poet_muon_workspace(dims, dims, n + 1) < 0
