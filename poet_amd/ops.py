@@ -598,6 +598,11 @@ def _apart(a, an, ar, b, bn, br, N, HW, C, name):
     raise ValueError(f"poet_amd: {name} overlaps an input that it is not")
 
 
+def _params_apart(dgamma, dbeta, gamma, beta, size):
+    """Whether the two gradients' `size` bytes share none with each other or with the parameters (other workgroups read these meanwhile)."""
+    return abs(dgamma - dbeta) >= size and all(abs(d - p) >= size for d in (dgamma, dbeta) for p in (gamma, beta))
+
+
 def _gna_args(x, params, G, act):
     """Checks what both directions share: (device, N, HW, C, activation code)."""
     if not x.is_cuda:
@@ -662,8 +667,8 @@ def groupnorm_act_bwd(dy, x, stats, gamma, beta, G, act="none", dx=None, dgamma=
         raise ValueError("poet_amd: dx has x's type, and dy, dx live on x's device")
     if not (stats.dtype is torch.float32 and stats.device == dev and stats.is_contiguous() and stats.numel() == 2 * N * G):
         raise ValueError("poet_amd: stats must be the contiguous fp32 (N, G, 2) tensor of the forward pass")
-    if (dgamma is None) != (dbeta is None) or dgamma is not None and C > 0 and dgamma.data_ptr() == dbeta.data_ptr():
-        raise ValueError("poet_amd: dgamma and dbeta go together, and are two tensors")
+    if (dgamma is None) != (dbeta is None) or dgamma is not None and not _params_apart(dgamma.data_ptr(), dbeta.data_ptr(), gamma.data_ptr(), beta.data_ptr(), 4 * C):
+        raise ValueError("poet_amd: dgamma and dbeta go together, and are two tensors apart from each other and from gamma and beta")
     xd, yd = dcode(x), dcode(dy)
     if N == 0 or HW == 0 or dx is None and dgamma is None:
         if dgamma is not None and not accumulate:

@@ -68,3 +68,18 @@ def test_squares_beyond_fp32_are_not_finite(ops, HW, size):
     ops.groupnorm_act_fwd(big, w, b, y, 8, "silu")
     r = ref(big, w, b, 8, "silu", 1e-5)
     check(y, r["y"], r["tol_y"], "deviations of 1e15")
+
+
+def test_overlapping_parameter_gradients_are_refused(ops):
+    """dgamma / dbeta on each other, or on gamma / beta, which other workgroups read meanwhile: refused, nothing written."""
+    x, w, b, dy = make(2, 50, 64, torch.float32)
+    stats = torch.empty(2, 8, 2, device="cuda")
+    ops.groupnorm_act_fwd(x, w, b, torch.empty_like(x), 8, "silu", stats=stats)
+    buf = torch.full((200,), 7.0, device="cuda")
+    w0, b0 = w.clone(), b.clone()
+    for dw, db in ((buf[:64], buf[:64]), (buf[:64], buf[63:127]), (w, buf[:64]), (buf[:64], w), (b, buf[:64]), (buf[:64], b)):
+        with pytest.raises(ValueError):
+            ops.groupnorm_act_bwd(dy, x, stats, w, b, 8, "silu", dgamma=dw, dbeta=db)
+    assert (buf == 7).all() and torch.equal(w, w0) and torch.equal(b, b0)
+    ops.groupnorm_act_bwd(dy, x, stats, w, b, 8, "silu", dgamma=buf[:64], dbeta=buf[64:128])
+    assert (buf[128:] == 7).all() and (buf[:128] != 7).all()

@@ -85,3 +85,11 @@ def test_more_narrow_matrices_than_a_launch_has_workgroups_are_refused():
     assert lib.poet_muon_workspace(dims, dims, n) < 0 and b"too many matrices" in lib.poet_hip_last_error()
     dims[n] = 300
     assert lib.poet_muon_workspace(dims, dims, n + 1) < 0
+
+
+def test_parameter_gradients_apart_from_each_other_and_from_the_parameters():
+    from poet_amd.ops import _params_apart
+    assert _params_apart(0, 256, 512, 768, 256) and _params_apart(768, 512, 0, 0, 256)
+    for a in ((0, 0, 512, 768), (0, 252, 512, 768), (0, 256, 512 - 4, 768), (512, 0, 512, 768), (0, 768 + 4, 512, 768), (600, 0, 4096, 380)):
+        assert not _params_apart(*a, 256), a
+    assert _params_apart(0, 0, 0, 0, 0)                     # (no channels)
