@@ -22,9 +22,10 @@
 // A few groups of an image whose rows fit a workgroup's registers need ONE launch and one read (gna_fit_kernel below).
 // Nothing is accumulated with atomics: results do not depend on the order of workgroups.
 //
-// Measured: 8 x 19200 x 256 fp16 + GELU forward 61 us, 51 with x still in the cache (1 17.9, 2 4.9, 3 32.7: 4.8 TB/s in 3); the same in fp32,
-// forward and backward, 250 us (31.7 + 5 + 54.9, 70.2 + 5.1 + 78.9: 5.7 and 6.0 TB/s in 3, what the cache kept included); 16 x 4800 x 256
-// bf16 + SiLU 23 us forward in one launch (3.4 TB/s: one workgroup of 1024 a CU, the load, the sums and the store one after the other).
+// Measured: 8 x 19200 x 256 fp16 + GELU forward 63 us, 53 with x still in the cache (1 19.6, 2 4.6, 3 32.3: 4.9 TB/s in 3; the mean's correction costs
+// 1.7 in 1); the same in fp32, forward and backward, 251 us (32.7 + 4.8 + 54.4, 70.0 + 4.9 + 78.7: 5.8 and 6.0 TB/s in 3, what the cache kept
+// included); 16 x 4800 x 256 bf16 + SiLU 22 us forward in one launch (3.6 TB/s: one workgroup of 1024 a CU, the load, the sums and the store one
+// after the other; 0.8 of it the correction).
 #include "common.cuh"
 
 #include <type_traits>
@@ -448,7 +449,7 @@ template <typename TX, typename TY, int V, int ACT> __global__ __launch_bounds__
 
 // ---- whole images in registers: one launch ------------------------------------------------------------------------------------
 // Where the rows of a few groups of an image fit a workgroup's registers (up to 192 KB), x is read once, the statistics are plain two-pass
-// sums over registers, and a forward pass is ONE launch: what small calls cost is launches, and a level of 4800 rows saves its re-read.  Needs
+// sums over registers (the mean corrected by the deviations from it), and a forward pass is ONE launch: what small calls cost is launches, and a level of 4800 rows saves its re-read.  Needs
 // whole vectors in a group.  A workgroup takes gpw neighbouring groups: lanes l of a row's LPR = gpw * cpg / V, rows threadIdx / LPR + u RP.
 template <typename T, int V> struct Raw {
     u32x4_t w;

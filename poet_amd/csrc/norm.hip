@@ -18,7 +18,8 @@ constexpr int LN_MAXIT = 4;   // d <= 1024
 template <typename T> struct is_f16 { static constexpr bool value = false; };
 template <> struct is_f16<f16_t> { static constexpr bool value = true; };
 // sum + a b in two roundings: these sums keep the bits they had when their products were packed in pairs (a pair was multiplied and added, a
-// lone product fused, as the vectoriser happened to decide)
+// lone product fused, as the vectoriser happened to decide).  Fused, the bf16 forward of the smallest GELU configuration is 1.73e-2 off where this is 1.19e-2;
+// a training step takes as long either way (11.94 - 11.98 ms, fused 11.95 - 12.01: LayerNorm waits for memory)
 __device__ __forceinline__ float add_mul(float sum, float a, float b) {
 #pragma clang fp contract(off)
     return sum + a * b;
