@@ -66,6 +66,8 @@ class ParamArena:
                  weight_decay=1e-4, betas=(0.9, 0.999), eps=1e-8, exclude=("transformer.reference_points",), lr_backbone_mult=0.1, muon=None):
         muon = {} if muon is True else dict(muon) if muon or isinstance(muon, dict) else None
         self._check_muon(muon)
+        if muon is not None and not lr >= 0:                  # (set_lr's factor, which the matrices take by its magnitude, would turn its sign)
+            raise ValueError(f"ParamArena: with Muon updates the learning rate must not be negative, got {lr}")
         named = [(n, p) for n, p in model.named_parameters() if p.requires_grad and not any(e in n for e in exclude)]
         # Only the hot path's own parameters live here (their gradients are written by the HIP backward programs).  Anything
         # else that is trainable -- e.g. a real backbone, which the reference trains at lr_backbone (main.py:253-271) -- would

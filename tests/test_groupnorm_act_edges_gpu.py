@@ -15,8 +15,8 @@ CONSTANT = [(41, 8), (47, 8), (55, 1), (61, 12), (83, 12), (300, 8), (700, 3), (
 @pytest.mark.parametrize("dtype", list(DTYPES))
 @pytest.mark.parametrize("HW,cpg", CONSTANT)
 def test_constant_groups_are_exactly_beta(ops, HW, cpg, dtype):
-    """x = c over a group: the mean is c (each fp32 sum of n equal deviations j ulp(c), n j < 2^24, is exact, and so is its quotient by n), the
-    variance 0, h = 0 and z = beta, whatever 1 / sqrt(eps) = 316 would make of a mean one ulp off.  The stored statistics say the same."""
+    """x = c over a group: the mean is c (a first mean is some ulps off; the n equal deviations from it, their sum and its quotient by n are right to
+    2^-20 of those ulps, so the corrected mean rounds to c), the variance 0, h = 0 and z = beta, whatever 1 / sqrt(eps) = 316 would make of a mean one ulp off.  The stored statistics say the same."""
     dt, G = DTYPES[dtype], 4
     C = G * cpg
     for k, v in enumerate((1000.0, 0.3, -77.77)):

@@ -93,3 +93,10 @@ def test_parameter_gradients_apart_from_each_other_and_from_the_parameters():
     for a in ((0, 0, 512, 768), (0, 252, 512, 768), (0, 256, 512 - 4, 768), (512, 0, 512, 768), (0, 768 + 4, 512, 768), (600, 0, 4096, 380)):
         assert not _params_apart(*a, 256), a
     assert _params_apart(0, 0, 0, 0, 0)                     # (no channels)
+
+
+def test_a_negative_rate_is_refused_with_muon():
+    for lr in (-1e-3, float("nan")):
+        with pytest.raises(ValueError, match="negative"):
+            arena(lr=lr, muon=True)
+    assert arena(lr=-1e-3).lr == -1e-3
